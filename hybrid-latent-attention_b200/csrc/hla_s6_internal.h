@@ -76,6 +76,8 @@ struct HistoryPlan {
 
 int history_plan(const HistoryArgs& a, HistoryPlan* plan);
 int history_split(const HistoryArgs& a, const HistoryPlan& plan, cudaStream_t stream);
+// The split over a 4-bit cache (q4_history.cu): a.scale includes the K tensor scale, a.cache_st_block counts bytes.
+int q4_history_split(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, cudaStream_t stream);
 int history_reduce_strided(const HistoryArgs& a, const HistoryPlan& plan, const uint8_t* empty, void* out,
                            int64_t o_st, int64_t o_sh, float* out_f32, float* lse, int64_t lse_st, int64_t lse_sh,
                            cudaStream_t stream);

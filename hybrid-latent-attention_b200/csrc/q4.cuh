@@ -1,0 +1,97 @@
+// The 4-bit format shared by the latent cache (q4_history.cu, q4_rows.cu) and the weights (q4_linear.cu).
+//
+// A group of 32 consecutive columns of a row shares one e4m3 scale s; a value is (n - 8) * s * ts with the
+// code n in 1..15 and one tensor scale ts.  (n - 8) * s has at most 3 + 4 significant bits, so it is exact
+// in bf16 (8 bits): the kernels feed the tensor cores bf16 values without a rounding, and ts is applied to
+// the fp32 accumulators.  Codes travel in 32-bit words of 8 columns, nibble i column 2i and nibble i + 4
+// column 2i + 1: one shift and one and-or leave two neighbouring columns in the two halves of a register.
+//
+// A latent cache page is page / 16 tiles of 16 rows, 17 W bytes each (W = latent width, G = W / 32 groups):
+//   K codes  [G][16 rows][16 B]    a row's group is one 16-byte chunk
+//   V codes  [W / 8][16 rows][4 B] the rows of 8 columns side by side: V is contracted over rows
+//   K scales [16 rows][G]   V scales [G][16 rows]
+// Every byte belongs to one row, so rows are committed independently of one another.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace hla {
+
+constexpr int kQ4Group = 32;  // columns that share a scale
+
+// A packed weight [N, K] is [N / 16][K / 128] tiles (zero padded) of 16 rows x 128 columns: codes
+// [2][32 lanes][16 B], scales [32 lanes][2], lane 4 g + c and half h holding row 8 h + g, columns 32 c .. -
+// the A fragment of mma.m16n8k16 read straight from global memory, one 16-byte load per half.
+constexpr int kQ4WeightTile = 1088;
+
+struct Q4Tile {  // byte offsets inside a 16-row tile of latent width W
+  int W;
+  __host__ __device__ explicit Q4Tile(int w) : W(w) {}
+  __host__ __device__ int bytes() const { return 17 * W; }
+  __host__ __device__ int k_codes(int group, int row) const { return group * 256 + row * 16; }
+  __host__ __device__ int v_codes(int octet, int row) const { return 8 * W + octet * 64 + row * 4; }
+  __host__ __device__ int k_scale(int row, int group) const { return 16 * W + row * (W / kQ4Group) + group; }
+  __host__ __device__ int v_scale(int group, int row) const { return 16 * W + W / 2 + group * 16 + row; }
+};
+
+__device__ __forceinline__ uint32_t bf2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Two e4m3 bytes (low 16 bits of v) -> bf16x2 (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_bf2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  return pack_bf16(f.x, f.y);
+}
+
+// A scale pair as the dequantiser wants it: s and -24 s.
+struct Q4Scale {
+  uint32_t s, c;
+  __device__ __forceinline__ explicit Q4Scale(uint32_t s2) : s(s2), c(bf2_mul(s2, 0xc1c0c1c0u)) {}  // -24
+};
+
+// (n - 8) * s of nibbles i and i + 4 of a word: the nibbles moved to bits 3..6 of each half are the top
+// mantissa bits of a bf16 in [16, 32), i.e. 16 + n, and (16 + n) s - 24 s = (n - 8) s, exact at every
+// step (24 s has 6 significant bits).
+template <int I>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w, const Q4Scale& s) {
+  const uint32_t sh = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return bf2_fma((sh & 0x00780078u) | 0x41804180u, s.s, s.c);
+}
+
+// Scale byte of a group: e4m3(amax / (7 ts)), a true division so that ties fall as the format says.
+__device__ __forceinline__ uint32_t q4_scale_byte(float amax, float ts) {
+  return __nv_cvt_float_to_fp8(__fdiv_rn(amax, 7.f * ts), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float q4_scale_value(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+// Code of x in a group whose step is s * ts (0: a group of zeros).  |x| / step < 7.5 except where the scale
+// saturated or was rounded in e4m3's subnormal range, hence the clamp; an infinity takes
+// the group's largest code, a NaN code 1 (the stored rows hold no NaN).
+__device__ __forceinline__ uint32_t q4_code(float x, float step) {
+  if (!(step > 0.f)) return 8u;
+  return static_cast<uint32_t>(8 + static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x, step)), -7.f), 7.f)));
+}
+// The word of 8 columns' codes.
+__device__ __forceinline__ uint32_t q4_word(const uint32_t (&n)[8]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= (n[2 * i] << (4 * i)) | (n[2 * i + 1] << (16 + 4 * i));
+  return w;
+}
+__device__ __forceinline__ int q4_code_at(uint32_t w, int col) {
+  return static_cast<int>((w >> (4 * (col >> 1) + 16 * (col & 1))) & 15u) - 8;
+}
+
+}  // namespace hla

@@ -1,0 +1,216 @@
+"""4-bit latent cache and 4-bit weights of the S6 path on B200.
+
+The bf16 ops of ``s6_ops`` / ``s6_layer`` / ``cache_export`` in their 4-bit form: rows of 17/16 bytes per latent
+column instead of 4 (544 bytes for a 512-wide latent, bf16 2048), weights of 17/32 bytes per value.
+
+* ``new_cache``          an empty 4-bit cache ``[num_blocks, 1, page, 17 * width / 16]`` (uint8)
+* ``commit_rows``        rotate, quantise and scatter the rows of a step (``hla_s6_commit_rows``'s 4-bit form;
+                         s6_layer.py:135-147 + unified_kv_cache_update, ouro_latent.py:127-129)
+* ``history_attention``  the paged reader (s6_ops.py:117-161); ``s6_ops.history_attention`` calls it for a uint8
+                         cache, ``s6_layer.attend`` and ``ouro_attention`` take such caches too
+* ``gather_rows`` / ``gather_slots``  rows back as bf16 (the export's gather, cache_export.py:160-174)
+* ``quantize_weight`` / ``linear``    packed weights, and ``x . w^T`` with them (register.py:45-61,
+                         ouro_latent.py:109-110, 130)
+
+Format: a group of 32 consecutive columns shares one e4m3 scale ``s``; a value is ``(n - 8) * s * ts`` with a
+code ``n`` in 1..15 and one tensor scale ``ts``: ``s = e4m3(amax / (7 ts))``, ``n = 8 + rint(x / (s ts))``.  The
+byte layout is in include/hla_s6.h.  The tensor scales (``k_scale`` / ``v_scale`` of a cache, ``scale`` of a
+weight) are not stored with the codes: every call on the same data passes the same values.  A scale covers groups
+with amax between 0.11 ts and 3136 ts at full precision; ``tensor_scale`` picks one.
+
+As everywhere in this package the ops run on CUDA tensors only, on the current stream of their device, never
+synchronise and can be captured in CUDA graphs.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+GROUP = 32
+WEIGHT_TILE_BYTES = 1088   # HLA_S6_Q4_WEIGHT_TILE_BYTES
+BF16 = torch.bfloat16
+
+
+def row_bytes(width):
+    """Bytes of one 4-bit cache row (K and V) of latent width ``width``."""
+    return 17 * width // 16
+
+
+def cache_width(cache):
+    """Latent width of a 4-bit cache."""
+    return cache.shape[-1] * 16 // 17
+
+
+def tensor_scale(amax):
+    """The smallest power of two that lets the largest group scale reach e4m3's range for values up to ``amax``
+    (a float); a power of two keeps every stored value exact in bf16."""
+    return 2.0 ** math.ceil(math.log2(amax / (7 * 448))) if amax > 0 else 1.0
+
+
+def new_cache(num_blocks, page, width, device='cuda'):
+    """A zeroed 4-bit latent cache (every row reads as zeros)."""
+    if width not in (256, 512, 1024) or page < 16 or page % 16:
+        raise ValueError('a 4-bit latent cache has width 256, 512 or 1024 and a page of a multiple of 16 rows')
+    return torch.zeros(num_blocks, 1, page, row_bytes(width), dtype=torch.uint8, device=device)
+
+
+def _on_device(*tensors):
+    """Every tensor on one CUDA device, which is made current for the launch."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != dev):
+            raise ValueError('S6 4-bit ops take CUDA tensors of one device (no CPU path exists)')
+    return torch.cuda.device(dev)
+
+
+def _cache_geometry(cache, width):
+    """``(num_blocks, block stride in bytes, page)`` of a 4-bit cache of latent width ``width``."""
+    if cache.dim() != 4 or cache.shape[1] != 1 or cache.shape[-1] != row_bytes(width) or cache.dtype != torch.uint8:
+        raise ValueError(f'a 4-bit latent cache of width {width} must be uint8 [num_blocks, 1, page, '
+                         f'{row_bytes(width)}], got {cache.dtype} {tuple(cache.shape)}')
+    if cache.stride(-1) != 1 or cache.stride(2) != cache.shape[-1]:
+        raise ValueError('the bytes of a 4-bit cache page must be contiguous')
+    return cache.shape[0], cache.stride(0), cache.shape[2]
+
+
+def _block_table(table):
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(-1) != 1:
+        raise ValueError('block_table must be int32 [rows, max_blocks] with a unit last-dim stride')
+
+
+def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, k_scale=1.0, v_scale=1.0,
+                      empty=None, error_flag=None):
+    """``s6_ops.history_attention`` over a 4-bit cache: ``(o [T, H, W] bf16, lse [H, T] fp32)`` of the softmax of
+    ``q_lat [T, H, W]`` over the first ``ctx[t]`` rows; empty rows give ``o = 0``, ``lse = -inf``.
+    ``error_flag`` (int32 [1], optional) receives 5 for a block-table entry outside the cache."""
+    if q_lat.dim() != 3 or q_lat.stride(-1) != 1 or q_lat.dtype != BF16:
+        raise ValueError('q_lat must be bf16 [T, H, W] with a unit last-dim stride')
+    T, H, W = q_lat.shape
+    nb, sb, page = _cache_geometry(cache, W)
+    _block_table(block_table)
+    if ctx.dtype != torch.int32 or ctx.shape != (T,) or block_table.shape[0] < T:
+        raise ValueError('ctx must be int32 [T] and block_table hold a row per token')
+    if empty is not None:
+        if empty.shape != (T,):
+            raise ValueError('empty must be [T]')
+        empty = empty.contiguous() if empty.dtype in (torch.bool, torch.uint8) else (empty != 0)
+    with _on_device(q_lat, cache, block_table, ctx, empty, error_flag):
+        need = T * H * num_kv_splits * (W + 1)
+        buffer = workspace.ensure(q_lat.device)
+        if need > buffer.numel():
+            raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {buffer.numel()}')
+        o = torch.empty(T, H, W, dtype=BF16, device=q_lat.device)
+        lse = torch.empty(H, T, dtype=torch.float32, device=q_lat.device)
+        ctx = ctx.contiguous()
+        _lib.call('hla_s6_history_attention_q4', q_lat.data_ptr(), q_lat.stride(0), q_lat.stride(1), cache.data_ptr(),
+                  nb, sb, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], ctx.data_ptr(),
+                  _lib.ptr(empty), T, H, W, page, float(scale), int(num_kv_splits), buffer.data_ptr(), need,
+                  float(k_scale), float(v_scale), o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(),
+                  _lib.ptr(error_flag), _lib.stream_of(q_lat))
+    return o, lse
+
+
+def commit_rows(row, positions, table, cache, block_table, query_start_loc, k_scale=1.0, v_scale=1.0):
+    """Commit ``row [T, 2 W]`` (K | V, bf16): the K half latent-RoPE'd by ``table [max_position, W]`` at
+    ``positions [T]`` (int64), both halves quantised and stored at ``block_table[request, pos // page] * page +
+    pos % page``.  Returns the slots (int64 [T]); padding tokens (``t >= query_start_loc[-1]``) and positions
+    without a block in the cache are skipped, their slot is -1.  Two tokens of one call must not share a slot."""
+    if row.dim() != 2 or row.dtype != BF16 or row.stride(-1) != 1:
+        raise ValueError('row must be bf16 [T, 2 * width] with a unit last-dim stride')
+    T, W = row.shape[0], row.shape[1] // 2
+    nb, sb, page = _cache_geometry(cache, W)
+    if table.dim() != 2 or table.dtype != BF16 or table.stride(-1) != 1 or table.shape[1] != W:
+        raise ValueError(f'table must be bf16 [max_position, {W}] = [cos | sin]')
+    _block_table(block_table)
+    if (positions.dtype != torch.int64 or positions.shape != (T,) or query_start_loc.dtype != torch.int32
+            or query_start_loc.dim() != 1 or block_table.shape[0] < query_start_loc.shape[0] - 1):
+        raise ValueError('positions must be int64 [T], query_start_loc int32 [R + 1], block_table [R, max_blocks]')
+    with _on_device(row, positions, table, cache, block_table, query_start_loc):
+        positions, query_start_loc = positions.contiguous(), query_start_loc.contiguous()
+        slots = torch.empty(T, dtype=torch.int64, device=row.device)
+        _lib.call('hla_s6_commit_rows_q4', row.data_ptr(), row.stride(0), W, positions.data_ptr(), table.data_ptr(),
+                  table.stride(0), table.shape[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
+                  block_table.stride(0), block_table.shape[1], query_start_loc.data_ptr(),
+                  query_start_loc.shape[0] - 1, T, float(k_scale), float(v_scale), slots.data_ptr(),
+                  _lib.stream_of(row))
+    return slots
+
+
+def _gather(cache, blocks, slots, rows, k_scale, v_scale, out, error_flag):
+    W = cache_width(cache)
+    nb, sb, page = _cache_geometry(cache, W)
+    index = blocks if slots is None else slots
+    if index.dim() != 1 or index.dtype != (torch.int32 if slots is None else torch.int64):
+        raise ValueError('blocks must be int32 [n], slots int64 [n]')
+    if rows < 0 or (slots is None and -(-rows // page) > blocks.shape[0]):
+        raise IndexError('the block list does not cover the rows')
+    if out is not None and (out.shape != (rows, 2 * W) or out.dtype != BF16 or out.stride(-1) != 1):
+        raise ValueError(f'out must be bf16 [{rows}, {2 * W}] with a unit last-dim stride')
+    with _on_device(cache, index, out, error_flag):
+        index = index.contiguous()
+        if out is None:
+            out = torch.empty(rows, 2 * W, dtype=BF16, device=cache.device)
+        if rows:
+            _lib.call('hla_s6_gather_rows_q4', cache.data_ptr(), nb, sb, W, page,
+                      index.data_ptr() if slots is None else None, None if slots is None else index.data_ptr(), rows,
+                      float(k_scale), float(v_scale), out.data_ptr(), out.stride(0), _lib.ptr(error_flag),
+                      _lib.stream_of(cache))
+    return out
+
+
+def gather_rows(cache, blocks, length, k_scale=1.0, v_scale=1.0, out=None, error_flag=None):
+    """Rows 0 .. length - 1 of a request as bf16 ``[length, 2 W]`` (rotated K | V): row i is row ``i % page`` of
+    block ``blocks[i // page]`` (int32).  A block outside the cache gives zeros and sets ``error_flag`` to 5."""
+    return _gather(cache, blocks, None, int(length), k_scale, v_scale, out, error_flag)
+
+
+def gather_slots(cache, slots, k_scale=1.0, v_scale=1.0, out=None, error_flag=None):
+    """The rows at ``slots`` (int64, as ``commit_rows`` returns them; -1 gives zeros) as bf16 ``[n, 2 W]``."""
+    return _gather(cache, None, slots, slots.shape[0], k_scale, v_scale, out, error_flag)
+
+
+def weight_tiles(out_features, in_features):
+    """Shape of a packed weight: ``[ceil(out / 16), ceil(in / 128), 1088]`` (uint8)."""
+    return -(-out_features // 16), -(-in_features // 128), WEIGHT_TILE_BYTES
+
+
+def quantize_weight(weight, scale=None):
+    """``(packed, scale)`` of a bf16 weight ``[N, K]``, K a multiple of 32.  ``scale`` defaults to
+    ``tensor_scale`` of its largest value (which reads it back: call this once, at load time)."""
+    if weight.dim() != 2 or weight.dtype != BF16 or weight.stride(-1) != 1:
+        raise ValueError('weight must be bf16 [N, K] with a unit last-dim stride')
+    N, K = weight.shape
+    if K < GROUP or K % GROUP or N < 1:
+        raise ValueError('a 4-bit weight needs in_features a multiple of 32')
+    with _on_device(weight):
+        if scale is None:
+            scale = tensor_scale(float(weight.abs().amax()))
+        packed = torch.empty(weight_tiles(N, K), dtype=torch.uint8, device=weight.device)
+        _lib.call('hla_s6_quantize_weight_q4', weight.data_ptr(), weight.stride(0), N, K, float(scale),
+                  packed.data_ptr(), _lib.stream_of(weight))
+    return packed, float(scale)
+
+
+def linear(x, packed, out_features, scale, residual=None, out=None):
+    """``bf16(scale * x . w^T + residual)`` for ``x [T, K]`` bf16 and the packed weight ``[N, K]``: fp32 sums, one
+    rounding.  ``residual`` and ``out`` are bf16 ``[T, N]``; ``out`` may be ``residual``."""
+    if x.dim() != 2 or x.dtype != BF16 or x.stride(-1) != 1:
+        raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
+    T, K = x.shape
+    N = int(out_features)
+    if packed.dtype != torch.uint8 or packed.shape != weight_tiles(N, K) or not packed.is_contiguous():
+        raise ValueError(f'packed must be contiguous uint8 {list(weight_tiles(N, K))}, got {packed.dtype} '
+                         f'{list(packed.shape)}')
+    for y in (residual, out):
+        if y is not None and (y.shape != (T, N) or y.dtype != BF16 or y.stride(-1) != 1):
+            raise ValueError(f'residual and out must be bf16 [{T}, {N}] with a unit last-dim stride')
+    with _on_device(x, packed, residual, out):
+        if out is None:
+            out = torch.empty(T, N, dtype=BF16, device=x.device)
+        _lib.call('hla_s6_linear_q4', x.data_ptr(), x.stride(0), packed.data_ptr(), T, N, K, float(scale),
+                  _lib.ptr(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
+                  _lib.stream_of(x))
+    return out

@@ -18,7 +18,7 @@ from collections import namedtuple
 
 import torch
 
-from . import _lib
+from . import _lib, q4
 
 INF = float('inf')
 BACKEND = 'b200'
@@ -152,11 +152,16 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
     ``cache`` is the logical vLLM layout ``[num_blocks, 1, block, 2W]`` (K then V on the last dim);
     ``block_table[T, max_blocks]`` int32 per token (only columns ``< ceil(ctx[t]/block)`` are read);
     ``ctx[T]`` int32.  Returns ``(o[T,H,W] bf16, lse[H,T] fp32)``; empty rows give ``o = 0``,
-    ``lse = -inf`` (reference s6_ops.py:117-161).  ``k_scale``/``v_scale`` are accepted for
-    signature compatibility; like the reference adapter, quantized caches are not supported.
+    ``lse = -inf`` (reference s6_ops.py:117-161).  A uint8 ``cache`` is a 4-bit cache
+    (``[num_blocks, 1, block, 17 * W / 16]``, ``q4.history_attention``) with the tensor scales
+    ``k_scale`` / ``v_scale`` (floats, None is 1); a bf16 cache ignores them, they are accepted for
+    signature compatibility.
     """
     _require(backend, 'history')
     _check_cuda(q_lat, cache, block_table, ctx)
+    if cache.dtype == torch.uint8:
+        return q4.history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace,
+                                    1.0 if k_scale is None else k_scale, 1.0 if v_scale is None else v_scale, empty)
     if q_lat.dim() != 3 or q_lat.stride(-1) != 1:
         raise ValueError('q_lat must be [T, H, W] with a unit last-dim stride')
     if q_lat.dtype != torch.bfloat16:

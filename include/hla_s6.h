@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 4
+#define HLA_S6_ABI_VERSION 5
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1
 #define HLA_S6_EOVERFLOW 2
@@ -422,6 +422,75 @@ int hla_s6_export_rows(const void* const* main_caches, const void* const* l1_cac
                        int64_t l1_num_blocks, int64_t l1_stride_block, int64_t l1_stride_row, int32_t l1_width,
                        int32_t l1_block_size, const int32_t* l1_blocks, int64_t l1_blocks_len, int64_t length, void* out, int* error_flag,
                        void* stream);
+
+/* ---------------------------------------------------------------- 4-bit latent cache and weights
+ * A group of 32 consecutive columns shares one e4m3 scale s; a value is (n - 8) * s * ts with a code n
+ * in 1..15 and one tensor scale ts > 0 (k_scale, v_scale of a cache; scale of a weight).  Quantising:
+ * s = e4m3(amax / (7 ts)), saturated at 448; n = 8 + rint(x / (s ts)) clamped to 1..15; a group whose
+ * scale rounds to 0 stores zeros.  Codes travel in 32-bit words of 8 columns: nibble i holds column 2i,
+ * nibble i + 4 column 2i + 1.
+ *
+ * A 4-bit latent cache is uint8 [num_blocks, 1, page, 17 * width / 16], width 256, 512 or 1024, page a
+ * multiple of 16, any block stride (bytes) that is a multiple of 16 and holds a page; the bytes of a page
+ * are contiguous: page / 16 tiles of 16 rows, each (G = width / 32)
+ *   K codes [G][16 rows][16 B] | V codes [width / 8][16 rows][4 B] | K scales [16 rows][G] | V scales [G][16 rows].
+ * Each byte belongs to one row.  The tensor scales are not stored: every call on a cache gives the same. */
+
+/* hla_s6_history_attention over a 4-bit cache: the same contract, outputs and workspace
+ * (T * num_kv_splits * H * (width + 1) floats, 16-byte aligned); q_lat rows 16-byte aligned. */
+int hla_s6_history_attention_q4(const void* q_lat, int64_t q_stride_t, int64_t q_stride_h, const void* cache,
+                                int64_t num_blocks, int64_t cache_stride_block, const int32_t* block_table,
+                                int64_t block_table_stride, int32_t max_blocks, const int32_t* ctx,
+                                const uint8_t* empty, int32_t num_tokens, int32_t num_heads, int32_t width,
+                                int32_t page, float scale, int32_t num_kv_splits, float* workspace,
+                                int64_t workspace_floats, float k_scale, float v_scale, void* out,
+                                int64_t out_stride_t, int64_t out_stride_h, float* lse, int* error_flag,
+                                void* stream);
+
+/* hla_s6_history_partials over a 4-bit cache: the partials are those that hla_s6_history_reduce,
+ * hla_s6_history_reduce_exchange and hla_s6_decode_combine take (same T, H, width, page, splits,
+ * workspace).  flags as hla_s6_history_partials. */
+int hla_s6_history_partials_q4(const void* q_lat, int64_t q_stride_t, int64_t q_stride_h, const void* cache,
+                               int64_t num_blocks, int64_t cache_stride_block, const int32_t* block_table,
+                               int64_t block_table_stride, int32_t max_blocks, const int32_t* ctx, int32_t num_tokens,
+                               int32_t num_heads, int32_t width, int32_t page, float scale, int32_t num_kv_splits,
+                               float* workspace, int64_t workspace_floats, float k_scale, float v_scale,
+                               int* error_flag, int32_t flags, void* stream);
+
+/* hla_s6_commit_rows into a 4-bit cache: the K half latent-RoPE'd in the torch bf16 order, then both halves
+ * quantised.  Padding tokens and tokens without a slot in the cache are skipped (slot_out -1).  Infinite
+ * values take their group's largest code.  Two tokens of one call must not share a slot.  row and table rows
+ * 16-byte aligned. */
+int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, const int64_t* positions,
+                          const void* table, int64_t table_stride, int64_t max_position, void* cache,
+                          int64_t num_blocks, int64_t cache_stride_block, int32_t page, const int32_t* block_table,
+                          int64_t block_table_stride, int32_t max_blocks, const int32_t* query_start_loc,
+                          int32_t num_reqs, int32_t num_tokens, float k_scale, float v_scale, int64_t* slot_out,
+                          void* stream);
+
+/* Rows of a 4-bit cache as bf16 [num_rows, 2 * width] (K | V, row stride out_stride elements, 16-byte aligned
+ * rows): row i is row i % page of block blocks[i / page] (blocks int32, ceil(num_rows / page) entries), or -
+ * with slots (int64 [num_rows]) instead - cache row slots[i] (block * page + offset; negative: zeros).  A block
+ * outside the cache gives zeros and sets error_flag (5).  The rows hla_s6_export_rows gathers from a bf16
+ * cache (hla/vllm_latent/cache_export.py:160-174). */
+int hla_s6_gather_rows_q4(const void* cache, int64_t num_blocks, int64_t cache_stride_block, int32_t width,
+                          int32_t page, const int32_t* blocks, const int64_t* slots, int64_t num_rows, float k_scale,
+                          float v_scale, void* out, int64_t out_stride, int* error_flag, void* stream);
+
+/* Bytes of a packed 4-bit weight [out_features, in_features]: ceil(out / 16) * ceil(in / 128) tiles of 1088
+ * bytes, tile (i, j) = codes [2][8][4][16 B] | scales [8][4][2] with row 16 i + 8 h + g, columns
+ * 128 j + 32 c .. + 31 at codes[h][g][c] and scales[g][c][h]; rows and columns past the matrix hold zeros.
+ * hla_s6_quantize_weight_q4 packs a bf16 weight (rows 16-byte aligned, in_features a multiple of 32). */
+#define HLA_S6_Q4_WEIGHT_TILE_BYTES 1088
+int hla_s6_quantize_weight_q4(const void* weight, int64_t weight_stride_n, int32_t out_features, int32_t in_features,
+                              float scale, void* packed, void* stream);
+
+/* out[t, n] = bf16(scale * sum_k x[t, k] w[n, k] + residual[t, n]) with a packed 4-bit weight; residual
+ * (bf16, may be NULL) and out have unit last strides, out may be residual.  The 4-bit form of
+ * hla_s6_writer_project and of the adapter's QKV / output projections (ouro_latent.py:109-110, 130). */
+int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens, int32_t out_features,
+                     int32_t in_features, float scale, const void* residual, int64_t residual_stride_t, void* out,
+                     int64_t out_stride_t, void* stream);
 
 #ifdef __cplusplus
 }
