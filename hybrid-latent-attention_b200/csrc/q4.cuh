@@ -69,6 +69,44 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t w, const Q4Scale& s) {
   return bf2_fma((sh & 0x00780078u) | 0x41804180u, s.s, s.c);
 }
 
+// The same in fp16, which needs one shift and two multiplications by 16 for the four pairs of a word instead of
+// four shifts: a nibble at bits 4..7 of a half under the exponent of 64 is 64 + n, and (64 + n) s - 72 s =
+// (n - 8) s (72 s has 8 significant bits, 72 * 448 < 65504: exact).
+struct Q4ScaleH {
+  uint32_t s, c;
+};
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+__device__ __forceinline__ Q4ScaleH q4_scale_h(uint32_t s2) { return Q4ScaleH{s2, h2_mul(s2, 0xd480d480u)}; }  // -72
+// Scales of two groups (bytes b0 | b1 << 8), each for both halves of a pair.
+__device__ __forceinline__ void q4_scales_h(uint32_t bytes, Q4ScaleH& a, Q4ScaleH& b) {
+  const Q4ScaleH p = q4_scale_h(e4m3x2_to_h2(bytes));
+  a = Q4ScaleH{__byte_perm(p.s, 0, 0x1010), __byte_perm(p.c, 0, 0x1010)};
+  b = Q4ScaleH{__byte_perm(p.s, 0, 0x3232), __byte_perm(p.c, 0, 0x3232)};
+}
+// The four pairs of a word: r[i] = columns 2i, 2i + 1 (or rows, where the halves of w come from two rows).
+__device__ __forceinline__ void q4_word_h(uint32_t w, const Q4ScaleH& s, uint32_t& r0, uint32_t& r1, uint32_t& r2,
+                                          uint32_t& r3) {
+  constexpr uint32_t kMask = 0x00f000f0u, kMagic = 0x54005400u;
+  const uint32_t t = w >> 8;
+  r0 = h2_fma(((w * 16u) & kMask) | kMagic, s.s, s.c);
+  r1 = h2_fma((w & kMask) | kMagic, s.s, s.c);
+  r2 = h2_fma(((t * 16u) & kMask) | kMagic, s.s, s.c);
+  r3 = h2_fma((t & kMask) | kMagic, s.s, s.c);
+}
+
 // Scale byte of a group: e4m3(amax / (7 ts)), a true division so that ties fall as the format says.
 __device__ __forceinline__ uint32_t q4_scale_byte(float amax, float ts) {
   return __nv_cvt_float_to_fp8(__fdiv_rn(amax, 7.f * ts), __NV_SATFINITE, __NV_E4M3);

@@ -4,11 +4,33 @@
 // (slot = CTA + row, slot ranges in meta) in the same workspace, so the reduces and the fused combine of
 // history.cu / combine.cu follow it unchanged.
 //
-// One warp owns 128 latent columns of 16-row tiles; heads are the M = 16 dimension of mma.m16n8k16.
-// Codes are dequantised in registers into bf16 fragments (exact).
+// What bounds it.  A row of 512-wide latents is 544 bytes and 32768 multiply-adds for 16 heads: 60 flop per
+// byte, four times the bf16 reader's.  mma.sync runs at 1024 multiply-adds per clock and SM here (8 clocks of
+// issue per m16n8k16 and scheduler, measured), which alone is 0.7 of the time HBM gives a row; the codes also
+// have to become f16 values, two per register, at about 11 instructions per word of 8.  A first version on
+// mma.sync did both on the same schedulers and took 260 us where the bytes take 43 (64 requests of 8160 rows).
+// So the products are on tcgen05, which issues asynchronously from one thread, and the schedulers only
+// dequantise.  Written to shared memory the dequantised values would need 2 KB a row in and 2 KB out of it
+// beside the codes, more than its bandwidth; the A operand of tcgen05.mma may lie in tensor memory instead,
+// which the dequantising threads write directly.  Keys (for the scores) and latent columns (for the output)
+// are therefore the M = 128 lanes and the heads are N = 16:
+//   S^T [128 keys x 16 heads]    = K [128 x W] (tensor memory) . Q^T (shared memory, f16)
+//   O^T [128 columns x 16 heads] += V^T [128 x 16 rows] (tensor memory) . P^T (shared memory, f16), W / 128 of them
+// One CTA per SM takes 128 rows ("step") at a time:
+//   warps 0-3  K: a thread dequantises one row into its lane; then the softmax of the step before: a thread has
+//              the 16 heads' scores of its key.  The exponent base of a head only moves when a score passes it by
+//              2^4 (a vote), so the output is rescaled rarely and the common step needs no reduction at all.
+//   warps 4-7  V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column).
+//   warp 8, 9  one thread each issues the score and the value products.
+//   warp 10    bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
+// f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
+// of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
+// 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
+// bits or, below p = 2^-25, to a multiple of 2^-35.
 #include "../../include/hla_s6.h"
 #include "hla_s6_internal.h"
 #include "q4.cuh"
+#include "tc.cuh"
 
 namespace hla {
 
@@ -17,7 +39,7 @@ struct Q4HistoryParams {
   int64_t q_st, q_sh;
   const uint8_t* cache;
   int64_t num_blocks, c_sb;
-  int page;
+  int tpp;  // 16-row tiles per page
   const int32_t* bt;
   int64_t bt_st;
   int32_t max_blocks;
@@ -28,236 +50,630 @@ struct Q4HistoryParams {
   float* ws_o;
   float* ws_lse;
   int2* meta;
-  int32_t slots_cap, grid, stream_mode;
+  int32_t slots_cap, parts, stream_mode;  // parts: CTAs of the page partition (stream mode)
   int* err;
+  uint64_t wait_ns;
 };
 
-// The scale bytes of rows row0, row0 + 1 with those at or past `valid` zeroed.
-__device__ __forceinline__ uint32_t mask_rows(uint32_t bytes, int row0, int valid) {
-  if (row0 >= valid) return 0u;
-  return row0 + 1 >= valid ? bytes & 0xffu : bytes;
+template <int W>
+struct Q4Cfg {
+  static constexpr int NB = W / 128;             // blocks of 128 latent columns (output accumulators)
+  static constexpr int TILE = 17 * W;            // bytes of 16 rows
+  static constexpr int UT = 2048 / W;            // tiles per ring unit
+  static constexpr int UNIT = UT * TILE;         // 34816
+  static constexpr int UNITS = 5;
+  static constexpr int VT = UT / 2;              // tiles per V chunk: 64 tensor-memory columns
+  // Dequantise a step's K rows before the softmax of the step before?  Its V chunks may wait for that softmax,
+  // so the ring has to hold both steps.
+  static constexpr bool AHEAD = 2 * (8 / UT) <= UNITS;
+  static constexpr int Q_BYTES = 32 * W;
+  static constexpr int P_BYTES = 4096;
+  // tensor-memory columns: two K chunks (128 rows x 128 latent columns), two V chunks, two score tiles, output
+  static constexpr uint32_t AK = 0, AV = 128, S = 256, O = 288;
+  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
+};
+constexpr int kQ4HistThreads = 11 * 32;
+// log2 of how far a score may pass its head's exponent base before the base moves, and of the factor the
+// probabilities carry: together they end at 2^15, f16's largest power of two.  A small first term lets small
+// probabilities keep f16's precision, a large one makes rescales rare (each costs about one step).
+constexpr float kQ4Over = 4.f, kQ4Lift = 11.f;
+
+// Sum or maximum of each of 16 values over a warp: halving exchanges, after which lane l holds value rev16(l % 16)
+// of all 32 lanes.
+template <bool MAX>
+__device__ __forceinline__ float reduce16(float (&v)[16], int lane) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int half = 8 >> k;
+    const bool up = (lane >> k) & 1;
+#pragma unroll
+    for (int j = 0; j < half; ++j) {
+      const float give = up ? v[j] : v[j + half], keep = up ? v[j + half] : v[j];
+      const float got = __shfl_xor_sync(0xffffffffu, give, 1 << k);
+      v[j] = MAX ? fmaxf(keep, got) : keep + got;
+    }
+  }
+  const float got = __shfl_xor_sync(0xffffffffu, v[0], 16);
+  return MAX ? fmaxf(v[0], got) : v[0] + got;
+}
+__device__ __forceinline__ int rev16(int l) { return ((l & 1) << 3) | ((l & 2) << 1) | ((l & 4) >> 1) | ((l & 8) >> 3); }
+
+// Barrier of `threads` threads that returns whether the predicate holds in any of them.
+__device__ __forceinline__ bool named_bar_or(int id, int threads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(pred ? 1u : 0u), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
 }
 
+// The steps of a CTA: up to 8 consecutive tiles of one row's segment.  Every role walks them by itself.
+struct Q4Walk {
+  const Q4HistoryParams& p;
+  const int* pref;  // page prefix (stream mode)
+  int r, pg, p1, tile, tend, n, ctx, slot;
+  bool first, last;
+  __device__ Q4Walk(const Q4HistoryParams& p_, const int* pref_, int r0, int p0, int p1_)
+      : p(p_), pref(pref_), r(r0), pg(p0), p1(p1_), tile(0), tend(0), n(0), ctx(0), slot(0), first(false), last(false) {}
+  __device__ __forceinline__ bool next() {
+    tile += n;
+    first = tile >= tend;
+    if (first) {
+      if (p.stream_mode) {
+        if (pg >= p1) return false;
+        while (pg >= pref[r + 1]) ++r;
+        const int base = pref[r], end = min(p1, pref[r + 1]);
+        ctx = p.ctx[r];
+        tile = (pg - base) * p.tpp;
+        tend = min((end - base) * p.tpp, (ctx + 15) >> 4);
+        pg = end;
+        slot = blockIdx.x + r;
+      } else {
+        for (r = pg; r < p.T; r += gridDim.x) {
+          ctx = p.ctx[r];
+          if (ctx > 0) break;
+        }
+        if (r >= p.T) return false;
+        pg = r + gridDim.x;
+        tile = 0;
+        tend = (ctx + 15) >> 4;
+        slot = r;
+      }
+    }
+    n = min(8, tend - tile);
+    last = tile + n >= tend;
+    return true;
+  }
+};
+
 template <int W>
-__global__ void __launch_bounds__(W / 4) q4_history_kernel(const Q4HistoryParams p) {
-  constexpr int NC = W / 128, G = W / kQ4Group;
-  __shared__ float4 xbuf[2][NC][2][32];
-  extern __shared__ int pref[];  // [T + 1] page prefix (stream mode)
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
-  const int T = p.T, page = p.page;
-  int64_t P = 0, GR = 1, p0 = 0, p1 = 0;
-  int r = blockIdx.x;
+__global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4HistoryParams p) {
+  using C = Q4Cfg<W>;
+  constexpr int NB = C::NB, UT = C::UT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* qs = smem;
+  uint8_t* ps = qs + C::Q_BYTES;
+  uint8_t* units = ps + C::P_BYTES;
+  uint8_t* ctl = units + C::UNITS * C::UNIT;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
+  uint64_t* empty = full + C::UNITS;                  // [UNITS] unit read
+  uint64_t* akf = empty + C::UNITS;                   // [2] K chunk in tensor memory
+  uint64_t* ake = akf + 2;                            // [2] its MMAs are done
+  uint64_t* avf = ake + 2;                            // [2] V chunk
+  uint64_t* ave = avf + 2;
+  uint64_t* sf = ave + 2;                             // [2] scores of a step
+  uint64_t* pf = sf + 2;                              // probabilities of a step written
+  uint64_t* pv = pf + 1;                              // value products of a step done
+  uint64_t* drain = pv + 1;                           // [2] every MMA of an issuer is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  float* qscale = reinterpret_cast<float*>(ctl + 256);  // [2][16] score factor of a head, by segment parity
+  float* red = qscale + 32;                             // [4][16] per-warp maxima / sums
+  int* pref = reinterpret_cast<int*>(ctl + 1024);       // [T + 1] (stream mode)
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int r0 = 0, p0 = 0, p1 = 0;
+  int P = 0, G = 1;
   if (p.stream_mode) {
-    for (int t = tid; t < T; t += blockDim.x) pref[t + 1] = (max(p.ctx[t], 0) + page - 1) / page;
+    const int page = 16 * p.tpp;
+    for (int t = tid; t < p.T; t += blockDim.x) pref[t + 1] = (max(p.ctx[t], 0) + page - 1) / page;
     if (tid == 0) pref[0] = 0;
     __syncthreads();
     if (warp == 0) {
       int carry = 0;
-      for (int b = 0; b < T; b += 32) {
-        int v = b + lane < T ? pref[b + lane + 1] : 0;
+      for (int b = 0; b < p.T; b += 32) {
+        int v = b + lane < p.T ? pref[b + lane + 1] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int n = __shfl_up_sync(0xffffffffu, v, o);
           if (lane >= o) v += n;
         }
-        if (b + lane < T) pref[b + lane + 1] = v + carry;
+        if (b + lane < p.T) pref[b + lane + 1] = v + carry;
         carry += __shfl_sync(0xffffffffu, v, 31);
       }
     }
     __syncthreads();
-    P = pref[T];
-    GR = p.grid < P ? static_cast<int64_t>(p.grid) : P;
-    griddep_wait();
-    if (blockIdx.x == 0) {
-      for (int t = tid; t < T; t += blockDim.x) {
-        const int a = pref[t], b = pref[t + 1];
-        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, GR)) + t,
-                                      static_cast<int>(stream_owner(b - 1, P, GR)) + t + 1)
-                          : make_int2(0, 0);
+    P = pref[p.T];
+    G = min(p.parts, P);
+    if (static_cast<int>(blockIdx.x) >= G) {
+      if (blockIdx.x == 0) {  // no rows at all: every slot range is empty
+        griddep_wait();
+        for (int t = tid; t < p.T; t += blockDim.x) p.meta[t] = make_int2(0, 0);
       }
+      return;
     }
-    if (static_cast<int64_t>(blockIdx.x) >= GR) return;
-    p0 = stream_start(blockIdx.x, P, GR);
-    p1 = stream_start(blockIdx.x + 1, P, GR);
-    int lo = 0, hi = T;
+    p0 = static_cast<int>(stream_start(blockIdx.x, P, G));
+    p1 = static_cast<int>(stream_start(blockIdx.x + 1, P, G));
+    int lo = 0, hi = p.T;  // the row holding page p0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pref[mid] <= p0) lo = mid; else hi = mid;
     }
-    r = lo;
+    r0 = lo;
   } else {
-    griddep_wait();
-    p1 = (max(p.ctx[r], 0) + page - 1) / page;
-    if (p1 == 0) {
-      if (tid < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + tid] = -INFINITY;
-      return;
-    }
+    p0 = blockIdx.x;  // rows blockIdx.x, + gridDim.x, ...
   }
-  if (tid == 0) griddep_launch_dependents();
 
-  const Q4Tile tl(W);
-  int buf = 0;
-  for (int64_t pg = p0; pg < p1;) {  // one row's segment at a time
-    int64_t base = 0, end = p1;
-    if (p.stream_mode) {
-      while (pg >= pref[r + 1]) ++r;
-      base = pref[r];
-      end = min(p1, static_cast<int64_t>(pref[r + 1]));
+  if (warp == 8) tc::alloc(tmem_slot, 512);
+  if (tid == 9 * 32) {
+    for (int s = 0; s < C::UNITS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4 + (UT >= 8 ? 4 : UT / 2));  // the V warps, and the K warps of its tiles
     }
-    const int ctx = max(p.ctx[r], 0);
-    const int col0 = warp * 128;
-    uint32_t qa[8][4];
-    {
-      // fragment step s of this thread: latent columns col0 + 32 c4 + 4 s + {0,1} and {2,3}
-      const __nv_bfloat16* q0 = p.q + static_cast<int64_t>(r) * p.q_st + static_cast<int64_t>(g8) * p.q_sh + col0 + 32 * c4;
-      const __nv_bfloat16* q1 = q0 + 8 * p.q_sh;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        qa[s][0] = g8 < p.H ? *reinterpret_cast<const uint32_t*>(q0 + 4 * s) : 0u;
-        qa[s][1] = g8 + 8 < p.H ? *reinterpret_cast<const uint32_t*>(q1 + 4 * s) : 0u;
-        qa[s][2] = g8 < p.H ? *reinterpret_cast<const uint32_t*>(q0 + 4 * s + 2) : 0u;
-        qa[s][3] = g8 + 8 < p.H ? *reinterpret_cast<const uint32_t*>(q1 + 4 * s + 2) : 0u;
-      }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&akf[b], 4);
+      mbar_init(&ake[b], 1);
+      mbar_init(&avf[b], 4);
+      mbar_init(&ave[b], 1);
+      mbar_init(&sf[b], 1);
+      mbar_init(&drain[b], 1);
     }
-    float o[16][4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-    for (; pg < end; ++pg) {
-      const int lp = static_cast<int>(pg - base);
-      const int blk = lp < p.max_blocks ? p.bt[static_cast<int64_t>(r) * p.bt_st + lp] : -1;
-      const bool present = blk >= 0 && blk < p.num_blocks;  // an entry outside the cache reads as zeros
-      if (!present && tid == 0) record_error(p.err, kErrBlock);
-      const uint8_t* pb = p.cache + (present ? static_cast<int64_t>(blk) * p.c_sb : 0);
-      for (int sub = 0; sub < page; sub += 16) {
-        const int valid = min(16, ctx - lp * page - sub);
-        if (valid <= 0) break;
-        const uint8_t* tb = pb + (sub / 16) * tl.bytes();
-        // ---- partial scores over this warp's columns
-        float sc[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-          const int row = 8 * j + g8;
-          const uint4 kc = __ldg(reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * warp + c4, row)));
-          uint32_t sb = __ldg(tb + tl.k_scale(row, 4 * warp + c4));
-          if (!present) sb = 0;
-          const Q4Scale s(e4m3x2_to_bf2(sb | (sb << 8)));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = i == 0 ? kc.x : (i == 1 ? kc.y : (i == 2 ? kc.z : kc.w));
-            mma_bf16_16816(sc[j], qa[2 * i], q4_pair<0>(w, s), q4_pair<1>(w, s));
-            mma_bf16_16816(sc[j], qa[2 * i + 1], q4_pair<2>(w, s), q4_pair<3>(w, s));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) xbuf[buf][warp][j][lane] = make_float4(sc[j][0], sc[j][1], sc[j][2], sc[j][3]);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-#pragma unroll
-          for (int w = 0; w < NC; ++w) {
-            const float4 v = xbuf[buf][w][j][lane];
-            sc[j][0] += v.x; sc[j][1] += v.y; sc[j][2] += v.z; sc[j][3] += v.w;
-          }
-        }
-        buf ^= 1;
-        // ---- online softmax (log2 domain)
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool in = j * 8 + 2 * c4 + e < valid;
-            sc[j][e] = in ? sc[j][e] * p.scale_log2 : -INFINITY;
-            sc[j][2 + e] = in ? sc[j][2 + e] * p.scale_log2 : -INFINITY;
-            mx0 = fmaxf(mx0, sc[j][e]);
-            mx1 = fmaxf(mx1, sc[j][2 + e]);
-          }
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float mn0 = fmaxf(m_run[0], mx0), mn1 = fmaxf(m_run[1], mx1);
-        const float al0 = exp2f(m_run[0] - mn0), al1 = exp2f(m_run[1] - mn1);
-        m_run[0] = mn0;
-        m_run[1] = mn1;
-        float rs0 = 0.f, rs1 = 0.f;
-        uint32_t pa[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float e0 = exp2f(sc[j][0] - mn0), e1 = exp2f(sc[j][1] - mn0);
-          const float e2 = exp2f(sc[j][2] - mn1), e3 = exp2f(sc[j][3] - mn1);
-          rs0 += e0 + e1;
-          rs1 += e2 + e3;
-          pa[j * 2] = pack_bf16(e0, e1);
-          pa[j * 2 + 1] = pack_bf16(e2, e3);
-        }
-        l_run[0] = l_run[0] * al0 + rs0;
-        l_run[1] = l_run[1] * al1 + rs1;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          o[j][0] *= al0; o[j][1] *= al0;
-          o[j][2] *= al1; o[j][3] *= al1;
-        }
-        // ---- O += P . V: rows 2c, 2c + 1 and 8 + 2c, 9 + 2c of the 16 columns col0 + 16 g8 ..
-        const int vg = 4 * warp + (g8 >> 1);
-        uint32_t sv = *reinterpret_cast<const uint16_t*>(tb + tl.v_scale(vg, 2 * c4));
-        uint32_t sw = *reinterpret_cast<const uint16_t*>(tb + tl.v_scale(vg, 8 + 2 * c4));
-        // rows past the context (or of an absent page): a zero scale, whatever their bytes are
-        sv = mask_rows(present ? sv : 0u, 2 * c4, valid);
-        sw = mask_rows(present ? sw : 0u, 8 + 2 * c4, valid);
-        const Q4Scale s0(e4m3x2_to_bf2(sv)), s1(e4m3x2_to_bf2(sw));
-#pragma unroll
-        for (int oc = 0; oc < 2; ++oc) {
-          const int octet = 16 * warp + 2 * g8 + oc;
-          const uint2 u0 = __ldg(reinterpret_cast<const uint2*>(tb + tl.v_codes(octet, 2 * c4)));
-          const uint2 u1 = __ldg(reinterpret_cast<const uint2*>(tb + tl.v_codes(octet, 8 + 2 * c4)));
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {  // even, odd columns of the octet
-            const uint32_t sel = half ? 0x7632 : 0x5410;
-            const uint32_t a = __byte_perm(u0.x, u0.y, sel), b = __byte_perm(u1.x, u1.y, sel);
-            mma_bf16_16816(o[oc * 8 + half], pa, q4_pair<0>(a, s0), q4_pair<0>(b, s1));
-            mma_bf16_16816(o[oc * 8 + 2 + half], pa, q4_pair<1>(a, s0), q4_pair<1>(b, s1));
-            mma_bf16_16816(o[oc * 8 + 4 + half], pa, q4_pair<2>(a, s0), q4_pair<2>(b, s1));
-            mma_bf16_16816(o[oc * 8 + 6 + half], pa, q4_pair<3>(a, s0), q4_pair<3>(b, s1));
-          }
-        }
-      }
-    }
-    // ---- segment end: the normalised partial and its lse
-    float l0 = l_run[0], l1 = l_run[1];
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const int64_t slot = p.stream_mode ? static_cast<int64_t>(blockIdx.x) + r : r;
-    if (slot >= p.slots_cap) {
-      if (tid == 0) record_error(p.err, kErrSlots);
-    } else {
-      const float ln2 = 0.6931471805599453f;
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int h = g8 + 8 * hh;
-        if (h >= p.H) continue;
-        const float inv = p.v_ts / (hh ? l1 : l0);
-        float* dst = p.ws_o + (slot * p.H + h) * W + col0 + 32 * c4;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<float4*>(dst + 16 * e + j) =
-                make_float4(o[j][2 * hh + e] * inv, o[j + 1][2 * hh + e] * inv, o[j + 2][2 * hh + e] * inv,
-                            o[j + 3][2 * hh + e] * inv);
-        if (warp == 0 && c4 == 0) p.ws_lse[slot * p.H + h] = ((hh ? m_run[1] : m_run[0]) + log2f(hh ? l1 : l0)) * ln2;
-      }
-    }
+    mbar_init(pf, 4);
+    mbar_init(pv, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
   }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const tc::Waits wait{abort_flag, p.err, p.wait_ns};
+  const Q4Tile tl(W);
+  Q4Walk st(p, pref, r0, p0, p1);
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ K rows, softmax, output
+    // Launched as a programmatic dependent of the launch that writes q, this grid has been copying tiles
+    // meanwhile; q and the workspace are touched only once that launch has completed.
+    griddep_wait();
+    if (tid == 0) griddep_launch_dependents();
+    if (p.stream_mode && blockIdx.x == 0) {
+      for (int t = tid; t < p.T; t += 128) {
+        const int a = pref[t], b = pref[t + 1];
+        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
+                                      static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
+                          : make_int2(0, 0);
+      }
+    }
+    if (!p.stream_mode && warp == 0) {  // rows without history: their slot says so
+      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
+        if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
+    }
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    int unit0 = 0;      // ring position of the step's first unit
+    uint32_t kchunk = 0;
+    int seg = -1;       // segments started (Q loads)
+
+    auto load_q = [&](int r) {
+      // 8 threads per head, W / 8 columns each
+      const int h = tid >> 3, part = tid & 7;
+      const __nv_bfloat16* src = p.q + static_cast<int64_t>(r) * p.q_st + static_cast<int64_t>(h) * p.q_sh + part * (W / 8);
+      uint4 v[W / 64];
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < W / 64; ++i) {
+        v[i] = h < p.H ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xffff0000u))));
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      // a power of two that puts the head's largest element into [2^12, 2^13) (an infinity stays one)
+      int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
+      e = e > 110 ? 110 : (e < -110 ? -110 : e);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      if (part == 0) qscale[(seg & 1) * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < W / 64; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 hh = __floats2half2_rn(__uint_as_float(w[j] << 16) * down, __uint_as_float(w[j] & 0xffff0000u) * down);
+          u[j] = *reinterpret_cast<const uint32_t*>(&hh);
+        }
+        const int col = part * (W / 8) + 8 * i;
+        *reinterpret_cast<uint4*>(qs + (col >> 6) * 2048 + tc::sw128(h, (col >> 3) & 7)) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      fence_proxy_async();
+      named_bar_sync(1, 128);  // the score factors
+    };
+
+    // dequantise this step's K rows: thread = row 32 warp + lane, chunk by chunk of 128 latent columns
+    auto dequant_k = [&]() {
+      const int t0 = 2 * warp;                    // this warp's first tile of the step
+      const int u = t0 / UT;
+      const bool unit_there = u * UT < st.n;
+      const int ring = (unit0 + u) % C::UNITS;
+      const int tiu = t0 - u * UT + (lane >> 4);  // tile inside the unit
+      const uint8_t* tb = units + ring * C::UNIT + tiu * C::TILE;
+      const int row = lane & 15;
+      if (unit_there) wait(&full[ring], ((unit0 + u) / C::UNITS) & 1, kErrWaitFull);
+      __syncwarp();
+      uint32_t sc[W / 128];                       // the row's scales, four groups to a word
+#pragma unroll
+      for (int i = 0; i < W / 128; ++i) sc[i] = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * i));
+#pragma unroll
+      for (int kc = 0; kc < W / 128; ++kc, ++kchunk) {
+        const int buf = kchunk & 1;
+        if (kchunk >= 2) wait(&ake[buf], ((kchunk >> 1) - 1) & 1, kErrWaitEmpty);
+        __syncwarp();
+        tc::fence_after();
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t v[32];
+          Q4ScaleH s0, s1;
+          q4_scales_h((sc[kc] >> (16 * hf)) & 0xffffu, s0, s1);
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const uint4 c = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
+            const Q4ScaleH& s = gi ? s1 : s0;
+            q4_word_h(c.x, s, v[16 * gi], v[16 * gi + 1], v[16 * gi + 2], v[16 * gi + 3]);
+            q4_word_h(c.y, s, v[16 * gi + 4], v[16 * gi + 5], v[16 * gi + 6], v[16 * gi + 7]);
+            q4_word_h(c.z, s, v[16 * gi + 8], v[16 * gi + 9], v[16 * gi + 10], v[16 * gi + 11]);
+            q4_word_h(c.w, s, v[16 * gi + 12], v[16 * gi + 13], v[16 * gi + 14], v[16 * gi + 15]);
+          }
+          tc::st32(lane_base + C::AK + buf * 64 + hf * 32, v);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&akf[buf]);
+          if (kc == W / 128 - 1 && unit_there) mbar_arrive(&empty[ring]);
+        }
+      }
+      unit0 += (st.n + UT - 1) / UT;
+    };
+
+    float m[16], l[16];
+    auto softmax = [&](const Q4Walk& x, uint32_t i, int sseg) {
+      const int sb = i & 1;
+      wait(&sf[sb], (i >> 1) & 1, kErrWaitFull);
+      __syncwarp();
+      tc::fence_after();
+      uint32_t raw[16];
+      tc::ld16(lane_base + C::S + sb * 16, raw);
+      tc::wait_ld();
+      tc::fence_before();
+      const bool live = (x.tile << 4) + 32 * warp + lane < x.ctx && (32 * warp + lane) < (x.n << 4);
+      const float4* fs = reinterpret_cast<const float4*>(qscale + (sseg & 1) * 16);
+      float s[16];
+      float over = -INFINITY;
+#pragma unroll
+      for (int h4 = 0; h4 < 4; ++h4) {
+        const float4 f = fs[h4];
+        s[4 * h4] = live ? __uint_as_float(raw[4 * h4]) * f.x : -INFINITY;
+        s[4 * h4 + 1] = live ? __uint_as_float(raw[4 * h4 + 1]) * f.y : -INFINITY;
+        s[4 * h4 + 2] = live ? __uint_as_float(raw[4 * h4 + 2]) * f.z : -INFINITY;
+        s[4 * h4 + 3] = live ? __uint_as_float(raw[4 * h4 + 3]) * f.w : -INFINITY;
+      }
+      if (x.first) {
+#pragma unroll
+        for (int h = 0; h < 16; ++h) {
+          m[h] = -INFINITY;
+          l[h] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 16; ++h) over = fmaxf(over, s[h] - m[h]);
+      }
+      // the step's probabilities replace the last step's, and a rescale touches the output: the value products
+      // of the step before have to be done for either
+      if (i > 0) wait(pv, (i - 1) & 1, kErrWaitFull);
+      __syncwarp();
+      if (named_bar_or(1, 128, x.first || over > kQ4Over)) {
+        // new bases: the maximum over the step's keys, per head
+        float mx[16];
+#pragma unroll
+        for (int h = 0; h < 16; ++h) mx[h] = s[h];
+        const float top = reduce16<true>(mx, lane);
+        if (lane < 16) red[warp * 16 + rev16(lane)] = top;
+        named_bar_sync(1, 128);
+        float al[16];
+#pragma unroll
+        for (int h = 0; h < 16; ++h) {
+          const float mn = fmaxf(fmaxf(fmaxf(red[h], red[16 + h]), fmaxf(red[32 + h], red[48 + h])), m[h]);
+          al[h] = mn == m[h] ? 1.f : exp2f(m[h] - mn);
+          m[h] = mn;
+          l[h] *= al[h];
+        }
+        if (!x.first) {
+          tc::fence_after();
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint32_t o[16];
+            tc::ld16(lane_base + C::O + b * 16, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int h = 0; h < 16; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * al[h]);
+            tc::st16(lane_base + C::O + b * 16, o);
+          }
+          tc::wait_st();
+          tc::fence_before();
+        }
+        named_bar_sync(1, 128);  // red is read before it is written again
+      }
+      const int key = 32 * warp + lane;
+      uint8_t* pk = ps + (key >> 6) * 2048 + (key & 7) * 2;
+#pragma unroll
+      for (int h = 0; h < 16; ++h) {
+        const float e = s[h] == -INFINITY ? 0.f : exp2f(s[h] - m[h] + kQ4Lift);
+        l[h] += e;
+        *reinterpret_cast<__half*>(pk + tc::sw128(h, (key >> 3) & 7)) = __float2half_rn(e);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pf);
+    };
+
+    auto write_out = [&](const Q4Walk& x, uint32_t i) {
+      float t[16];
+#pragma unroll
+      for (int h = 0; h < 16; ++h) t[h] = l[h];
+      const float sum = reduce16<false>(t, lane);
+      if (lane < 16) red[warp * 16 + rev16(lane)] = sum;
+      named_bar_sync(1, 128);
+      float inv[16];
+#pragma unroll
+      for (int h = 0; h < 16; ++h) inv[h] = red[h] + red[16 + h] + red[32 + h] + red[48 + h];
+      const bool room = x.slot < p.slots_cap;
+      if (!room && tid == 0) record_error(p.err, kErrSlots);
+      if (room && warp == 0) {
+        float mine_m = 0.f, mine_l = 1.f;
+#pragma unroll
+        for (int h = 0; h < 16; ++h)
+          if (lane == h) {
+            mine_m = m[h];
+            mine_l = inv[h];
+          }
+        if (lane < p.H)
+          p.ws_lse[static_cast<int64_t>(x.slot) * p.H + lane] = (mine_m + (log2f(mine_l) - kQ4Lift)) * 0.6931471805599453f;
+      }
+#pragma unroll
+      for (int h = 0; h < 16; ++h) inv[h] = inv[h] == 0.f ? 0.f : p.v_ts / inv[h];  // 0: every score is -inf
+      wait(pv, i & 1, kErrWaitFull);
+      __syncwarp();
+      tc::fence_after();
+      // lane 8 q + g of warp w holds columns (8 w + g) 4 NB + q NB .. + NB - 1, one per block
+      constexpr int NV = NB < 4 ? NB : 4;
+      const int col = (8 * warp + (lane & 7)) * 4 * NB + (lane >> 3) * NB;
+#pragma unroll
+      for (int b0 = 0; b0 < NB; b0 += NV) {
+        uint32_t o[NV][16];
+#pragma unroll
+        for (int b = 0; b < NV; ++b) tc::ld16(lane_base + C::O + (b0 + b) * 16, o[b]);
+        tc::wait_ld();
+        if (room) {
+#pragma unroll
+          for (int h = 0; h < 16; ++h) {
+            if (h >= p.H) continue;
+            float* dst = p.ws_o + (static_cast<int64_t>(x.slot) * p.H + h) * W + col + b0;
+            if constexpr (NV == 4)
+              *reinterpret_cast<float4*>(dst) =
+                  make_float4(__uint_as_float(o[0][h]) * inv[h], __uint_as_float(o[1][h]) * inv[h],
+                              __uint_as_float(o[2][h]) * inv[h], __uint_as_float(o[3][h]) * inv[h]);
+            else
+              *reinterpret_cast<float2*>(dst) =
+                  make_float2(__uint_as_float(o[0][h]) * inv[h], __uint_as_float(o[1][h]) * inv[h]);
+          }
+        }
+      }
+      tc::fence_before();
+      named_bar_sync(1, 128);  // red is read before it is written again
+    };
+
+    if (st.next()) {
+      Q4Walk cur = st;
+      ++seg;
+      load_q(st.r);
+      dequant_k();
+      for (uint32_t i = 0;; ++i) {
+        const int cur_seg = seg;
+        const bool more = st.next();
+        if (more && C::AHEAD) {
+          if (st.first) {
+            wait(&sf[i & 1], (i >> 1) & 1, kErrWaitFull);  // the scores of step i read Q no more
+            ++seg;
+            load_q(st.r);
+          }
+          dequant_k();
+        }
+        softmax(cur, i, cur_seg);
+        if (cur.last) write_out(cur, i);
+        if (!more) break;
+        if (!C::AHEAD) {
+          if (st.first) {
+            ++seg;
+            load_q(st.r);
+          }
+          dequant_k();
+        }
+        cur.r = st.r; cur.tile = st.tile; cur.n = st.n; cur.ctx = st.ctx; cur.slot = st.slot;
+        cur.first = st.first; cur.last = st.last;
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ V columns
+    const int w = warp - 4, g = lane >> 2, c = lane & 3;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int col0 = (8 * w + g) * 4 * NB;  // this thread's 4 NB columns
+    int unit0 = 0;
+    uint32_t vchunk = 0;
+    while (st.next()) {
+      for (int t0 = 0; t0 < st.n; t0 += C::VT, ++vchunk) {
+        const int u = t0 / UT, ring = (unit0 + u) % C::UNITS, buf = vchunk & 1;
+        if (t0 == u * UT) wait(&full[ring], ((unit0 + u) / C::UNITS) & 1, kErrWaitFull);
+        if (vchunk >= 2) wait(&ave[buf], ((vchunk >> 1) - 1) & 1, kErrWaitEmpty);
+        __syncwarp();
+        tc::fence_after();
+#pragma unroll
+        for (int ti = 0; ti < C::VT; ++ti) {
+          if (t0 + ti >= st.n) break;
+          const uint8_t* tb = units + ring * C::UNIT + (t0 + ti - u * UT) * C::TILE;
+          uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + tl.v_scale(col0 >> 5, 4 * c));
+          // rows past the context get a zero scale, whatever their bytes are
+          const int valid = st.ctx - ((st.tile + t0 + ti) << 4) - 4 * c;
+          if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
+          const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
+          uint32_t v[4 * NB][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
+#pragma unroll
+          for (int oc = 0; oc < NB / 2; ++oc) {
+            const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.v_codes((col0 >> 3) + oc, 4 * c));
+            const uint32_t ev0 = __byte_perm(x.x, x.y, 0x5410), od0 = __byte_perm(x.x, x.y, 0x7632);
+            const uint32_t ev1 = __byte_perm(x.z, x.w, 0x5410), od1 = __byte_perm(x.z, x.w, 0x7632);
+            uint32_t (*d)[2] = v + 8 * oc;
+            q4_word_h(ev0, s01, d[0][0], d[2][0], d[4][0], d[6][0]);
+            q4_word_h(od0, s01, d[1][0], d[3][0], d[5][0], d[7][0]);
+            q4_word_h(ev1, s23, d[0][1], d[2][1], d[4][1], d[6][1]);
+            q4_word_h(od1, s23, d[1][1], d[3][1], d[5][1], d[7][1]);
+          }
+          // block b: columns q NB + b of q = 2 hf (lanes 0..7 of the half) and 2 hf + 1 (lanes 8..15)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              tc::st_16x256(lane_base + (static_cast<uint32_t>(hf * 16) << 16) + C::AV + buf * 64 + b * (C::VT * 8) + ti * 8,
+                            v[2 * hf * NB + b][0], v[2 * hf * NB + b][1], v[(2 * hf + 1) * NB + b][0],
+                            v[(2 * hf + 1) * NB + b][1]);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&avf[buf]);
+          if (t0 + C::VT >= st.n || (t0 + C::VT) % UT == 0) mbar_arrive(&empty[ring]);
+        }
+      }
+      unit0 += (st.n + UT - 1) / UT;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ score products
+    if (lane == 0) {
+      const uint64_t qd = tc::desc_sw128(smem_u32(qs));
+      uint32_t kchunk = 0;
+      for (uint32_t i = 0; st.next(); ++i) {
+#pragma unroll 1
+        for (int kc = 0; kc < W / 128; ++kc, ++kchunk) {
+          const int buf = kchunk & 1;
+          wait(&akf[buf], (kchunk >> 1) & 1, kErrWaitFull);
+          tc::fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            tc::mma_ts(tmem + C::S + (i & 1) * 16, tmem + C::AK + buf * 64 + ks * 8,
+                       qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16, tc::idesc(0, 128, 16), kc | ks);
+          tc::commit(&ake[buf]);
+        }
+        tc::commit(&sf[i & 1]);
+      }
+      tc::commit(&drain[0]);
+      if (!mbar_wait(&drain[0], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ value products
+    if (lane == 0) {
+      const uint64_t pd = tc::desc_sw128(smem_u32(ps));
+      uint32_t vchunk = 0;
+      for (uint32_t i = 0; st.next(); ++i) {
+        wait(pf, i & 1, kErrWaitFull);
+        for (int t0 = 0; t0 < st.n; t0 += C::VT, ++vchunk) {
+          const int buf = vchunk & 1;
+          wait(&avf[buf], (vchunk >> 1) & 1, kErrWaitFull);
+          tc::fence_after();
+#pragma unroll
+          for (int ti = 0; ti < C::VT; ++ti) {
+            const int t = t0 + ti;
+            if (t >= st.n) break;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              tc::mma_ts(tmem + C::O + b * 16, tmem + C::AV + buf * 64 + b * (C::VT * 8) + ti * 8,
+                         pd + ((t >> 2) * 2048 + (t & 3) * 32) / 16, tc::idesc(0, 128, 16), !st.first || t > 0);
+          }
+          tc::commit(&ave[buf]);
+        }
+        tc::commit(pv);
+      }
+      tc::commit(&drain[1]);
+      if (!mbar_wait(&drain[1], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
+    }
+  } else {
+    // ------------------------------------------------------------------ tile copies
+    // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
+    const uint64_t policy = l2_policy_evict_first();
+    int unit = 0;
+    while (st.next()) {
+      for (int t0 = 0; t0 < st.n; t0 += UT, ++unit) {
+        const int ring = unit % C::UNITS, n = min(UT, st.n - t0);
+        const int t = st.tile + t0 + lane;
+        const int lp = t / p.tpp;
+        int blk = -1;
+        if (lane < n) {
+          if (lp < p.max_blocks) blk = p.bt[static_cast<int64_t>(st.r) * p.bt_st + lp];
+          if (blk < 0 || blk >= p.num_blocks) {
+            record_error(p.err, kErrBlock);
+            blk = -1;
+          }
+        }
+        if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
+        __syncwarp();
+        uint8_t* dst = units + ring * C::UNIT + lane * C::TILE;
+        const unsigned absent = __ballot_sync(0xffffffffu, lane < n && blk < 0);
+        if (lane < n && blk < 0) {  // a page outside the table or the cache reads as zeros
+          for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent)) * C::TILE);
+        __syncwarp();
+        if (lane < n && blk >= 0)
+          tc::bulk_load(dst, p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE,
+                        C::TILE, &full[ring], policy);
+      }
+    }
+    // after an abort no role may have waited for the last copies: they must land before the CTA ends
+    if (wait.aborted() && lane == 0)
+      for (int u = max(0, unit - C::UNITS); u < unit; ++u) mbar_wait(&full[u % C::UNITS], (u / C::UNITS) & 1, p.wait_ns);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::dealloc(tmem, 512);
 }
 
 template <int W>
 static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, cudaStream_t stream) {
+  using C = Q4Cfg<W>;
   Q4HistoryParams p;
   p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.q_st = a.q_st;
@@ -265,7 +681,7 @@ static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, 
   p.cache = static_cast<const uint8_t*>(a.cache);
   p.num_blocks = a.num_blocks;
   p.c_sb = a.cache_st_block;
-  p.page = a.page;
+  p.tpp = a.page / 16;
   p.bt = a.block_table;
   p.bt_st = a.bt_st;
   p.max_blocks = a.max_blocks;
@@ -278,13 +694,21 @@ static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, 
   p.ws_lse = plan.ws_lse;
   p.meta = plan.meta;
   p.slots_cap = plan.slots_cap;
-  p.grid = plan.grid;
   p.stream_mode = plan.stream_mode;
   p.err = a.err;
+  p.wait_ns = wait_limit_ns();
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // one CTA per SM (its ring and tensor memory fill one); within the slots the plan's workspace holds
+  const int grid = std::min(plan.grid, sms);
+  p.parts = grid;
+  static unsigned attr_mask = 0;
+  ensure_smem_limit(q4_history_kernel<W>, C::SMEM + 4 * (kHistoryMaxStreamRows + 1), attr_mask);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.grid);
-  cfg.blockDim = dim3(W / 4);
-  cfg.dynamicSmemBytes = plan.stream_mode ? (a.T + 1) * sizeof(int) : 0;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kQ4HistThreads);
+  cfg.dynamicSmemBytes = C::SMEM + (plan.stream_mode ? 4 * (a.T + 1) : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -5,8 +5,12 @@ Error bounds, each a sum of roundings counted at half a step (bf16 2^-8, fp32 2^
 * commit and gather are exact: same codes, same scales, values exact in bf16 for power-of-two tensor scales.
 * history: a score is an fp32 sum of exact products; a tensor-core step adds 16 products and truncates, so it is
   off by at most (W / 16 + 8) * 2^-22 * sum|q k| * scale =: d, which moves every p by a factor exp(+-2 d).  p is
-  rounded to bf16 for the value product (2^-8 of sum p|v| / l); the sums over rows add (rows / 16 + 8) * 2^-22;
+  rounded for the value product (at most 2^-8 of sum p|v| / l); the sums over rows add (rows / 16 + 8) * 2^-22;
   the result is rounded once (2^-8 |o|).  lse is off by d plus a few fp32 steps.
+  Small p: the kernel holds 2^11 p in f16, whose numbers below 2^-14 are multiples of 2^-24, so a p is off by at
+  most 2^-25 / 2^11 = 2^-36 where that is more than its relative rounding (a p of e^-59 becomes 0).  p is relative
+  to a base that is the maximum of some step's keys, so one key has p = 1 or more, l >= 1, and the error this adds
+  to sum p v / l is at most 2^-36 sum|v|.
 * linear: (K / 16 + 8) * 2^-22 * sum|x w| * scale, and the final rounding.
 """
 import numpy as np
@@ -90,7 +94,8 @@ class History:
                 assert (o[t] == 0).all() and np.isneginf(lse[:, t]).all()
                 continue
             d = (self.W / 16 + 8) * U32 * aq
-            tol = (U16 + 2 * d[:, None] + (k.shape[0] / 16 + 8) * U32) * av * 1.01 + U16 * 1.01 * np.abs(eo) + 1e-30
+            tol = ((U16 + 2 * d[:, None] + (k.shape[0] / 16 + 8) * U32) * av * 1.01 + U16 * 1.01 * np.abs(eo)
+                   + 2.0 ** -36 * np.abs(v).sum(0))
             assert (np.abs(o[t] - eo) <= tol).all(), (t, np.abs(o[t] - eo).max(), (np.abs(o[t] - eo) / tol).max())
             assert (np.abs(lse[:, t] - el) <= d + 8 * U32 * (1 + np.abs(el)) + (k.shape[0] / 16 + 8) * U32).all(), t
 
