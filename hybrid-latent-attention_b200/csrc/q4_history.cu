@@ -17,12 +17,15 @@
 //   S^T [128 keys x 16 heads]    = K [128 x W] (tensor memory) . Q^T (shared memory, f16)
 //   O^T [128 columns x 16 heads] += V^T [128 x 16 rows] (tensor memory) . P^T (shared memory, f16), W / 128 of them
 // One CTA per SM takes 128 rows ("step") at a time:
-//   warps 0-3  K: a thread dequantises one row into its lane; then the softmax of the step before: a thread has
-//              the 16 heads' scores of its key.  The exponent base of a head only moves when a score passes it by
-//              2^4 (a vote), so the output is rescaled rarely and the common step needs no reduction at all.
-//   warps 4-7  V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column).
-//   warp 8, 9  one thread each issues the score and the value products.
-//   warp 10    bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
+//   warps 0-3   K: a thread dequantises one row into its lane, 128 columns (a chunk) at a time.
+//   warps 4-7   V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column).
+//   warps 8-11  softmax: a thread has the 16 heads' scores of its key.  The exponent base of a head only moves when
+//               a score passes it by 2^4 (a vote), so the output is rescaled rarely and the common step needs no
+//               reduction at all.  They also write the segment's output.
+//   warp 12, 13 one thread each issues the score and the value products.
+//   warp 14     bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
+// The dequantising loops are kept rolled (about 250 instructions each): unrolled over a step they outgrew the
+// instruction caches, and the warps of a scheduler run different code.
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
 // of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
 // 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
@@ -63,16 +66,16 @@ struct Q4Cfg {
   static constexpr int UNIT = UT * TILE;         // 34816
   static constexpr int UNITS = 5;
   static constexpr int VT = UT / 2;              // tiles per V chunk: 64 tensor-memory columns
-  // Dequantise a step's K rows before the softmax of the step before?  Its V chunks may wait for that softmax,
-  // so the ring has to hold both steps.
-  static constexpr bool AHEAD = 2 * (8 / UT) <= UNITS;
+  static constexpr int BUFS = W == 1024 ? 2 : 3; // K and V chunks in tensor memory
   static constexpr int Q_BYTES = 32 * W;
   static constexpr int P_BYTES = 4096;
-  // tensor-memory columns: two K chunks (128 rows x 128 latent columns), two V chunks, two score tiles, output
-  static constexpr uint32_t AK = 0, AV = 128, S = 256, O = 288;
+  // tensor-memory columns: K chunks (128 rows x 128 latent columns), V chunks, two score tiles, output
+  static constexpr uint32_t AK = 0, AV = AK + BUFS * 64, S = AV + BUFS * 64, O = S + 32;
+  static_assert(O + NB * 16 <= 512, "tensor memory");
   static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
 };
-constexpr int kQ4HistThreads = 11 * 32;
+constexpr int kQSlots = 4;  // score factors of this many segments: the K warps run at most 3 segments ahead
+constexpr int kQ4HistThreads = 15 * 32;
 // log2 of how far a score may pass its head's exponent base before the base moves, and of the factor the
 // probabilities carry: together they end at 2^15, f16's largest power of two.  A small first term lets small
 // probabilities keep f16's precision, a large one makes rescales rare (each costs about one step).
@@ -165,18 +168,20 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   uint8_t* ctl = units + C::UNITS * C::UNIT;
   uint64_t* full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
   uint64_t* empty = full + C::UNITS;                  // [UNITS] unit read
-  uint64_t* akf = empty + C::UNITS;                   // [2] K chunk in tensor memory
-  uint64_t* ake = akf + 2;                            // [2] its MMAs are done
-  uint64_t* avf = ake + 2;                            // [2] V chunk
-  uint64_t* ave = avf + 2;
-  uint64_t* sf = ave + 2;                             // [2] scores of a step
-  uint64_t* pf = sf + 2;                              // probabilities of a step written
+  uint64_t* akf = empty + C::UNITS;                   // [BUFS] K chunk in tensor memory
+  uint64_t* ake = akf + C::BUFS;                      // [BUFS] its MMAs are done
+  uint64_t* avf = ake + C::BUFS;                      // [BUFS] V chunk
+  uint64_t* ave = avf + C::BUFS;
+  uint64_t* sf = ave + C::BUFS;                       // [2] scores of a step
+  uint64_t* se = sf + 2;                              // [2] read
+  uint64_t* qf = se + 2;                              // [kQSlots] score factors of a segment
+  uint64_t* pf = qf + kQSlots;                              // probabilities of a step written
   uint64_t* pv = pf + 1;                              // value products of a step done
   uint64_t* drain = pv + 1;                           // [2] every MMA of an issuer is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  float* qscale = reinterpret_cast<float*>(ctl + 256);  // [2][16] score factor of a head, by segment parity
-  float* red = qscale + 32;                             // [4][16] per-warp maxima / sums
+  float* qscale = reinterpret_cast<float*>(ctl + 384);  // [kQSlots][16] score factor of a head, by segment
+  float* red = qscale + kQSlots * 16;                   // [4][16] per-warp maxima / sums
   int* pref = reinterpret_cast<int*>(ctl + 1024);       // [T + 1] (stream mode)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -222,20 +227,24 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     p0 = blockIdx.x;  // rows blockIdx.x, + gridDim.x, ...
   }
 
-  if (warp == 8) tc::alloc(tmem_slot, 512);
-  if (tid == 9 * 32) {
+  if (warp == 12) tc::alloc(tmem_slot, 512);
+  if (tid == 13 * 32) {
     for (int s = 0; s < C::UNITS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 4 + (UT >= 8 ? 4 : UT / 2));  // the V warps, and the K warps of its tiles
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < C::BUFS; ++b) {
       mbar_init(&akf[b], 4);
       mbar_init(&ake[b], 1);
       mbar_init(&avf[b], 4);
       mbar_init(&ave[b], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&sf[b], 1);
+      mbar_init(&se[b], 4);
       mbar_init(&drain[b], 1);
     }
+    for (int b = 0; b < kQSlots; ++b) mbar_init(&qf[b], 4);
     mbar_init(pf, 4);
     mbar_init(pv, 1);
     *abort_flag = 0;
@@ -251,27 +260,16 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   Q4Walk st(p, pref, r0, p0, p1);
 
   if (warp < 4) {
-    // ------------------------------------------------------------------ K rows, softmax, output
+    // ------------------------------------------------------------------ K rows
     // Launched as a programmatic dependent of the launch that writes q, this grid has been copying tiles
-    // meanwhile; q and the workspace are touched only once that launch has completed.
+    // meanwhile; q is read only once that launch has completed.
     griddep_wait();
-    if (tid == 0) griddep_launch_dependents();
-    if (p.stream_mode && blockIdx.x == 0) {
-      for (int t = tid; t < p.T; t += 128) {
-        const int a = pref[t], b = pref[t + 1];
-        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
-                                      static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
-                          : make_int2(0, 0);
-      }
-    }
-    if (!p.stream_mode && warp == 0) {  // rows without history: their slot says so
-      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
-        if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
-    }
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int u0 = 2 * warp / UT, row = lane & 15;           // the unit of the step with this warp's two tiles
+    const int tile_off = (2 * warp - u0 * UT + (lane >> 4)) * C::TILE;
     int unit0 = 0;      // ring position of the step's first unit
-    uint32_t kchunk = 0;
-    int seg = -1;       // segments started (Q loads)
+    int buf = 0, bphase = 1;  // chunk buffer, and the parity of its last release
+    int seg = 0;
 
     auto load_q = [&](int r) {
       // 8 threads per head, W / 8 columns each
@@ -293,7 +291,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
       e = e > 110 ? 110 : (e < -110 ? -110 : e);
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      if (part == 0) qscale[(seg & 1) * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      if (part == 0) qscale[seg % kQSlots * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
       for (int i = 0; i < W / 64; ++i) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -307,34 +305,31 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         *reinterpret_cast<uint4*>(qs + (col >> 6) * 2048 + tc::sw128(h, (col >> 3) & 7)) = make_uint4(u[0], u[1], u[2], u[3]);
       }
       fence_proxy_async();
-      named_bar_sync(1, 128);  // the score factors
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qf[seg % kQSlots]);
+      ++seg;
     };
 
-    // dequantise this step's K rows: thread = row 32 warp + lane, chunk by chunk of 128 latent columns
-    auto dequant_k = [&]() {
-      const int t0 = 2 * warp;                    // this warp's first tile of the step
-      const int u = t0 / UT;
-      const bool unit_there = u * UT < st.n;
-      const int ring = (unit0 + u) % C::UNITS;
-      const int tiu = t0 - u * UT + (lane >> 4);  // tile inside the unit
-      const uint8_t* tb = units + ring * C::UNIT + tiu * C::TILE;
-      const int row = lane & 15;
-      if (unit_there) wait(&full[ring], ((unit0 + u) / C::UNITS) & 1, kErrWaitFull);
-      __syncwarp();
-      uint32_t sc[W / 128];                       // the row's scales, four groups to a word
-#pragma unroll
-      for (int i = 0; i < W / 128; ++i) sc[i] = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * i));
-#pragma unroll
-      for (int kc = 0; kc < W / 128; ++kc, ++kchunk) {
-        const int buf = kchunk & 1;
-        if (kchunk >= 2) wait(&ake[buf], ((kchunk >> 1) - 1) & 1, kErrWaitEmpty);
+    for (uint32_t i = 0; st.next(); ++i) {
+      if (st.first) {
+        if (i > 0) wait(&sf[(i - 1) & 1], ((i - 1) >> 1) & 1, kErrWaitFull);  // the scores before read Q no more
+        load_q(st.r);
+      }
+      const int ring = (unit0 + u0) % C::UNITS;
+      const bool unit_there = u0 * UT < st.n;
+      const uint8_t* tb = units + ring * C::UNIT + tile_off;
+      if (unit_there) wait(&full[ring], ((unit0 + u0) / C::UNITS) & 1, kErrWaitFull);
+#pragma unroll 1
+      for (int kc = 0; kc < W / 128; ++kc) {
+        wait(&ake[buf], bphase, kErrWaitEmpty);
         __syncwarp();
         tc::fence_after();
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * kc));
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t v[32];
           Q4ScaleH s0, s1;
-          q4_scales_h((sc[kc] >> (16 * hf)) & 0xffffu, s0, s1);
+          q4_scales_h((sc >> (16 * hf)) & 0xffffu, s0, s1);
 #pragma unroll
           for (int gi = 0; gi < 2; ++gi) {
             const uint4 c = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
@@ -353,12 +348,42 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           mbar_arrive(&akf[buf]);
           if (kc == W / 128 - 1 && unit_there) mbar_arrive(&empty[ring]);
         }
+        if (++buf == C::BUFS) {
+          buf = 0;
+          bphase ^= 1;
+        }
       }
       unit0 += (st.n + UT - 1) / UT;
-    };
-
+    }
+  } else if (warp >= 8 && warp < 12) {
+    // ------------------------------------------------------------------ softmax, output
+    // the workspace may still be read by what runs before the launch this grid waits for
+    griddep_wait();
+    const int stid = tid - 256, sw = warp - 8;
+    if (stid == 0) griddep_launch_dependents();
+    if (p.stream_mode && blockIdx.x == 0) {
+      for (int t = stid; t < p.T; t += 128) {
+        const int a = pref[t], b = pref[t + 1];
+        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
+                                      static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
+                          : make_int2(0, 0);
+      }
+    }
+    if (!p.stream_mode && sw == 0) {  // rows without history: their slot says so
+      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
+        if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
+    }
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(sw * 32) << 16);
+    const int key = 32 * sw + lane;
+    uint8_t* pk = ps + (key >> 6) * 2048 + (key & 7) * 2;
+    int seg = 0;
     float m[16], l[16];
-    auto softmax = [&](const Q4Walk& x, uint32_t i, int sseg) {
+    for (uint32_t i = 0; st.next(); ++i) {
+      if (st.first) {
+        wait(&qf[seg % kQSlots], (seg / kQSlots) & 1, kErrWaitFull);
+        ++seg;
+      }
+      const float4* fs = reinterpret_cast<const float4*>(qscale + (seg - 1) % kQSlots * 16);
       const int sb = i & 1;
       wait(&sf[sb], (i >> 1) & 1, kErrWaitFull);
       __syncwarp();
@@ -367,8 +392,9 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       tc::ld16(lane_base + C::S + sb * 16, raw);
       tc::wait_ld();
       tc::fence_before();
-      const bool live = (x.tile << 4) + 32 * warp + lane < x.ctx && (32 * warp + lane) < (x.n << 4);
-      const float4* fs = reinterpret_cast<const float4*>(qscale + (sseg & 1) * 16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&se[sb]);
+      const bool live = (st.tile << 4) + key < st.ctx && key < (st.n << 4);
       float s[16];
       float over = -INFINITY;
 #pragma unroll
@@ -379,7 +405,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         s[4 * h4 + 2] = live ? __uint_as_float(raw[4 * h4 + 2]) * f.z : -INFINITY;
         s[4 * h4 + 3] = live ? __uint_as_float(raw[4 * h4 + 3]) * f.w : -INFINITY;
       }
-      if (x.first) {
+      if (st.first) {
 #pragma unroll
         for (int h = 0; h < 16; ++h) {
           m[h] = -INFINITY;
@@ -393,13 +419,13 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       // of the step before have to be done for either
       if (i > 0) wait(pv, (i - 1) & 1, kErrWaitFull);
       __syncwarp();
-      if (named_bar_or(1, 128, x.first || over > kQ4Over)) {
+      if (named_bar_or(1, 128, st.first || over > kQ4Over)) {
         // new bases: the maximum over the step's keys, per head
         float mx[16];
 #pragma unroll
         for (int h = 0; h < 16; ++h) mx[h] = s[h];
         const float top = reduce16<true>(mx, lane);
-        if (lane < 16) red[warp * 16 + rev16(lane)] = top;
+        if (lane < 16) red[sw * 16 + rev16(lane)] = top;
         named_bar_sync(1, 128);
         float al[16];
 #pragma unroll
@@ -409,7 +435,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           m[h] = mn;
           l[h] *= al[h];
         }
-        if (!x.first) {
+        if (!st.first) {
           tc::fence_after();
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
@@ -425,8 +451,6 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         }
         named_bar_sync(1, 128);  // red is read before it is written again
       }
-      const int key = 32 * warp + lane;
-      uint8_t* pk = ps + (key >> 6) * 2048 + (key & 7) * 2;
 #pragma unroll
       for (int h = 0; h < 16; ++h) {
         const float e = s[h] == -INFINITY ? 0.f : exp2f(s[h] - m[h] + kQ4Lift);
@@ -436,21 +460,21 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(pf);
-    };
+      if (!st.last) continue;
 
-    auto write_out = [&](const Q4Walk& x, uint32_t i) {
+      // ---- segment end: the normalised partial and its lse
       float t[16];
 #pragma unroll
       for (int h = 0; h < 16; ++h) t[h] = l[h];
       const float sum = reduce16<false>(t, lane);
-      if (lane < 16) red[warp * 16 + rev16(lane)] = sum;
+      if (lane < 16) red[sw * 16 + rev16(lane)] = sum;
       named_bar_sync(1, 128);
       float inv[16];
 #pragma unroll
       for (int h = 0; h < 16; ++h) inv[h] = red[h] + red[16 + h] + red[32 + h] + red[48 + h];
-      const bool room = x.slot < p.slots_cap;
-      if (!room && tid == 0) record_error(p.err, kErrSlots);
-      if (room && warp == 0) {
+      const bool room = st.slot < p.slots_cap;
+      if (!room && stid == 0) record_error(p.err, kErrSlots);
+      if (room && sw == 0) {
         float mine_m = 0.f, mine_l = 1.f;
 #pragma unroll
         for (int h = 0; h < 16; ++h)
@@ -459,7 +483,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
             mine_l = inv[h];
           }
         if (lane < p.H)
-          p.ws_lse[static_cast<int64_t>(x.slot) * p.H + lane] = (mine_m + (log2f(mine_l) - kQ4Lift)) * 0.6931471805599453f;
+          p.ws_lse[static_cast<int64_t>(st.slot) * p.H + lane] = (mine_m + (log2f(mine_l) - kQ4Lift)) * 0.6931471805599453f;
       }
 #pragma unroll
       for (int h = 0; h < 16; ++h) inv[h] = inv[h] == 0.f ? 0.f : p.v_ts / inv[h];  // 0: every score is -inf
@@ -468,7 +492,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       tc::fence_after();
       // lane 8 q + g of warp w holds columns (8 w + g) 4 NB + q NB .. + NB - 1, one per block
       constexpr int NV = NB < 4 ? NB : 4;
-      const int col = (8 * warp + (lane & 7)) * 4 * NB + (lane >> 3) * NB;
+      const int col = (8 * sw + (lane & 7)) * 4 * NB + (lane >> 3) * NB;
 #pragma unroll
       for (int b0 = 0; b0 < NB; b0 += NV) {
         uint32_t o[NV][16];
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
 #pragma unroll
           for (int h = 0; h < 16; ++h) {
             if (h >= p.H) continue;
-            float* dst = p.ws_o + (static_cast<int64_t>(x.slot) * p.H + h) * W + col + b0;
+            float* dst = p.ws_o + (static_cast<int64_t>(st.slot) * p.H + h) * W + col + b0;
             if constexpr (NV == 4)
               *reinterpret_cast<float4*>(dst) =
                   make_float4(__uint_as_float(o[0][h]) * inv[h], __uint_as_float(o[1][h]) * inv[h],
@@ -492,53 +516,22 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       }
       tc::fence_before();
       named_bar_sync(1, 128);  // red is read before it is written again
-    };
-
-    if (st.next()) {
-      Q4Walk cur = st;
-      ++seg;
-      load_q(st.r);
-      dequant_k();
-      for (uint32_t i = 0;; ++i) {
-        const int cur_seg = seg;
-        const bool more = st.next();
-        if (more && C::AHEAD) {
-          if (st.first) {
-            wait(&sf[i & 1], (i >> 1) & 1, kErrWaitFull);  // the scores of step i read Q no more
-            ++seg;
-            load_q(st.r);
-          }
-          dequant_k();
-        }
-        softmax(cur, i, cur_seg);
-        if (cur.last) write_out(cur, i);
-        if (!more) break;
-        if (!C::AHEAD) {
-          if (st.first) {
-            ++seg;
-            load_q(st.r);
-          }
-          dequant_k();
-        }
-        cur.r = st.r; cur.tile = st.tile; cur.n = st.n; cur.ctx = st.ctx; cur.slot = st.slot;
-        cur.first = st.first; cur.last = st.last;
-      }
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------------ V columns
     const int w = warp - 4, g = lane >> 2, c = lane & 3;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
     const int col0 = (8 * w + g) * 4 * NB;  // this thread's 4 NB columns
-    int unit0 = 0;
-    uint32_t vchunk = 0;
+    int unit0 = 0, buf = 0, bphase = 1;
     while (st.next()) {
-      for (int t0 = 0; t0 < st.n; t0 += C::VT, ++vchunk) {
-        const int u = t0 / UT, ring = (unit0 + u) % C::UNITS, buf = vchunk & 1;
+#pragma unroll 1
+      for (int t0 = 0; t0 < st.n; t0 += C::VT) {
+        const int u = t0 / UT, ring = (unit0 + u) % C::UNITS;
         if (t0 == u * UT) wait(&full[ring], ((unit0 + u) / C::UNITS) & 1, kErrWaitFull);
-        if (vchunk >= 2) wait(&ave[buf], ((vchunk >> 1) - 1) & 1, kErrWaitEmpty);
+        wait(&ave[buf], bphase, kErrWaitEmpty);
         __syncwarp();
         tc::fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int ti = 0; ti < C::VT; ++ti) {
           if (t0 + ti >= st.n) break;
           const uint8_t* tb = units + ring * C::UNIT + (t0 + ti - u * UT) * C::TILE;
@@ -575,43 +568,51 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           mbar_arrive(&avf[buf]);
           if (t0 + C::VT >= st.n || (t0 + C::VT) % UT == 0) mbar_arrive(&empty[ring]);
         }
+        if (++buf == C::BUFS) {
+          buf = 0;
+          bphase ^= 1;
+        }
       }
       unit0 += (st.n + UT - 1) / UT;
     }
-  } else if (warp == 8) {
+  } else if (warp == 12) {
     // ------------------------------------------------------------------ score products
     if (lane == 0) {
       const uint64_t qd = tc::desc_sw128(smem_u32(qs));
-      uint32_t kchunk = 0;
+      int buf = 0, bphase = 0;
       for (uint32_t i = 0; st.next(); ++i) {
+        if (i >= 2) wait(&se[i & 1], ((i >> 1) - 1) & 1, kErrWaitEmpty);
 #pragma unroll 1
-        for (int kc = 0; kc < W / 128; ++kc, ++kchunk) {
-          const int buf = kchunk & 1;
-          wait(&akf[buf], (kchunk >> 1) & 1, kErrWaitFull);
+        for (int kc = 0; kc < W / 128; ++kc) {
+          wait(&akf[buf], bphase, kErrWaitFull);
           tc::fence_after();
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
             tc::mma_ts(tmem + C::S + (i & 1) * 16, tmem + C::AK + buf * 64 + ks * 8,
                        qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16, tc::idesc(0, 128, 16), kc | ks);
           tc::commit(&ake[buf]);
+          if (++buf == C::BUFS) {
+            buf = 0;
+            bphase ^= 1;
+          }
         }
         tc::commit(&sf[i & 1]);
       }
       tc::commit(&drain[0]);
       if (!mbar_wait(&drain[0], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
     }
-  } else if (warp == 9) {
+  } else if (warp == 13) {
     // ------------------------------------------------------------------ value products
     if (lane == 0) {
       const uint64_t pd = tc::desc_sw128(smem_u32(ps));
-      uint32_t vchunk = 0;
+      int buf = 0, bphase = 0;
       for (uint32_t i = 0; st.next(); ++i) {
         wait(pf, i & 1, kErrWaitFull);
-        for (int t0 = 0; t0 < st.n; t0 += C::VT, ++vchunk) {
-          const int buf = vchunk & 1;
-          wait(&avf[buf], (vchunk >> 1) & 1, kErrWaitFull);
+#pragma unroll 1
+        for (int t0 = 0; t0 < st.n; t0 += C::VT) {
+          wait(&avf[buf], bphase, kErrWaitFull);
           tc::fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int ti = 0; ti < C::VT; ++ti) {
             const int t = t0 + ti;
             if (t >= st.n) break;
@@ -621,6 +622,10 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
                          pd + ((t >> 2) * 2048 + (t & 3) * 32) / 16, tc::idesc(0, 128, 16), !st.first || t > 0);
           }
           tc::commit(&ave[buf]);
+          if (++buf == C::BUFS) {
+            buf = 0;
+            bphase ^= 1;
+          }
         }
         tc::commit(pv);
       }
@@ -668,7 +673,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::dealloc(tmem, 512);
+  if (warp == 12) tc::dealloc(tmem, 512);
 }
 
 template <int W>

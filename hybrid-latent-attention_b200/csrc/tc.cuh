@@ -91,18 +91,31 @@ struct Waits {
   int* err;
   uint64_t limit_ns;
   __device__ __forceinline__ bool aborted() const { return *reinterpret_cast<volatile int*>(abort_flag) != 0; }
+  // One try suspends the thread for up to 20 us: a waiting warp takes few issue slots from the working ones.
+  __device__ __forceinline__ bool attempt(uint64_t* bar, uint32_t parity) const {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok != 0;
+  }
   __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity, int code) const {
-    if (mbar_try_wait(bar, parity)) return;
+    if (!attempt(bar, parity)) retry(bar, parity, code);
+  }
+  __device__ __noinline__ void retry(uint64_t* bar, uint32_t parity, int code) const {
     const uint64_t t0 = global_ns();
-    for (uint32_t it = 1;; ++it) {
-      if (mbar_try_wait(bar, parity)) return;
-      if ((it & 63u) == 0u) {
-        if (aborted()) return;
-        if (global_ns() - t0 > limit_ns) {
-          record_error(err, code);
-          atomicExch(abort_flag, 1);
-          return;
-        }
+    while (!attempt(bar, parity)) {
+      if (aborted()) return;
+      if (global_ns() - t0 > limit_ns) {
+        record_error(err, code);
+        atomicExch(abort_flag, 1);
+        return;
       }
     }
   }
