@@ -56,6 +56,7 @@ struct Q4HistoryParams {
   float* ws_lse;
   int2* meta;
   int32_t slots_cap, parts, stream_mode;  // parts: CTAs of the page partition (stream mode)
+  uint32_t sixteen;  // 16 (q4_word_h)
   int* err;
   uint64_t wait_ns;
 };
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   const uint32_t tmem = *tmem_slot;
   const tc::Waits wait{abort_flag, p.err, p.wait_ns};
   const Q4Tile tl(W);
+  const uint32_t sixteen = p.sixteen;
   Q4Walk st(p, pref, r0, p0, p1);
 
   if (warp < 8) {
@@ -348,10 +350,10 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           for (int gi = 0; gi < 2; ++gi) {
             const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
             uint32_t v[16];
-            q4_word_h(x.x, s[gi], v[0], v[1], v[2], v[3]);
-            q4_word_h(x.y, s[gi], v[4], v[5], v[6], v[7]);
-            q4_word_h(x.z, s[gi], v[8], v[9], v[10], v[11]);
-            q4_word_h(x.w, s[gi], v[12], v[13], v[14], v[15]);
+            q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
+            q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
+            q4_word_h(x.z, s[gi], sixteen, v[8], v[9], v[10], v[11]);
+            q4_word_h(x.w, s[gi], sixteen, v[12], v[13], v[14], v[15]);
             tc::st16(lane_base + C::AK + buf * 64 + (2 * hf + gi) * 16, v);
           }
         }
@@ -391,8 +393,10 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
             const uint8_t* tb = ub + (t0 + ti) * C::TILE;
             uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + tl.v_scale(col0 >> 5, 4 * c));
             // rows past the context get a zero scale, whatever their bytes are
-            const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
-            if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
+            if (st.last) {
+              const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
+              if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
+            }
             const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
             const uint32_t at = lane_base + C::AV + buf * C::VCOLS + ti * 8;
             constexpr int OH = NB >= 4 ? NB / 4 : 1;  // octets per half of the lanes (width 256: one for both)
@@ -403,10 +407,10 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
               for (int oc = 0; oc < OH; ++oc) {
                 const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.v_codes((col0 >> 3) + o0 + oc, 4 * c));
                 uint32_t (*d)[2] = v + 8 * oc;
-                q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, d[0][0], d[2][0], d[4][0], d[6][0]);
-                q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, d[1][0], d[3][0], d[5][0], d[7][0]);
-                q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, d[0][1], d[2][1], d[4][1], d[6][1]);
-                q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, d[1][1], d[3][1], d[5][1], d[7][1]);
+                q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
+                q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, sixteen, d[0][1], d[2][1], d[4][1], d[6][1]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, sixteen, d[1][1], d[3][1], d[5][1], d[7][1]);
               }
               // block b: columns q NB + b of q = 2 hf (lanes 0..7 of half hf) and 2 hf + 1 (lanes 8..15)
               constexpr int HALVES = NB >= 4 ? 1 : 2;
@@ -472,14 +476,17 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       __syncwarp();
       if (lane == 0) mbar_arrive(&se[sb]);
       // a step that is not full: dead keys score -inf
-      const bool dead = (st.tile << 4) + key >= st.ctx || key >= (st.n << 4);
+      const bool dead = st.last && ((st.tile << 4) + key >= st.ctx || key >= (st.n << 4));
       float x[8], over = -INFINITY;
       if (!st.first) {
 #pragma unroll
-        for (int h = 0; h < 8; ++h) {
-          x[h] = dead ? -INFINITY : fmaf(__uint_as_float(raw[h]), f[h], -mm[h]);
-          over = fmaxf(over, x[h]);
+        for (int h = 0; h < 8; ++h) x[h] = fmaf(__uint_as_float(raw[h]), f[h], -mm[h]);
+        if (dead) {
+#pragma unroll
+          for (int h = 0; h < 8; ++h) x[h] = -INFINITY;
         }
+#pragma unroll
+        for (int h = 0; h < 8; ++h) over = fmaxf(over, x[h]);
       }
       if (i > 1) wait(&pv[sb], ((i - 2) >> 1) & 1, kErrWaitFull);  // these probabilities replace those of step i - 2
       __syncwarp();
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     }
   } else if (warp == 24) {
     // ------------------------------------------------------------------ score products
-    if (lane == 0) {
+    if (tc::elect()) {
       const uint64_t qd = tc::desc_sw128(smem_u32(qs));
       uint32_t c = 0;
       int seg = 0;
@@ -594,15 +601,17 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           ++seg;
         }
         if (i >= 2) wait(&se[i & 1], ((i >> 1) - 1) & 1, kErrWaitEmpty);
-#pragma unroll 1
+        const uint32_t d = tmem + C::S + (i & 1) * 16;
+#pragma unroll
         for (int kc = 0; kc < W / 128; ++kc, ++c) {
           const uint32_t buf = c % C::BUFS;
           wait(&akf[buf], (c / C::BUFS) & 1, kErrWaitFull);
           tc::fence_after();
+          const uint32_t a = tmem + C::AK + buf * 64;
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            tc::mma_ts(tmem + C::S + (i & 1) * 16, tmem + C::AK + buf * 64 + ks * 8,
-                       qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16, tc::idesc(0, 128, 16), kc | ks);
+            tc::mma_ts(d, a + ks * 8, qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16, tc::idesc(0, 128, 16),
+                       kc | ks);
           tc::commit(&ake[buf]);
         }
         tc::commit(&sf[i & 1]);
@@ -612,24 +621,27 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     }
   } else if (warp == 25) {
     // ------------------------------------------------------------------ value products
-    if (lane == 0) {
-      const uint64_t pd = tc::desc_sw128(smem_u32(ps));
+    if (tc::elect()) {
       uint32_t c = 0;
       for (uint32_t i = 0; st.next(); ++i) {
         wait(&pf[i & 1], (i >> 1) & 1, kErrWaitFull);
-#pragma unroll 1
-        for (int t0 = 0; t0 < st.n; t0 += C::VT, ++c) {
+        const uint64_t pd = tc::desc_sw128(smem_u32(ps) + (i & 1) * 4096);
+        const uint32_t keep = !st.first;
+#pragma unroll
+        for (int t0 = 0; t0 < 8; t0 += C::VT, ++c) {
+          if (t0 >= st.n) break;
           const uint32_t buf = c % C::BUFS;
           wait(&avf[buf], (c / C::BUFS) & 1, kErrWaitFull);
           tc::fence_after();
-#pragma unroll 1
+          const uint32_t a = tmem + C::AV + buf * C::VCOLS;
+#pragma unroll
           for (int ti = 0; ti < C::VT; ++ti) {
             const int t = t0 + ti;
             if (t >= st.n) break;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-              tc::mma_ts(tmem + C::O + b * 16, tmem + C::AV + buf * C::VCOLS + b * (C::VT * 8) + ti * 8,
-                         pd + ((i & 1) * 4096 + (t >> 2) * 2048 + (t & 3) * 32) / 16, tc::idesc(0, 128, 16), !st.first || t > 0);
+              tc::mma_ts(tmem + C::O + b * 16, a + b * (C::VT * 8) + ti * 8, pd + ((t >> 2) * 2048 + (t & 3) * 32) / 16,
+                         tc::idesc(0, 128, 16), t ? 1u : keep);
           }
           tc::commit(&ave[buf]);
         }
@@ -706,6 +718,7 @@ static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, 
   p.meta = plan.meta;
   p.slots_cap = plan.slots_cap;
   p.stream_mode = plan.stream_mode;
+  p.sixteen = 16;
   p.err = a.err;
   p.wait_ns = wait_limit_ns();
   int dev = 0, sms = 148;

@@ -23,6 +23,20 @@ __host__ __device__ constexpr uint32_t idesc(int type, int m, int n) {
   return (1u << 4) | (uint32_t(type) << 7) | (uint32_t(type) << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
+// True in one lane of a converged warp.  MMAs are issued under this predicate and in unrolled code: the operands
+// of tcgen05.mma are uniform registers, and under `lane == 0` or in a rolled loop the compiler moves them there one
+// instruction after the other (150 and 100 clocks an MMA; 9 as written, for M = 128, N = 16 with A in tensor memory).
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(p));
+  return p != 0;
+}
 // D[tmem] (+)= A[tmem] . B[smem]^T
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
