@@ -17,15 +17,18 @@
 //   S^T [128 keys x 16 heads]    = K [128 x W] (tensor memory) . Q^T (shared memory, f16)
 //   O^T [128 columns x 16 heads] += V^T [128 x 16 rows] (tensor memory) . P^T (shared memory, f16), W / 128 of them
 // One CTA per SM takes 128 rows ("step") at a time:
-//   warps 0-7   K: a thread dequantises one row into its lane, 128 columns (a chunk) at a time; the two groups of
+//   warps 0-7   softmax: a thread has the scores of its key for the 8 heads of its group of four warps.  The
+//               exponent base of a head only moves when a score passes it by 2^4 (a vote), so the output is rescaled
+//               rarely and the common step needs no reduction at all.  They also write the segment's output.
+//   warp 8, 9   one thread each issues the score and the value products.
+//   warp 10, 11 bulk copies of the K and the V half of tiles into rings of 4 and 6 units of 17408 bytes (the halves
+//               of 2, 4 or 8 tiles).  Two rings, because V is used a step later than K: in one ring the V halves
+//               kept the room that the next copies needed.
+//   warps 12-19 K: a thread dequantises one row into its lane, 128 columns (a chunk) at a time; the two groups of
 //               four warps take turns.
-//   warps 8-15  V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column);
+//   warps 20-27 V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column);
 //               two groups as well.
-//   warps 16-23 softmax: a thread has the scores of its key for the 8 heads of its group.  The exponent base of a
-//               head only moves when a score passes it by 2^4 (a vote), so the output is rescaled rarely and the
-//               common step needs no reduction at all.  They also write the segment's output.
-//   warp 24, 25 one thread each issues the score and the value products.
-//   warp 26     bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
+// The warps whose latency the others wait for come first: the schedulers prefer the lower of two ready warps.
 // The dequantising loops are kept rolled: unrolled over a step they outgrew the instruction caches, and the warps
 // of a scheduler run different code (190 us unrolled with one group of each, 137 us rolled with a softmax group).
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
@@ -66,8 +69,9 @@ struct Q4Cfg {
   static constexpr int NB = W / 128;             // blocks of 128 latent columns (output accumulators)
   static constexpr int TILE = 17 * W;            // bytes of 16 rows
   static constexpr int UT = 2048 / W;            // tiles per ring unit
-  static constexpr int UNIT = UT * TILE;         // 34816
-  static constexpr int UNITS = 5;
+  static constexpr int SCALES = 16384;           // a unit: the codes of its tiles (8 W bytes each), then their scales
+  static constexpr int UNIT = SCALES + 1024;
+  static constexpr int KU = 4, VU = 6;           // units of the K and of the V ring
   static constexpr int VT = W == 256 ? 2 : 1;    // tiles per V chunk
   static constexpr int VCOLS = NB * VT * 8;      // its tensor-memory columns
   static constexpr int BUFS = W == 1024 ? 2 : 4; // K chunks and V chunks in tensor memory
@@ -76,10 +80,10 @@ struct Q4Cfg {
   // tensor-memory columns: K chunks (128 rows x 128 latent columns), V chunks, two score tiles, output
   static constexpr uint32_t AK = 0, AV = AK + BUFS * 64, S = AV + BUFS * VCOLS, O = S + 32;
   static_assert(O + NB * 16 <= 512, "tensor memory");
-  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
+  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + (KU + VU) * UNIT + 1024;  // + 4 (T + 1) in stream mode
 };
 constexpr int kQSlots = 4;  // score factors of this many segments: the K warps run at most 3 segments ahead
-constexpr int kQ4HistThreads = 27 * 32;
+constexpr int kQ4HistThreads = 28 * 32;
 // log2 of how far a score may pass its head's exponent base before the base moves, and of the factor the
 // probabilities carry: together they end at 2^15, f16's largest power of two.  A small first term lets small
 // probabilities keep f16's precision, a large one makes rescales rare (each costs about one step).
@@ -179,11 +183,14 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;
   uint8_t* ps = qs + C::Q_BYTES;
-  uint8_t* units = ps + C::P_BYTES;
-  uint8_t* ctl = units + C::UNITS * C::UNIT;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
-  uint64_t* empty = full + C::UNITS;                  // [UNITS] unit read
-  uint64_t* akf = empty + C::UNITS;                   // [BUFS] K chunk in tensor memory
+  uint8_t* kunits = ps + C::P_BYTES;
+  uint8_t* vunits = kunits + C::KU * C::UNIT;
+  uint8_t* ctl = vunits + C::VU * C::UNIT;
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(ctl);  // [KU] unit copied
+  uint64_t* kempty = kfull + C::KU;                   // [KU] unit read
+  uint64_t* vfull = kempty + C::KU;                   // [VU]
+  uint64_t* vempty = vfull + C::VU;
+  uint64_t* akf = vempty + C::VU;                     // [BUFS] K chunk in tensor memory
   uint64_t* ake = akf + C::BUFS;                      // [BUFS] its MMAs are done
   uint64_t* avf = ake + C::BUFS;                      // [BUFS] V chunk
   uint64_t* ave = avf + C::BUFS;
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   uint64_t* drain = pv + 2;                           // [2] every MMA of an issuer is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  float* qscale = reinterpret_cast<float*>(ctl + 384);  // [kQSlots][16] score factor of a head, by segment
+  float* qscale = reinterpret_cast<float*>(ctl + 512);  // [kQSlots][16] score factor of a head, by segment
   float* red = qscale + kQSlots * 16;                   // [2][4][8] per-warp maxima / sums
   int* pref = reinterpret_cast<int*>(ctl + 1024);       // [T + 1] (stream mode)
 
@@ -242,11 +249,15 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     p0 = blockIdx.x;  // rows blockIdx.x, + gridDim.x, ...
   }
 
-  if (warp == 24) tc::alloc(tmem_slot, 512);
-  if (tid == 25 * 32) {
-    for (int s = 0; s < C::UNITS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 8 + UT);  // the V warps, and the K warps of its tiles (one for two tiles in each group)
+  if (warp == 8) tc::alloc(tmem_slot, 512);
+  if (tid == 9 * 32) {
+    for (int u = 0; u < C::KU; ++u) {
+      mbar_init(&kfull[u], 1);
+      mbar_init(&kempty[u], UT);  // the K warps of its tiles: one for two tiles in each group
+    }
+    for (int u = 0; u < C::VU; ++u) {
+      mbar_init(&vfull[u], 1);
+      mbar_init(&vempty[u], 8);
     }
     for (int b = 0; b < C::BUFS; ++b) {
       mbar_init(&akf[b], 4);
@@ -276,178 +287,20 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   Q4Walk st(p, pref, r0, p0, p1);
 
   if (warp < 8) {
-    // ------------------------------------------------------------------ K rows
-    // Launched as a programmatic dependent of the launch that writes q, this grid has been copying tiles
-    // meanwhile; q is read only once that launch has completed.
-    griddep_wait();
-    const int grp = warp >> 2, w = warp & 3;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
-    const int u0 = 2 * w / UT, row = lane & 15;              // the unit of the step with this warp's two tiles
-    const int tile_off = (2 * w - u0 * UT + (lane >> 4)) * C::TILE;
-    int unit0 = 0;        // ring position of the step's first unit
-    uint32_t chunk = 0;   // chunks before this step
-    int seg = 0;
-    for (uint32_t i = 0; st.next(); ++i) {
-      if (st.first) {
-        if (i > 0) wait(&sf[(i - 1) & 1], ((i - 1) >> 1) & 1, kErrWaitFull);  // the scores before read Q no more
-        // the row's queries: 16 threads per head, W / 16 columns each
-        const int h = tid >> 4, part = tid & 15;
-        const __nv_bfloat16* src = p.q + static_cast<int64_t>(st.r) * p.q_st + static_cast<int64_t>(h) * p.q_sh + part * (W / 16);
-        uint4 v[W / 128];
-        float amax = 0.f;
-#pragma unroll
-        for (int k = 0; k < W / 128; ++k) {
-          v[k] = h < p.H ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[j] << 16)), fabsf(__uint_as_float(x[j] & 0xffff0000u))));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // a power of two that puts the head's largest element into [2^12, 2^13) (an infinity stays one)
-        int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
-        e = e > 110 ? 110 : (e < -110 ? -110 : e);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        if (part == 0) qscale[seg % kQSlots * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-        for (int k = 0; k < W / 128; ++k) {
-          const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-          uint32_t u[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 hh = __floats2half2_rn(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
-            u[j] = *reinterpret_cast<const uint32_t*>(&hh);
-          }
-          const int col = part * (W / 16) + 8 * k;
-          *reinterpret_cast<uint4*>(qs + (col >> 6) * 2048 + tc::sw128(h, (col >> 3) & 7)) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&qf[seg % kQSlots]);
-        ++seg;
-      } else if (i > 1) {
-        // keeps a warp that runs ahead within two steps, so that the wait above never meets an older phase
-        wait(&sf[i & 1], ((i - 2) >> 1) & 1, kErrWaitFull);
-      }
-      const int ring = (unit0 + u0) % C::UNITS;
-      const bool unit_there = u0 * UT < st.n;
-      const uint8_t* tb = units + ring * C::UNIT + tile_off;
-      if (unit_there) wait(&full[ring], ((unit0 + u0) / C::UNITS) & 1, kErrWaitFull);
-#pragma unroll 1
-      for (int kc = grp; kc < W / 128; kc += 2) {
-        const uint32_t c = chunk + kc, buf = c % C::BUFS;
-        wait(&ake[buf], ((c / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
-        __syncwarp();
-        tc::fence_after();
-        const uint32_t sc = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * kc));
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          Q4ScaleH s[2];
-          q4_scales_h((sc >> (16 * hf)) & 0xffffu, s[0], s[1]);
-#pragma unroll
-          for (int gi = 0; gi < 2; ++gi) {
-            const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
-            uint32_t v[16];
-            q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
-            q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
-            q4_word_h(x.z, s[gi], sixteen, v[8], v[9], v[10], v[11]);
-            q4_word_h(x.w, s[gi], sixteen, v[12], v[13], v[14], v[15]);
-            tc::st16(lane_base + C::AK + buf * 64 + (2 * hf + gi) * 16, v);
-          }
-        }
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&akf[buf]);
-      }
-      if (lane == 0 && unit_there) mbar_arrive(&empty[ring]);
-      unit0 += (st.n + UT - 1) / UT;
-      chunk += W / 128;
-    }
-  } else if (warp < 16) {
-    // ------------------------------------------------------------------ V columns
-    const int w = warp & 3, g = lane >> 2, c = lane & 3;
-    const uint32_t grp = (warp >> 2) & 1;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
-    const int col0 = (8 * w + g) * 4 * NB;  // this thread's 4 NB columns
-    int unit = 0;
-    uint32_t chunk = 0;
-    while (st.next()) {
-      for (int ut = 0; ut < st.n; ut += UT, ++unit) {
-        const int ring = unit % C::UNITS;
-        const uint8_t* ub = units + ring * C::UNIT;
-        wait(&full[ring], (unit / C::UNITS) & 1, kErrWaitFull);
-        const int tiles = min(UT, st.n - ut);
-#pragma unroll 1
-        for (int t0 = ((chunk + ut / C::VT) & 1) == grp ? 0 : C::VT; t0 < tiles; t0 += 2 * C::VT) {
-          // chunks alternate between the groups over all steps, so that a buffer always belongs to the same group:
-          // a group that met a buffer's barrier out of turn could take an older phase for the one it waits for
-          const uint32_t ch = chunk + (ut + t0) / C::VT, buf = ch % C::BUFS;
-          wait(&ave[buf], ((ch / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
-          __syncwarp();
-          tc::fence_after();
-#pragma unroll 1
-          for (int ti = 0; ti < C::VT && t0 + ti < tiles; ++ti) {
-            const uint8_t* tb = ub + (t0 + ti) * C::TILE;
-            uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + tl.v_scale(col0 >> 5, 4 * c));
-            // rows past the context get a zero scale, whatever their bytes are
-            if (st.last) {
-              const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
-              if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
-            }
-            const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
-            const uint32_t at = lane_base + C::AV + buf * C::VCOLS + ti * 8;
-            constexpr int OH = NB >= 4 ? NB / 4 : 1;  // octets per half of the lanes (width 256: one for both)
-#pragma unroll
-            for (int o0 = 0; o0 < NB / 2; o0 += OH) {
-              uint32_t v[8 * OH][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
-#pragma unroll
-              for (int oc = 0; oc < OH; ++oc) {
-                const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.v_codes((col0 >> 3) + o0 + oc, 4 * c));
-                uint32_t (*d)[2] = v + 8 * oc;
-                q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
-                q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
-                q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, sixteen, d[0][1], d[2][1], d[4][1], d[6][1]);
-                q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, sixteen, d[1][1], d[3][1], d[5][1], d[7][1]);
-              }
-              // block b: columns q NB + b of q = 2 hf (lanes 0..7 of half hf) and 2 hf + 1 (lanes 8..15)
-              constexpr int HALVES = NB >= 4 ? 1 : 2;
-#pragma unroll
-              for (int hl = 0; hl < HALVES; ++hl) {
-                const int hf = NB >= 4 ? o0 / OH : hl;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                  tc::st_16x256(at + (static_cast<uint32_t>(hf * 16) << 16) + b * (C::VT * 8), v[2 * hl * NB + b][0],
-                                v[2 * hl * NB + b][1], v[(2 * hl + 1) * NB + b][0], v[(2 * hl + 1) * NB + b][1]);
-              }
-            }
-          }
-          tc::wait_st();
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&avf[buf]);
-        }
-        if (lane == 0) mbar_arrive(&empty[ring]);
-      }
-      chunk += (st.n + C::VT - 1) / C::VT;
-    }
-  } else if (warp < 24) {
     // ------------------------------------------------------------------ softmax, output: heads 8 grp .. + 7
     // the workspace may still be read by what runs before the launch this grid waits for
     griddep_wait();
-    const int grp = (warp >> 2) & 1, w = warp & 3, h0 = 8 * grp;
-    if (warp == 16 && lane == 0) griddep_launch_dependents();
+    const int grp = warp >> 2, w = warp & 3, h0 = 8 * grp;
+    if (tid == 0) griddep_launch_dependents();
     if (p.stream_mode && blockIdx.x == 0) {
-      for (int t = tid - 512; t < p.T; t += 256) {
+      for (int t = tid; t < p.T; t += 256) {
         const int a = pref[t], b = pref[t + 1];
         p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
                                       static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
                           : make_int2(0, 0);
       }
     }
-    if (!p.stream_mode && warp == 16) {  // rows without history: their slot says so
+    if (!p.stream_mode && warp == 0) {  // rows without history: their slot says so
       for (int r = blockIdx.x; r < p.T; r += gridDim.x)
         if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
     }
@@ -589,7 +442,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       tc::fence_before();
       named_bar_sync(bar, 128);  // myred is read before it is written again
     }
-  } else if (warp == 24) {
+  } else if (warp == 8) {
     // ------------------------------------------------------------------ score products
     if (tc::elect()) {
       const uint64_t qd = tc::desc_sw128(smem_u32(qs));
@@ -619,7 +472,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       tc::commit(&drain[0]);
       if (!mbar_wait(&drain[0], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
     }
-  } else if (warp == 25) {
+  } else if (warp == 9) {
     // ------------------------------------------------------------------ value products
     if (tc::elect()) {
       uint32_t c = 0;
@@ -650,48 +503,222 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       tc::commit(&drain[1]);
       if (!mbar_wait(&drain[1], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
     }
-  } else {
-    // ------------------------------------------------------------------ tile copies
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ tile copies: K by warp 10, V by warp 11
     // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
     const uint64_t policy = l2_policy_evict_first();
-    int unit = 0;
+    const int half = warp - 10, depth = half ? C::VU : C::KU;
+    uint8_t* units = half ? vunits : kunits;
+    uint64_t* full = half ? vfull : kfull;
+    uint64_t* empty = half ? vempty : kempty;
+    // lanes 0 .. 15 take the codes of a tile each, lanes 16 .. 31 the scales
+    const int mine = lane & 15;
+    const uint32_t bytes = lane < 16 ? 8 * W : W / 2;
+    const uint32_t src_off = lane < 16 ? tl.v_codes(0, 0) * half : tl.k_scale(0, 0) + half * (W / 2);
+    const uint32_t dst_off = (lane < 16 ? 0 : C::SCALES) + mine * bytes;
+    int unit = 0, ring = 0;
+    uint32_t phase = 1;  // parity of a unit's last release
     while (st.next()) {
       for (int t0 = 0; t0 < st.n; t0 += UT, ++unit) {
-        const int ring = unit % C::UNITS, n = min(UT, st.n - t0);
-        const int t = st.tile + t0 + lane;
+        const int n = min(UT, st.n - t0);
+        const int t = st.tile + t0 + mine;
         const int lp = t / p.tpp;
         int blk = -1;
-        if (lane < n) {
+        if (mine < n) {
           if (lp < p.max_blocks) blk = p.bt[static_cast<int64_t>(st.r) * p.bt_st + lp];
           if (blk < 0 || blk >= p.num_blocks) {
             record_error(p.err, kErrBlock);
             blk = -1;
           }
         }
-        if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
+        wait(&empty[ring], phase, kErrWaitEmpty);
         __syncwarp();
-        uint8_t* dst = units + ring * C::UNIT + lane * C::TILE;
-        const unsigned absent = __ballot_sync(0xffffffffu, lane < n && blk < 0);
-        if (lane < n && blk < 0) {  // a page outside the table or the cache reads as zeros
-          for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
+        uint8_t* dst = units + ring * C::UNIT + dst_off;
+        const unsigned absent = __ballot_sync(0xffffffffu, mine < n && blk < 0);
+        if (mine < n && blk < 0) {  // a page outside the table or the cache reads as zeros
+          for (uint32_t o = 0; o < bytes; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent)) * C::TILE);
+        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent & 0xffffu)) * (C::TILE / 2));
         __syncwarp();
-        if (lane < n && blk >= 0)
-          tc::bulk_load(dst, p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE,
-                        C::TILE, &full[ring], policy);
+        if (mine < n && blk >= 0)
+          tc::bulk_load(dst, p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE + src_off,
+                        bytes, &full[ring], policy);
+        if (++ring == depth) {
+          ring = 0;
+          phase ^= 1;
+        }
       }
     }
     // after an abort no role may have waited for the last copies: they must land before the CTA ends
     if (wait.aborted() && lane == 0)
-      for (int u = max(0, unit - C::UNITS); u < unit; ++u) mbar_wait(&full[u % C::UNITS], (u / C::UNITS) & 1, p.wait_ns);
+      for (int u = max(0, unit - depth); u < unit; ++u) mbar_wait(&full[u % depth], (u / depth) & 1, p.wait_ns);
+  } else if (warp < 20) {
+    // ------------------------------------------------------------------ K rows
+    // Launched as a programmatic dependent of the launch that writes q, this grid has been copying tiles
+    // meanwhile; q is read only once that launch has completed.
+    griddep_wait();
+    const int ktid = tid - 12 * 32, grp = ktid >> 7, w = warp & 3;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int u0 = 2 * w / UT, row = lane & 15;              // the unit of the step with this warp's two tiles
+    const int tiu = 2 * w - u0 * UT + (lane >> 4);           // this lane's tile in that unit
+    const int code_off = tiu * 8 * W + row * 16, scale_off = C::SCALES + (tiu * 16 + row) * (W / kQ4Group);
+    int unit0 = 0;        // ring position of the step's first unit
+    uint32_t chunk = 0;   // chunks before this step
+    int seg = 0;
+    for (uint32_t i = 0; st.next(); ++i) {
+      if (st.first) {
+        if (i > 0) wait(&sf[(i - 1) & 1], ((i - 1) >> 1) & 1, kErrWaitFull);  // the scores before read Q no more
+        // the row's queries: 16 threads per head, W / 16 columns each
+        const int h = ktid >> 4, part = ktid & 15;
+        const __nv_bfloat16* src = p.q + static_cast<int64_t>(st.r) * p.q_st + static_cast<int64_t>(h) * p.q_sh + part * (W / 16);
+        uint4 v[W / 128];
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < W / 128; ++k) {
+          v[k] = h < p.H ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[j] << 16)), fabsf(__uint_as_float(x[j] & 0xffff0000u))));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        // a power of two that puts the head's largest element into [2^12, 2^13) (an infinity stays one)
+        int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
+        e = e > 110 ? 110 : (e < -110 ? -110 : e);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        if (part == 0) qscale[seg % kQSlots * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+        for (int k = 0; k < W / 128; ++k) {
+          const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          uint32_t u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __half2 hh = __floats2half2_rn(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
+            u[j] = *reinterpret_cast<const uint32_t*>(&hh);
+          }
+          const int col = part * (W / 16) + 8 * k;
+          *reinterpret_cast<uint4*>(qs + (col >> 6) * 2048 + tc::sw128(h, (col >> 3) & 7)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&qf[seg % kQSlots]);
+        ++seg;
+      } else if (i > 1) {
+        // keeps a warp that runs ahead within two steps, so that the wait above never meets an older phase
+        wait(&sf[i & 1], ((i - 2) >> 1) & 1, kErrWaitFull);
+      }
+      const int ring = (unit0 + u0) % C::KU;
+      const bool unit_there = u0 * UT < st.n;
+      const uint8_t* codes = kunits + ring * C::UNIT + code_off;
+      const uint8_t* scales = kunits + ring * C::UNIT + scale_off;
+      if (unit_there) wait(&kfull[ring], ((unit0 + u0) / C::KU) & 1, kErrWaitFull);
+#pragma unroll 1
+      for (int kc = grp; kc < W / 128; kc += 2) {
+        const uint32_t c = chunk + kc, buf = c % C::BUFS;
+        wait(&ake[buf], ((c / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+        __syncwarp();
+        tc::fence_after();
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(scales + 4 * kc);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          Q4ScaleH s[2];
+          q4_scales_h((sc >> (16 * hf)) & 0xffffu, s[0], s[1]);
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const uint4 x = *reinterpret_cast<const uint4*>(codes + kc * 1024 + (2 * hf + gi) * 256);
+            uint32_t v[16];
+            q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
+            q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
+            q4_word_h(x.z, s[gi], sixteen, v[8], v[9], v[10], v[11]);
+            q4_word_h(x.w, s[gi], sixteen, v[12], v[13], v[14], v[15]);
+            tc::st16(lane_base + C::AK + buf * 64 + (2 * hf + gi) * 16, v);
+          }
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&akf[buf]);
+      }
+      if (lane == 0 && unit_there) mbar_arrive(&kempty[ring]);
+      unit0 += (st.n + UT - 1) / UT;
+      chunk += W / 128;
+    }
+  } else {
+    // ------------------------------------------------------------------ V columns
+    const int w = warp & 3, g = lane >> 2, c = lane & 3;
+    const uint32_t grp = warp >= 24;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int col0 = (8 * w + g) * 4 * NB;  // this thread's 4 NB columns
+    int unit = 0;
+    uint32_t chunk = 0;
+    while (st.next()) {
+      for (int ut = 0; ut < st.n; ut += UT, ++unit) {
+        const int ring = unit % C::VU;
+        const uint8_t* ub = vunits + ring * C::UNIT;
+        wait(&vfull[ring], (unit / C::VU) & 1, kErrWaitFull);
+        const int tiles = min(UT, st.n - ut);
+#pragma unroll 1
+        for (int t0 = ((chunk + ut / C::VT) & 1) == grp ? 0 : C::VT; t0 < tiles; t0 += 2 * C::VT) {
+          // chunks alternate between the groups over all steps, so that a buffer always belongs to the same group:
+          // a group that met a buffer's barrier out of turn could take an older phase for the one it waits for
+          const uint32_t ch = chunk + (ut + t0) / C::VT, buf = ch % C::BUFS;
+          wait(&ave[buf], ((ch / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+          __syncwarp();
+          tc::fence_after();
+#pragma unroll 1
+          for (int ti = 0; ti < C::VT && t0 + ti < tiles; ++ti) {
+            const uint8_t* codes = ub + (t0 + ti) * 8 * W + col0 * 8 + 16 * c;
+            uint32_t sb = *reinterpret_cast<const uint32_t*>(ub + C::SCALES + (t0 + ti) * (W / 2) + (col0 >> 5) * 16 + 4 * c);
+            // rows past the context get a zero scale, whatever their bytes are
+            if (st.last) {
+              const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
+              if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
+            }
+            const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
+            const uint32_t at = lane_base + C::AV + buf * C::VCOLS + ti * 8;
+            constexpr int OH = NB >= 4 ? NB / 4 : 1;  // octets per half of the lanes (width 256: one for both)
+#pragma unroll
+            for (int o0 = 0; o0 < NB / 2; o0 += OH) {
+              uint32_t v[8 * OH][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
+#pragma unroll
+              for (int oc = 0; oc < OH; ++oc) {
+                const uint4 x = *reinterpret_cast<const uint4*>(codes + (o0 + oc) * 64);
+                uint32_t (*d)[2] = v + 8 * oc;
+                q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
+                q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, sixteen, d[0][1], d[2][1], d[4][1], d[6][1]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, sixteen, d[1][1], d[3][1], d[5][1], d[7][1]);
+              }
+              // block b: columns q NB + b of q = 2 hf (lanes 0..7 of half hf) and 2 hf + 1 (lanes 8..15)
+              constexpr int HALVES = NB >= 4 ? 1 : 2;
+#pragma unroll
+              for (int hl = 0; hl < HALVES; ++hl) {
+                const int hf = NB >= 4 ? o0 / OH : hl;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                  tc::st_16x256(at + (static_cast<uint32_t>(hf * 16) << 16) + b * (C::VT * 8), v[2 * hl * NB + b][0],
+                                v[2 * hl * NB + b][1], v[(2 * hl + 1) * NB + b][0], v[(2 * hl + 1) * NB + b][1]);
+              }
+            }
+          }
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&avf[buf]);
+        }
+        if (lane == 0) mbar_arrive(&vempty[ring]);
+      }
+      chunk += (st.n + C::VT - 1) / C::VT;
+    }
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 24) tc::dealloc(tmem, 512);
+  if (warp == 8) tc::dealloc(tmem, 512);
 }
 
 template <int W>
