@@ -16,17 +16,18 @@
 // are therefore the M = 128 lanes and the heads are N = 16:
 //   S^T [128 keys x 16 heads]    = K [128 x W] (tensor memory) . Q^T (shared memory, f16)
 //   O^T [128 columns x 16 heads] += V^T [128 x 16 rows] (tensor memory) . P^T (shared memory, f16), W / 128 of them
-// A CTA takes 128 rows ("step") at a time; two CTAs share an SM and fill each other's gaps:
-//   warps 0-3  dequantise the step's K rows into tensor memory (thread = row) in chunks of 128 columns, then the
-//              first two chunks of V (thread 4 g + c: 4 rows x W / 32 columns as 16x256b fragments, lane = column),
-//              which hides the score products' latency; then the softmax (thread = key) and the other V chunks.
-//              The exponent base of a head only moves when a score passes it by 2^4 (a vote), so the output is
-//              rescaled rarely and the common step needs no reduction at all.
-//   warp 4     one thread issues every product.
-//   warp 5     bulk copies of the K and V halves of tiles into a ring of units of 17408 bytes (the halves of 2, 4
-//              or 8 tiles), in the order in which they are used.
-// Roles of their own for K, V and the softmax (28 warps, one CTA per SM) took 102 us instead: each step then
-// crosses more barriers than it has work between them, and the roles' code competes for the instruction caches.
+// One CTA per SM takes 128 rows ("step") at a time:
+//   warps 0-7   K: a thread dequantises one row into its lane, 128 columns (a chunk) at a time; the two groups of
+//               four warps take turns.
+//   warps 8-15  V: thread 4 g + c takes 4 rows x W / 32 columns of a tile as a 16x256b fragment (lane = column);
+//               two groups as well.
+//   warps 16-23 softmax: a thread has the scores of its key for the 8 heads of its group.  The exponent base of a
+//               head only moves when a score passes it by 2^4 (a vote), so the output is rescaled rarely and the
+//               common step needs no reduction at all.  They also write the segment's output.
+//   warp 24, 25 one thread each issues the score and the value products.
+//   warp 26     bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
+// The dequantising loops are kept rolled: unrolled over a step they outgrew the instruction caches, and the warps
+// of a scheduler run different code (190 us unrolled with one group of each, 137 us rolled with a softmax group).
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
 // of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
 // 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
@@ -65,32 +66,32 @@ struct Q4Cfg {
   static constexpr int NB = W / 128;             // blocks of 128 latent columns (output accumulators)
   static constexpr int TILE = 17 * W;            // bytes of 16 rows
   static constexpr int UT = 2048 / W;            // tiles per ring unit
-  static constexpr int SCALES = 16384;           // a unit: the codes of its tiles (8 W bytes each), then their scales
-  static constexpr int UNIT = SCALES + 1024;
-  static constexpr int CTAS = W == 1024 ? 1 : 2; // per SM: 1024 columns of output need half the tensor memory
-  static constexpr int UNITS = W == 1024 ? 9 : 5;
-  static constexpr int VT = UT / 2;              // tiles per V chunk: 64 columns of tensor memory, as a K chunk
+  static constexpr int UNIT = UT * TILE;         // 34816
+  static constexpr int UNITS = 5;
+  static constexpr int VT = W == 256 ? 2 : 1;    // tiles per V chunk
+  static constexpr int VCOLS = NB * VT * 8;      // its tensor-memory columns
+  static constexpr int BUFS = W == 1024 ? 2 : 4; // K chunks and V chunks in tensor memory
   static constexpr int Q_BYTES = 32 * W;
-  static constexpr int P_BYTES = 4096;
-  // tensor-memory columns: two chunk buffers (K: 128 rows x 128 columns; V), the scores, the output
-  static constexpr uint32_t A = 0, S = 128, O = 144;
-  static constexpr uint32_t COLS = W == 1024 ? 512 : 256;
-  static_assert(O + NB * 16 <= COLS, "tensor memory");
-  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 768;  // + 4 (T + 1) in stream mode
+  static constexpr int P_BYTES = 2 * 4096;  // two steps
+  // tensor-memory columns: K chunks (128 rows x 128 latent columns), V chunks, two score tiles, output
+  static constexpr uint32_t AK = 0, AV = AK + BUFS * 64, S = AV + BUFS * VCOLS, O = S + 32;
+  static_assert(O + NB * 16 <= 512, "tensor memory");
+  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
 };
-constexpr int kQ4HistThreads = 6 * 32;
+constexpr int kQSlots = 4;  // score factors of this many segments: the K warps run at most 3 segments ahead
+constexpr int kQ4HistThreads = 27 * 32;
 // log2 of how far a score may pass its head's exponent base before the base moves, and of the factor the
 // probabilities carry: together they end at 2^15, f16's largest power of two.  A small first term lets small
 // probabilities keep f16's precision, a large one makes rescales rare (each costs about one step).
 constexpr float kQ4Over = 4.f, kQ4Lift = 11.f;
 
-// Sum or maximum of each of 16 values over a warp: halving exchanges, after which lane l holds value rev16(l % 16)
+// Sum or maximum of each of 8 values over a warp: halving exchanges, after which lane l holds value rev8(l % 8)
 // of all 32 lanes.
 template <bool MAX>
-__device__ __forceinline__ float reduce16(float (&v)[16], int lane) {
+__device__ __forceinline__ float reduce8(float (&v)[8], int lane) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int half = 8 >> k;
+  for (int k = 0; k < 3; ++k) {
+    const int half = 4 >> k;
     const bool up = (lane >> k) & 1;
 #pragma unroll
     for (int j = 0; j < half; ++j) {
@@ -99,10 +100,14 @@ __device__ __forceinline__ float reduce16(float (&v)[16], int lane) {
       v[j] = MAX ? fmaxf(keep, got) : keep + got;
     }
   }
-  const float got = __shfl_xor_sync(0xffffffffu, v[0], 16);
-  return MAX ? fmaxf(v[0], got) : v[0] + got;
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
+    v[0] = MAX ? fmaxf(v[0], got) : v[0] + got;
+  }
+  return v[0];
 }
-__device__ __forceinline__ int rev16(int l) { return ((l & 1) << 3) | ((l & 2) << 1) | ((l & 4) >> 1) | ((l & 8) >> 3); }
+__device__ __forceinline__ int rev8(int l) { return ((l & 1) << 2) | (l & 2) | ((l & 4) >> 2); }
 
 // 2^x to 2^-22 relative (0 for -inf and below 2^-126, where it only feeds sums of terms up to 2^15).
 __device__ __forceinline__ float ex2(float x) {
@@ -167,7 +172,7 @@ struct Q4Walk {
 };
 
 template <int W>
-__global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_kernel(const Q4HistoryParams p) {
+__global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4HistoryParams p) {
   using C = Q4Cfg<W>;
   constexpr int NB = C::NB, UT = C::UT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -178,17 +183,21 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
   uint8_t* ctl = units + C::UNITS * C::UNIT;
   uint64_t* full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
   uint64_t* empty = full + C::UNITS;                  // [UNITS] unit read
-  uint64_t* af = empty + C::UNITS;                    // [2] chunk in tensor memory
-  uint64_t* ae = af + 2;                              // [2] its products are done
-  uint64_t* sf = ae + 2;                              // scores of a step
-  uint64_t* pf = sf + 1;                              // probabilities of a step written
-  uint64_t* pv = pf + 1;                              // value products of a step done
-  uint64_t* drain = pv + 1;                           // every product is done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* akf = empty + C::UNITS;                   // [BUFS] K chunk in tensor memory
+  uint64_t* ake = akf + C::BUFS;                      // [BUFS] its MMAs are done
+  uint64_t* avf = ake + C::BUFS;                      // [BUFS] V chunk
+  uint64_t* ave = avf + C::BUFS;
+  uint64_t* sf = ave + C::BUFS;                       // [2] scores of a step
+  uint64_t* se = sf + 2;                              // [2] read
+  uint64_t* qf = se + 2;                              // [kQSlots] score factors of a segment
+  uint64_t* pf = qf + kQSlots;                        // [2] probabilities of a step written
+  uint64_t* pv = pf + 2;                              // [2] value products of a step done
+  uint64_t* drain = pv + 2;                           // [2] every MMA of an issuer is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  float* qscale = reinterpret_cast<float*>(ctl + 256);  // [16] score factor of a head
-  float* red = qscale + 16;                             // [4][16] per-warp maxima / sums
-  int* pref = reinterpret_cast<int*>(ctl + 768);        // [T + 1] (stream mode)
+  float* qscale = reinterpret_cast<float*>(ctl + 384);  // [kQSlots][16] score factor of a head, by segment
+  float* red = qscale + kQSlots * 16;                   // [2][4][8] per-warp maxima / sums
+  int* pref = reinterpret_cast<int*>(ctl + 1024);       // [T + 1] (stream mode)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int r0 = 0, p0 = 0, p1 = 0;
@@ -233,20 +242,26 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
     p0 = blockIdx.x;  // rows blockIdx.x, + gridDim.x, ...
   }
 
-  if (warp == 4) tc::alloc(tmem_slot, C::COLS);
-  if (tid == 5 * 32) {
-    for (int u = 0; u < C::UNITS; ++u) {
-      mbar_init(&full[u], 1);
-      mbar_init(&empty[u], 4);
+  if (warp == 24) tc::alloc(tmem_slot, 512);
+  if (tid == 25 * 32) {
+    for (int s = 0; s < C::UNITS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 8 + UT);  // the V warps, and the K warps of its tiles (one for two tiles in each group)
+    }
+    for (int b = 0; b < C::BUFS; ++b) {
+      mbar_init(&akf[b], 4);
+      mbar_init(&ake[b], 1);
+      mbar_init(&avf[b], 4);
+      mbar_init(&ave[b], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&af[b], 4);
-      mbar_init(&ae[b], 1);
+      mbar_init(&sf[b], 1);
+      mbar_init(&se[b], 8);
+      mbar_init(&pf[b], 8);
+      mbar_init(&pv[b], 1);
+      mbar_init(&drain[b], 1);
     }
-    mbar_init(sf, 1);
-    mbar_init(pf, 4);
-    mbar_init(pv, 1);
-    mbar_init(drain, 1);
+    for (int b = 0; b < kQSlots; ++b) mbar_init(&qf[b], 8);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -256,79 +271,48 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
   const tc::Waits wait{abort_flag, p.err, p.wait_ns};
+  const Q4Tile tl(W);
   const uint32_t sixteen = p.sixteen;
   Q4Walk st(p, pref, r0, p0, p1);
 
-  if (warp < 4) {
+  if (warp < 8) {
+    // ------------------------------------------------------------------ K rows
     // Launched as a programmatic dependent of the launch that writes q, this grid has been copying tiles
-    // meanwhile; q and the workspace (which what runs before that launch may still read) are touched only once
-    // that launch has completed.
+    // meanwhile; q is read only once that launch has completed.
     griddep_wait();
-    if (tid == 0) griddep_launch_dependents();
-    if (p.stream_mode && blockIdx.x == 0) {
-      for (int t = tid; t < p.T; t += 128) {
-        const int a = pref[t], b = pref[t + 1];
-        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
-                                      static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
-                          : make_int2(0, 0);
-      }
-    }
-    if (!p.stream_mode && warp == 0) {  // rows without history: their slot says so
-      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
-        if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
-    }
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const int key = tid;
-    // K: the unit of the step with this warp's two tiles, and this lane's row in it
-    const int u0 = 2 * warp / UT, tiu = 2 * warp - u0 * UT + (lane >> 4), row = lane & 15;
-    const int kcode = tiu * 8 * W + row * 16, kscale = C::SCALES + (tiu * 16 + row) * (W / kQ4Group);
-    // V: this thread's 4 NB columns
-    const int c4 = lane & 3, col0 = (8 * warp + (lane >> 2)) * 4 * NB;
-    const int vcode = col0 * 8 + 16 * c4, vscale = C::SCALES + (col0 >> 5) * 16 + 4 * c4;
-    uint8_t* pk = ps + (key >> 6) * 2048 + (key & 7) * 2;  // + swizzled chunk of a head
-    int slot0 = 0;              // ring slot of the step's first unit
-    uint32_t ring_phase = 0;    // and its parity
-    uint32_t chunk = 0;         // chunks so far: buffer chunk & 1
-    float mm[16], l[16];        // the base of a head minus kQ4Lift; this key's share of the sums
-
-    auto chunk_begin = [&]() {
-      wait(&ae[chunk & 1], ((chunk >> 1) & 1) ^ 1, kErrWaitEmpty);
-      __syncwarp();
-      tc::fence_after();
-    };
-    auto chunk_end = [&]() {
-      tc::wait_st();
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&af[chunk & 1]);
-      ++chunk;
-    };
-
+    const int grp = warp >> 2, w = warp & 3;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int u0 = 2 * w / UT, row = lane & 15;              // the unit of the step with this warp's two tiles
+    const int tile_off = (2 * w - u0 * UT + (lane >> 4)) * C::TILE;
+    int unit0 = 0;        // ring position of the step's first unit
+    uint32_t chunk = 0;   // chunks before this step
+    int seg = 0;
     for (uint32_t i = 0; st.next(); ++i) {
-      const int nu = (st.n + UT - 1) / UT;
       if (st.first) {
-        // the row's queries: 8 threads per head, W / 8 columns each (every product with the last row's is done)
-        const int h = tid >> 3, part = tid & 7;
-        const __nv_bfloat16* src = p.q + static_cast<int64_t>(st.r) * p.q_st + static_cast<int64_t>(h) * p.q_sh + part * (W / 8);
-        uint4 v[W / 64];
+        if (i > 0) wait(&sf[(i - 1) & 1], ((i - 1) >> 1) & 1, kErrWaitFull);  // the scores before read Q no more
+        // the row's queries: 16 threads per head, W / 16 columns each
+        const int h = tid >> 4, part = tid & 15;
+        const __nv_bfloat16* src = p.q + static_cast<int64_t>(st.r) * p.q_st + static_cast<int64_t>(h) * p.q_sh + part * (W / 16);
+        uint4 v[W / 128];
         float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < W / 64; ++k) {
+        for (int k = 0; k < W / 128; ++k) {
           v[k] = h < p.H ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0u, 0u, 0u, 0u);
           const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[j] << 16)), fabsf(__uint_as_float(x[j] & 0xffff0000u))));
         }
+        __syncwarp();
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         // a power of two that puts the head's largest element into [2^12, 2^13) (an infinity stays one)
         int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127 - 12;
         e = e > 110 ? 110 : (e < -110 ? -110 : e);
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        if (part == 0) qscale[h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if (part == 0) qscale[seg % kQSlots * 16 + h] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-        for (int k = 0; k < W / 64; ++k) {
+        for (int k = 0; k < W / 128; ++k) {
           const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
           uint32_t u[4];
 #pragma unroll
@@ -336,229 +320,262 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
             const __half2 hh = __floats2half2_rn(__uint_as_float(x[j] << 16) * down, __uint_as_float(x[j] & 0xffff0000u) * down);
             u[j] = *reinterpret_cast<const uint32_t*>(&hh);
           }
-          const int col = part * (W / 8) + 8 * k;
+          const int col = part * (W / 16) + 8 * k;
           *reinterpret_cast<uint4*>(qs + (col >> 6) * 2048 + tc::sw128(h, (col >> 3) & 7)) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        fence_proxy_async();     // ordered before the products by the chunk barriers below
-        named_bar_sync(1, 128);  // qscale
-      }
-
-      // ---- K: thread = row
-      {
-        int slot = slot0 + u0;
-        const bool wrap = slot >= C::UNITS;
-        if (wrap) slot -= C::UNITS;
-        const uint8_t* ub = units + slot * C::UNIT;
-        if (u0 < nu) wait(&full[slot], ring_phase ^ (wrap ? 1u : 0u), kErrWaitFull);
-#pragma unroll 1
-        for (int kc = 0; kc < W / 128; ++kc) {
-          const uint32_t sc = *reinterpret_cast<const uint32_t*>(ub + kscale + 4 * kc);
-          chunk_begin();
-          const uint32_t at = lane_base + C::A + (chunk & 1) * 64;
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            Q4ScaleH s[2];
-            q4_scales_h((sc >> (16 * hf)) & 0xffffu, s[0], s[1]);
-#pragma unroll
-            for (int gi = 0; gi < 2; ++gi) {
-              const uint4 x = *reinterpret_cast<const uint4*>(ub + kcode + kc * 1024 + (2 * hf + gi) * 256);
-              uint32_t v[16];
-              q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
-              q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
-              q4_word_h(x.z, s[gi], sixteen, v[8], v[9], v[10], v[11]);
-              q4_word_h(x.w, s[gi], sixteen, v[12], v[13], v[14], v[15]);
-              tc::st16(at + (2 * hf + gi) * 16, v);
-            }
-          }
-          chunk_end();
-        }
-        // the step's K units are free: every warp releases each of them
-        if (lane == 0)
-          for (int u = 0; u < nu; ++u) mbar_arrive(&empty[slot0 + u < C::UNITS ? slot0 + u : slot0 + u - C::UNITS]);
-        slot0 += nu;
-        if (slot0 >= C::UNITS) {
-          slot0 -= C::UNITS;
-          ring_phase ^= 1u;
-        }
-      }
-
-      // ---- V: thread = 4 rows x 4 NB columns of a tile
-      auto dequant_v = [&](int t0) {
-        if (t0 % UT == 0) wait(&full[slot0], ring_phase, kErrWaitFull);
-        chunk_begin();
-        const uint8_t* ub = units + slot0 * C::UNIT;
-#pragma unroll 1
-        for (int ti = 0; ti < C::VT && t0 + ti < st.n; ++ti) {
-          const int tu = (t0 + ti) % UT;
-          uint32_t sb = *reinterpret_cast<const uint32_t*>(ub + vscale + tu * (W / 2));
-          // rows past the context get a zero scale, whatever their bytes are
-          if (st.last) {
-            const int valid = st.ctx - ((st.tile + t0 + ti) << 4) - 4 * c4;
-            if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
-          }
-          const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
-          const uint32_t at = lane_base + C::A + (chunk & 1) * 64 + ti * 8;
-          constexpr int OH = NB >= 4 ? NB / 4 : 1;  // octets per half of the lanes (width 256: one for both)
-#pragma unroll
-          for (int o0 = 0; o0 < NB / 2; o0 += OH) {
-            uint32_t v[8 * OH][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
-#pragma unroll
-            for (int oc = 0; oc < OH; ++oc) {
-              const uint4 x = *reinterpret_cast<const uint4*>(ub + vcode + tu * 8 * W + (o0 + oc) * 64);
-              uint32_t (*d)[2] = v + 8 * oc;
-              q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
-              q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
-              q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, sixteen, d[0][1], d[2][1], d[4][1], d[6][1]);
-              q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, sixteen, d[1][1], d[3][1], d[5][1], d[7][1]);
-            }
-            // block b: columns q NB + b of q = 2 hf (lanes 0..7 of half hf) and 2 hf + 1 (lanes 8..15)
-            constexpr int HALVES = NB >= 4 ? 1 : 2;
-#pragma unroll
-            for (int hl = 0; hl < HALVES; ++hl) {
-              const int hf = NB >= 4 ? o0 / OH : hl;
-#pragma unroll
-              for (int b = 0; b < NB; ++b)
-                tc::st_16x256(at + (static_cast<uint32_t>(hf * 16) << 16) + b * (C::VT * 8), v[2 * hl * NB + b][0],
-                              v[2 * hl * NB + b][1], v[(2 * hl + 1) * NB + b][0], v[(2 * hl + 1) * NB + b][1]);
-            }
-          }
-        }
-        chunk_end();
-        if ((t0 + C::VT) % UT == 0 || t0 + C::VT >= st.n) {  // the unit's last chunk
-          if (lane == 0) mbar_arrive(&empty[slot0]);
-          if (++slot0 == C::UNITS) {
-            slot0 = 0;
-            ring_phase ^= 1u;
-          }
-        }
-      };
-
-      // ---- softmax: thread = key
-      auto softmax = [&]() {
-        wait(sf, i & 1, kErrWaitFull);
-        __syncwarp();
-        tc::fence_after();
-        uint32_t raw[16];
-        tc::ld16(lane_base + C::S, raw);
-        float f[16];
-#pragma unroll
-        for (int h = 0; h < 16; h += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(qscale + h);
-          f[h] = x.x, f[h + 1] = x.y, f[h + 2] = x.z, f[h + 3] = x.w;
-        }
-        tc::wait_ld();
-        tc::fence_before();
-        // a step that is not full: dead keys score -inf
-        const bool dead = st.last && ((st.tile << 4) + key >= st.ctx || key >= (st.n << 4));
-        float x[16], over = -INFINITY;
-        if (!st.first) {
-#pragma unroll
-          for (int h = 0; h < 16; ++h) x[h] = fmaf(__uint_as_float(raw[h]), f[h], -mm[h]);
-          if (dead) {
-#pragma unroll
-            for (int h = 0; h < 16; ++h) x[h] = -INFINITY;
-          }
-#pragma unroll
-          for (int h = 0; h < 16; ++h) over = fmaxf(over, x[h]);
-        }
-        if (named_bar_or(1, 128, st.first || over > kQ4Lift + kQ4Over)) {
-          // new bases: the maximum over the step's keys, per head
-#pragma unroll
-          for (int h = 0; h < 16; ++h) x[h] = dead ? -INFINITY : __uint_as_float(raw[h]) * f[h];
-          float mx[16];
-#pragma unroll
-          for (int h = 0; h < 16; ++h) mx[h] = x[h];
-          const float top = reduce16<true>(mx, lane);
-          if (lane < 16) red[warp * 16 + rev16(lane)] = top;
-          named_bar_sync(1, 128);
-          float al[16];
-#pragma unroll
-          for (int h = 0; h < 16; ++h) {
-            float mn = fmaxf(fmaxf(red[h], red[16 + h]), fmaxf(red[32 + h], red[48 + h]));
-            if (!st.first) mn = fmaxf(mn, mm[h] + kQ4Lift);
-            mn = mn == -INFINITY ? -kQ4Lift : mn - kQ4Lift;  // every score -inf: any finite base
-            al[h] = st.first || mn == mm[h] ? 1.f : ex2(mm[h] - mn);
-            mm[h] = mn;
-            l[h] = st.first ? 0.f : l[h] * al[h];
-            x[h] -= mn;
-          }
-          if (!st.first) {
-            // the products of the step before are done: their chunks' buffers have been refilled since, or soon are
-            wait(pv, (i - 1) & 1, kErrWaitFull);
-            __syncwarp();
-            tc::fence_after();
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              uint32_t o[16];
-              tc::ld16(lane_base + C::O + b * 16, o);
-              tc::wait_ld();
-#pragma unroll
-              for (int h = 0; h < 16; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * al[h]);
-              tc::st16(lane_base + C::O + b * 16, o);
-            }
-            tc::wait_st();
-            tc::fence_before();
-          }
-          named_bar_sync(1, 128);  // red is read before it is written again
-        }
-        if (i > 0) wait(pv, (i - 1) & 1, kErrWaitFull);  // these probabilities replace the last step's
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < 16; ++h) {
-          const float e = ex2(x[h]);
-          l[h] += e;
-          *reinterpret_cast<__half*>(pk + (h >> 3) * 1024 + (h & 7) * 128 + ((((key >> 3) & 7) ^ (h & 7)) << 4)) =
-              __float2half_rn(e);
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pf);
-      };
-
-#pragma unroll 1
-      for (int t0 = 0, ck = 0; t0 < st.n; t0 += C::VT, ++ck) {
-        dequant_v(t0);
-        // two chunks fit the buffers before the first needs probabilities
-        if (ck == 1 || (ck == 0 && t0 + C::VT >= st.n)) softmax();
+        if (lane == 0) mbar_arrive(&qf[seg % kQSlots]);
+        ++seg;
+      } else if (i > 1) {
+        // keeps a warp that runs ahead within two steps, so that the wait above never meets an older phase
+        wait(&sf[i & 1], ((i - 2) >> 1) & 1, kErrWaitFull);
       }
+      const int ring = (unit0 + u0) % C::UNITS;
+      const bool unit_there = u0 * UT < st.n;
+      const uint8_t* tb = units + ring * C::UNIT + tile_off;
+      if (unit_there) wait(&full[ring], ((unit0 + u0) / C::UNITS) & 1, kErrWaitFull);
+#pragma unroll 1
+      for (int kc = grp; kc < W / 128; kc += 2) {
+        const uint32_t c = chunk + kc, buf = c % C::BUFS;
+        wait(&ake[buf], ((c / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+        __syncwarp();
+        tc::fence_after();
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * kc));
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          Q4ScaleH s[2];
+          q4_scales_h((sc >> (16 * hf)) & 0xffffu, s[0], s[1]);
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
+            uint32_t v[16];
+            q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
+            q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
+            q4_word_h(x.z, s[gi], sixteen, v[8], v[9], v[10], v[11]);
+            q4_word_h(x.w, s[gi], sixteen, v[12], v[13], v[14], v[15]);
+            tc::st16(lane_base + C::AK + buf * 64 + (2 * hf + gi) * 16, v);
+          }
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&akf[buf]);
+      }
+      if (lane == 0 && unit_there) mbar_arrive(&empty[ring]);
+      unit0 += (st.n + UT - 1) / UT;
+      chunk += W / 128;
+    }
+  } else if (warp < 16) {
+    // ------------------------------------------------------------------ V columns
+    const int w = warp & 3, g = lane >> 2, c = lane & 3;
+    const uint32_t grp = (warp >> 2) & 1;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int col0 = (8 * w + g) * 4 * NB;  // this thread's 4 NB columns
+    int unit = 0;
+    uint32_t chunk = 0;
+    while (st.next()) {
+      for (int ut = 0; ut < st.n; ut += UT, ++unit) {
+        const int ring = unit % C::UNITS;
+        const uint8_t* ub = units + ring * C::UNIT;
+        wait(&full[ring], (unit / C::UNITS) & 1, kErrWaitFull);
+        const int tiles = min(UT, st.n - ut);
+#pragma unroll 1
+        for (int t0 = ((chunk + ut / C::VT) & 1) == grp ? 0 : C::VT; t0 < tiles; t0 += 2 * C::VT) {
+          // chunks alternate between the groups over all steps, so that a buffer always belongs to the same group:
+          // a group that met a buffer's barrier out of turn could take an older phase for the one it waits for
+          const uint32_t ch = chunk + (ut + t0) / C::VT, buf = ch % C::BUFS;
+          wait(&ave[buf], ((ch / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+          __syncwarp();
+          tc::fence_after();
+#pragma unroll 1
+          for (int ti = 0; ti < C::VT && t0 + ti < tiles; ++ti) {
+            const uint8_t* tb = ub + (t0 + ti) * C::TILE;
+            uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + tl.v_scale(col0 >> 5, 4 * c));
+            // rows past the context get a zero scale, whatever their bytes are
+            if (st.last) {
+              const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
+              if (valid < 4) sb = valid <= 0 ? 0u : sb & ((1u << (8 * valid)) - 1u);
+            }
+            const Q4ScaleH s01 = q4_scale_h(e4m3x2_to_h2(sb & 0xffffu)), s23 = q4_scale_h(e4m3x2_to_h2(sb >> 16));
+            const uint32_t at = lane_base + C::AV + buf * C::VCOLS + ti * 8;
+            constexpr int OH = NB >= 4 ? NB / 4 : 1;  // octets per half of the lanes (width 256: one for both)
+#pragma unroll
+            for (int o0 = 0; o0 < NB / 2; o0 += OH) {
+              uint32_t v[8 * OH][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
+#pragma unroll
+              for (int oc = 0; oc < OH; ++oc) {
+                const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.v_codes((col0 >> 3) + o0 + oc, 4 * c));
+                uint32_t (*d)[2] = v + 8 * oc;
+                q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
+                q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x5410), s23, sixteen, d[0][1], d[2][1], d[4][1], d[6][1]);
+                q4_word_h(__byte_perm(x.z, x.w, 0x7632), s23, sixteen, d[1][1], d[3][1], d[5][1], d[7][1]);
+              }
+              // block b: columns q NB + b of q = 2 hf (lanes 0..7 of half hf) and 2 hf + 1 (lanes 8..15)
+              constexpr int HALVES = NB >= 4 ? 1 : 2;
+#pragma unroll
+              for (int hl = 0; hl < HALVES; ++hl) {
+                const int hf = NB >= 4 ? o0 / OH : hl;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                  tc::st_16x256(at + (static_cast<uint32_t>(hf * 16) << 16) + b * (C::VT * 8), v[2 * hl * NB + b][0],
+                                v[2 * hl * NB + b][1], v[(2 * hl + 1) * NB + b][0], v[(2 * hl + 1) * NB + b][1]);
+              }
+            }
+          }
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&avf[buf]);
+        }
+        if (lane == 0) mbar_arrive(&empty[ring]);
+      }
+      chunk += (st.n + C::VT - 1) / C::VT;
+    }
+  } else if (warp < 24) {
+    // ------------------------------------------------------------------ softmax, output: heads 8 grp .. + 7
+    // the workspace may still be read by what runs before the launch this grid waits for
+    griddep_wait();
+    const int grp = (warp >> 2) & 1, w = warp & 3, h0 = 8 * grp;
+    if (warp == 16 && lane == 0) griddep_launch_dependents();
+    if (p.stream_mode && blockIdx.x == 0) {
+      for (int t = tid - 512; t < p.T; t += 256) {
+        const int a = pref[t], b = pref[t + 1];
+        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
+                                      static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
+                          : make_int2(0, 0);
+      }
+    }
+    if (!p.stream_mode && warp == 16) {  // rows without history: their slot says so
+      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
+        if (p.ctx[r] <= 0 && lane < p.H && r < p.slots_cap) p.ws_lse[static_cast<int64_t>(r) * p.H + lane] = -INFINITY;
+    }
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int key = 32 * w + lane, bar = 1 + grp;
+    uint8_t* pk = ps + (key >> 6) * 2048 + grp * 1024 + (key & 7) * 2;  // + swizzled chunk of head h0 + h
+    float* myred = red + grp * 32;
+    int seg = 0;
+    float mm[8], l[8];  // the base of a head minus kQ4Lift; this key's share of the sums
+    for (uint32_t i = 0; st.next(); ++i) {
+      if (st.first) {
+        wait(&qf[seg % kQSlots], (seg / kQSlots) & 1, kErrWaitFull);
+        ++seg;
+      }
+      const float4* fs = reinterpret_cast<const float4*>(qscale + (seg - 1) % kQSlots * 16 + h0);
+      const int sb = i & 1;
+      wait(&sf[sb], (i >> 1) & 1, kErrWaitFull);
+      __syncwarp();
+      tc::fence_after();
+      uint32_t raw[8];
+      tc::ld8(lane_base + C::S + sb * 16 + h0, raw);
+      const float4 f0 = fs[0], f1 = fs[1];
+      const float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+      tc::wait_ld();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&se[sb]);
+      // a step that is not full: dead keys score -inf
+      const bool dead = st.last && ((st.tile << 4) + key >= st.ctx || key >= (st.n << 4));
+      float x[8], over = -INFINITY;
+      if (!st.first) {
+#pragma unroll
+        for (int h = 0; h < 8; ++h) x[h] = fmaf(__uint_as_float(raw[h]), f[h], -mm[h]);
+        if (dead) {
+#pragma unroll
+          for (int h = 0; h < 8; ++h) x[h] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 8; ++h) over = fmaxf(over, x[h]);
+      }
+      if (i > 1) wait(&pv[sb], ((i - 2) >> 1) & 1, kErrWaitFull);  // these probabilities replace those of step i - 2
+      __syncwarp();
+      if (named_bar_or(bar, 128, st.first || over > kQ4Lift + kQ4Over)) {
+        // new bases: the maximum over the step's keys, per head
+#pragma unroll
+        for (int h = 0; h < 8; ++h) x[h] = dead ? -INFINITY : __uint_as_float(raw[h]) * f[h];
+        float mx[8];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) mx[h] = x[h];
+        const float top = reduce8<true>(mx, lane);
+        if (lane < 8) myred[w * 8 + rev8(lane)] = top;
+        named_bar_sync(bar, 128);
+        float al[8];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) {
+          float mn = fmaxf(fmaxf(myred[h], myred[8 + h]), fmaxf(myred[16 + h], myred[24 + h]));
+          if (!st.first) mn = fmaxf(mn, mm[h] + kQ4Lift);
+          mn = mn == -INFINITY ? -kQ4Lift : mn - kQ4Lift;  // every score -inf: any finite base
+          al[h] = st.first || mn == mm[h] ? 1.f : ex2(mm[h] - mn);
+          mm[h] = mn;
+          l[h] = st.first ? 0.f : l[h] * al[h];
+          x[h] -= mn;
+        }
+        if (!st.first) {
+          wait(&pv[sb ^ 1], ((i - 1) >> 1) & 1, kErrWaitFull);  // no product touches the output meanwhile
+          __syncwarp();
+          tc::fence_after();
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint32_t o[8];
+            tc::ld8(lane_base + C::O + b * 16 + h0, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int h = 0; h < 8; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * al[h]);
+            tc::st8(lane_base + C::O + b * 16 + h0, o);
+          }
+          tc::wait_st();
+          tc::fence_before();
+        }
+        named_bar_sync(bar, 128);  // myred is read before it is written again
+      }
+#pragma unroll
+      for (int h = 0; h < 8; ++h) {
+        const float e = ex2(x[h]);
+        l[h] += e;
+        *reinterpret_cast<__half*>(pk + sb * 4096 + h * 128 + ((((key >> 3) & 7) ^ h) << 4)) = __float2half_rn(e);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pf[sb]);
       if (!st.last) continue;
 
       // ---- segment end: the normalised partial and its lse
-      float t[16];
+      float t[8];
 #pragma unroll
-      for (int h = 0; h < 16; ++h) t[h] = l[h];
-      const float sum = reduce16<false>(t, lane);
-      if (lane < 16) red[warp * 16 + rev16(lane)] = sum;
-      named_bar_sync(1, 128);
+      for (int h = 0; h < 8; ++h) t[h] = l[h];
+      const float sum = reduce8<false>(t, lane);
+      if (lane < 8) myred[w * 8 + rev8(lane)] = sum;
+      named_bar_sync(bar, 128);
 #pragma unroll
-      for (int h = 0; h < 16; ++h) t[h] = red[h] + red[16 + h] + red[32 + h] + red[48 + h];
+      for (int h = 0; h < 8; ++h) t[h] = myred[h] + myred[8 + h] + myred[16 + h] + myred[24 + h];
       const bool room = st.slot < p.slots_cap;
       if (!room && lane == 0) record_error(p.err, kErrSlots);
-      if (room && warp == 0) {
+      if (room && w == 0) {
 #pragma unroll
-        for (int h = 0; h < 16; ++h)
-          if (lane == h && h < p.H)
-            p.ws_lse[static_cast<int64_t>(st.slot) * p.H + h] = (mm[h] + log2f(t[h])) * 0.6931471805599453f;
+        for (int h = 0; h < 8; ++h)
+          if (lane == h && h0 + h < p.H)
+            p.ws_lse[static_cast<int64_t>(st.slot) * p.H + h0 + h] = (mm[h] + log2f(t[h])) * 0.6931471805599453f;
       }
 #pragma unroll
-      for (int h = 0; h < 16; ++h) t[h] = t[h] == 0.f ? 0.f : p.v_ts / t[h];  // 0: every score is -inf
-      wait(pv, i & 1, kErrWaitFull);
+      for (int h = 0; h < 8; ++h) t[h] = t[h] == 0.f ? 0.f : p.v_ts / t[h];  // 0: every score is -inf
+      wait(&pv[sb], (i >> 1) & 1, kErrWaitFull);
       __syncwarp();
       tc::fence_after();
       // lane 8 q + g of warp w holds columns (8 w + g) 4 NB + q NB .. + NB - 1, one per block
       constexpr int NV = NB < 4 ? NB : 4;
-      const int col = (8 * warp + (lane & 7)) * 4 * NB + (lane >> 3) * NB;
+      const int col = (8 * w + (lane & 7)) * 4 * NB + (lane >> 3) * NB;
 #pragma unroll
       for (int b0 = 0; b0 < NB; b0 += NV) {
-        uint32_t o[NV][16];
+        uint32_t o[NV][8];
 #pragma unroll
-        for (int b = 0; b < NV; ++b) tc::ld16(lane_base + C::O + (b0 + b) * 16, o[b]);
+        for (int b = 0; b < NV; ++b) tc::ld8(lane_base + C::O + (b0 + b) * 16 + h0, o[b]);
         tc::wait_ld();
         if (room) {
-          float* dst = p.ws_o + static_cast<int64_t>(st.slot) * p.H * W + col + b0;
+          float* dst = p.ws_o + (static_cast<int64_t>(st.slot) * p.H + h0) * W + col + b0;
 #pragma unroll
-          for (int h = 0; h < 16; ++h) {
-            if (h >= p.H) continue;
+          for (int h = 0; h < 8; ++h) {
+            if (h0 + h >= p.H) continue;
             if constexpr (NV == 4)
               *reinterpret_cast<float4*>(dst + h * W) =
                   make_float4(__uint_as_float(o[0][h]) * t[h], __uint_as_float(o[1][h]) * t[h],
@@ -570,34 +587,53 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
         }
       }
       tc::fence_before();
-      named_bar_sync(1, 128);  // red and the output are read before they are written again
+      named_bar_sync(bar, 128);  // myred is read before it is written again
     }
-  } else if (warp == 4) {
-    // ------------------------------------------------------------------ products
+  } else if (warp == 24) {
+    // ------------------------------------------------------------------ score products
     if (tc::elect()) {
-      const uint64_t qd = tc::desc_sw128(smem_u32(qs)), pd = tc::desc_sw128(smem_u32(ps));
+      const uint64_t qd = tc::desc_sw128(smem_u32(qs));
       uint32_t c = 0;
+      int seg = 0;
       for (uint32_t i = 0; st.next(); ++i) {
+        if (st.first) {
+          wait(&qf[seg % kQSlots], (seg / kQSlots) & 1, kErrWaitFull);
+          ++seg;
+        }
+        if (i >= 2) wait(&se[i & 1], ((i >> 1) - 1) & 1, kErrWaitEmpty);
+        const uint32_t d = tmem + C::S + (i & 1) * 16;
 #pragma unroll
         for (int kc = 0; kc < W / 128; ++kc, ++c) {
-          wait(&af[c & 1], (c >> 1) & 1, kErrWaitFull);
+          const uint32_t buf = c % C::BUFS;
+          wait(&akf[buf], (c / C::BUFS) & 1, kErrWaitFull);
           tc::fence_after();
-          const uint32_t a = tmem + C::A + (c & 1) * 64;
+          const uint32_t a = tmem + C::AK + buf * 64;
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            tc::mma_ts(tmem + C::S, a + ks * 8, qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16,
-                       tc::idesc(0, 128, 16), kc | ks);
-          tc::commit(&ae[c & 1]);
+            tc::mma_ts(d, a + ks * 8, qd + ((kc * 2 + (ks >> 2)) * 2048 + (ks & 3) * 32) / 16, tc::idesc(0, 128, 16),
+                       kc | ks);
+          tc::commit(&ake[buf]);
         }
-        tc::commit(sf);
-        wait(pf, i & 1, kErrWaitFull);
+        tc::commit(&sf[i & 1]);
+      }
+      tc::commit(&drain[0]);
+      if (!mbar_wait(&drain[0], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
+    }
+  } else if (warp == 25) {
+    // ------------------------------------------------------------------ value products
+    if (tc::elect()) {
+      uint32_t c = 0;
+      for (uint32_t i = 0; st.next(); ++i) {
+        wait(&pf[i & 1], (i >> 1) & 1, kErrWaitFull);
+        const uint64_t pd = tc::desc_sw128(smem_u32(ps) + (i & 1) * 4096);
         const uint32_t keep = !st.first;
 #pragma unroll
         for (int t0 = 0; t0 < 8; t0 += C::VT, ++c) {
           if (t0 >= st.n) break;
-          wait(&af[c & 1], (c >> 1) & 1, kErrWaitFull);
+          const uint32_t buf = c % C::BUFS;
+          wait(&avf[buf], (c / C::BUFS) & 1, kErrWaitFull);
           tc::fence_after();
-          const uint32_t a = tmem + C::A + (c & 1) * 64;
+          const uint32_t a = tmem + C::AV + buf * C::VCOLS;
 #pragma unroll
           for (int ti = 0; ti < C::VT; ++ti) {
             const int t = t0 + ti;
@@ -607,58 +643,45 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
               tc::mma_ts(tmem + C::O + b * 16, a + b * (C::VT * 8) + ti * 8, pd + ((t >> 2) * 2048 + (t & 3) * 32) / 16,
                          tc::idesc(0, 128, 16), t ? 1u : keep);
           }
-          tc::commit(&ae[c & 1]);
+          tc::commit(&ave[buf]);
         }
-        tc::commit(pv);
+        tc::commit(&pv[i & 1]);
       }
-      tc::commit(drain);
-      if (!mbar_wait(drain, 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
+      tc::commit(&drain[1]);
+      if (!mbar_wait(&drain[1], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
     }
   } else {
-    // ------------------------------------------------------------------ tile copies: a step's K units, then its V units
+    // ------------------------------------------------------------------ tile copies
     // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
     const uint64_t policy = l2_policy_evict_first();
-    // lanes 0 .. 15 take the codes of a tile each, lanes 16 .. 31 the scales
-    const int mine = lane & 15;
-    const uint32_t bytes = lane < 16 ? 8 * W : W / 2;
-    const uint32_t dst_off = (lane < 16 ? 0 : C::SCALES) + mine * bytes;
-    int unit = 0, ring = 0;
-    uint32_t phase = 1;  // parity of a unit's last release
+    int unit = 0;
     while (st.next()) {
-      const int nu = (st.n + UT - 1) / UT;
-      for (int hu = 0; hu < 2 * nu; ++hu, ++unit) {
-        const bool v = hu >= nu;
-        const int t0 = (v ? hu - nu : hu) * UT, n = min(UT, st.n - t0);
-        const int t = st.tile + t0 + mine;
+      for (int t0 = 0; t0 < st.n; t0 += UT, ++unit) {
+        const int ring = unit % C::UNITS, n = min(UT, st.n - t0);
+        const int t = st.tile + t0 + lane;
         const int lp = t / p.tpp;
         int blk = -1;
-        if (mine < n) {
+        if (lane < n) {
           if (lp < p.max_blocks) blk = p.bt[static_cast<int64_t>(st.r) * p.bt_st + lp];
           if (blk < 0 || blk >= p.num_blocks) {
             record_error(p.err, kErrBlock);
             blk = -1;
           }
         }
-        wait(&empty[ring], phase, kErrWaitEmpty);
+        if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
         __syncwarp();
-        uint8_t* dst = units + ring * C::UNIT + dst_off;
-        const unsigned absent = __ballot_sync(0xffffffffu, mine < n && blk < 0);
-        if (mine < n && blk < 0) {  // a page outside the table or the cache reads as zeros
-          for (uint32_t o = 0; o < bytes; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
+        uint8_t* dst = units + ring * C::UNIT + lane * C::TILE;
+        const unsigned absent = __ballot_sync(0xffffffffu, lane < n && blk < 0);
+        if (lane < n && blk < 0) {  // a page outside the table or the cache reads as zeros
+          for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent & 0xffffu)) * (C::TILE / 2));
+        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent)) * C::TILE);
         __syncwarp();
-        if (mine < n && blk >= 0)
-          tc::bulk_load(dst,
-                        p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE +
-                            (lane < 16 ? (v ? 8 * W : 0) : 16 * W + (v ? W / 2 : 0)),
-                        bytes, &full[ring], policy);
-        if (++ring == C::UNITS) {
-          ring = 0;
-          phase ^= 1;
-        }
+        if (lane < n && blk >= 0)
+          tc::bulk_load(dst, p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE,
+                        C::TILE, &full[ring], policy);
       }
     }
     // after an abort no role may have waited for the last copies: they must land before the CTA ends
@@ -668,7 +691,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, Q4Cfg<W>::CTAS) q4_history_ker
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 4) tc::dealloc(tmem, C::COLS);
+  if (warp == 24) tc::dealloc(tmem, 512);
 }
 
 template <int W>
@@ -701,8 +724,8 @@ static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, 
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // as many CTAs as shared and tensor memory hold at once; within the slots the plan's workspace holds
-  const int grid = std::min(plan.grid, sms * C::CTAS);
+  // one CTA per SM (its ring and tensor memory fill one); within the slots the plan's workspace holds
+  const int grid = std::min(plan.grid, sms);
   p.parts = grid;
   static unsigned attr_mask = 0;
   ensure_smem_limit(q4_history_kernel<W>, C::SMEM + 4 * (kHistoryMaxStreamRows + 1), attr_mask);
