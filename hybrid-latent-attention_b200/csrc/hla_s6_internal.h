@@ -117,6 +117,9 @@ int heads_cache_tmap(CUtensorMap* map, const void* base, int64_t num_blocks, int
 int contig_rows_tmap(CUtensorMap* map, const void* base, int64_t B, int64_t N, int W, int64_t st_b, int64_t st_n,
                      int tile);
 
+// 2-D TMA map over a [rows, cols] bf16 matrix with 128-row x 64-column boxes, SWIZZLE_128B (writer_tc.cu).
+int rows_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride_elems);
+
 // Targets of the fused sequence-split exchange (history_reduce_exchange): this rank's part - exchange
 // words z [T, H, W] then lse [H, T] - in every rank's receive slot, and the slot's local use counter
 // (the words carry the tag epoch + 1).

@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // 2-D TMA map over a [rows, K] bf16 matrix with 128-row x 64-column boxes, SWIZZLE_128B.
-static int rows_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride_elems) {
+int rows_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride_elems) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   if (!fn) {
     void* ptr = nullptr;
@@ -637,7 +637,7 @@ static int rows_tmap(CUtensorMap* map, const void* base, int64_t rows, int64_t c
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled failed (%d) for the writer operands", static_cast<int>(r));
+    set_error("cuTensorMapEncodeTiled failed (%d) for a matrix of rows", static_cast<int>(r));
     return kStatusCuda;
   }
   return kStatusOk;
