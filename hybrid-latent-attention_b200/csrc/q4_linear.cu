@@ -27,73 +27,90 @@ struct Q4LinearParams {
   int64_t res_st;
   __nv_bfloat16* out;
   int64_t o_st;
-  int vec;  // out (and residual) rows are 16-byte aligned
+  int vec;    // out (and residual) rows are 16-byte aligned
+  int split;  // CTAs of a cluster that share a tile's K (many tokens)
   uint64_t wait_ns;
 };
 
 // ------------------------------------------------------------------ few tokens
 constexpr int kQ4LinWarps = 8;
+constexpr int kQ4FewTokens = 64;
 
-template <int NT>
-__global__ void __launch_bounds__(kQ4LinWarps * 32) q4_linear_few_kernel(const Q4LinearParams p) {
-  __shared__ float red[kQ4LinWarps][NT][4][32];
+// A CTA: RT tiles of 16 output features x 8 NT tokens, K split over its 8 warps, which meet in shared memory.
+template <int NT, int RT>
+__global__ void __launch_bounds__(kQ4LinWarps * 32, NT == 1 ? 4 : 1) q4_linear_few_kernel(const Q4LinearParams p) {
+  __shared__ float red[kQ4LinWarps][RT][NT][4][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int kt_n = (p.K + 127) / 128, t0 = blockIdx.y * (8 * NT);
-  float acc[NT][4];
+  const int kt_n = (p.K + 127) / 128, t0 = blockIdx.y * (8 * NT), n_tiles = (p.N + 15) / 16;
+  float acc[RT][NT][4] = {};
+  const int64_t tile_row = static_cast<int64_t>(kt_n) * kQ4WeightTile;
+  const uint8_t* tile = p.w + blockIdx.x * RT * tile_row + warp * kQ4WeightTile;
+  const bool live0 = t0 + g < p.T;
+#pragma unroll 1
+  for (int kt = warp; kt < kt_n; kt += kQ4LinWarps, tile += kQ4LinWarps * kQ4WeightTile) {
+    uint4 lo[RT], hi[RT];
+    uint32_t sb[RT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  for (int kt = warp; kt < kt_n; kt += kQ4LinWarps) {
-    const uint8_t* tile = p.w + (static_cast<int64_t>(blockIdx.x) * kt_n + kt) * kQ4WeightTile;
-    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(tile) + lane);
-    const uint4 hi = __ldg(reinterpret_cast<const uint4*>(tile + 512) + lane);
-    const uint32_t sb = __ldg(reinterpret_cast<const uint16_t*>(tile + 1024) + lane);
+    for (int i = 0; i < RT; ++i) {
+      const bool ok = blockIdx.x * RT + i < n_tiles;  // tiles past the last read the first one's bytes, unused
+      const uint8_t* at = tile + (ok ? i * tile_row : 0);
+      lo[i] = __ldg(reinterpret_cast<const uint4*>(at) + lane);
+      hi[i] = __ldg(reinterpret_cast<const uint4*>(at + 512) + lane);
+      sb[i] = __ldg(reinterpret_cast<const uint16_t*>(at + 1024) + lane);
+    }
     uint4 xb[NT][4];
     const int col = kt * 128 + 32 * c;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int t = t0 + 8 * j + g;
-      const bool in = t < p.T && col < p.K;
-      const uint4* src = reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(t) * p.x_st + col);
+      const bool in = (NT == 1 ? live0 : t0 + 8 * j + g < p.T) && col < p.K;
+      const uint4* src = reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(t0 + 8 * j + g) * p.x_st + col);
 #pragma unroll
       for (int i = 0; i < 4; ++i) xb[j][i] = in ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
     }
-    const uint32_t s2 = e4m3x2_to_bf2(sb);
-    const Q4Scale s0(__byte_perm(s2, 0, 0x1010)), s1(__byte_perm(s2, 0, 0x3232));
-    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a0[4] = {q4_pair<0>(wl[i], s0), q4_pair<0>(wh[i], s1), q4_pair<1>(wl[i], s0),
-                              q4_pair<1>(wh[i], s1)};
-      const uint32_t a1[4] = {q4_pair<2>(wl[i], s0), q4_pair<2>(wh[i], s1), q4_pair<3>(wl[i], s0),
-                              q4_pair<3>(wh[i], s1)};
+    for (int r = 0; r < RT; ++r) {
+      const uint32_t s2 = e4m3x2_to_bf2(sb[r]);
+      const Q4Scale s0(__byte_perm(s2, 0, 0x1010)), s1(__byte_perm(s2, 0, 0x3232));
+      const uint32_t wl[4] = {lo[r].x, lo[r].y, lo[r].z, lo[r].w}, wh[4] = {hi[r].x, hi[r].y, hi[r].z, hi[r].w};
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma_bf16_16816(acc[j], a0, xb[j][i].x, xb[j][i].y);
-        mma_bf16_16816(acc[j], a1, xb[j][i].z, xb[j][i].w);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a0[4] = {q4_pair<0>(wl[i], s0), q4_pair<0>(wh[i], s1), q4_pair<1>(wl[i], s0),
+                                q4_pair<1>(wh[i], s1)};
+        const uint32_t a1[4] = {q4_pair<2>(wl[i], s0), q4_pair<2>(wh[i], s1), q4_pair<3>(wl[i], s0),
+                                q4_pair<3>(wh[i], s1)};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_bf16_16816(acc[r][j], a0, xb[j][i].x, xb[j][i].y);
+          mma_bf16_16816(acc[r][j], a1, xb[j][i].z, xb[j][i].w);
+        }
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[warp][j][e][lane] = acc[j][e];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][r][j][e][lane] = acc[r][j][e];
   __syncthreads();
-  // element (row n, token t) of tile j: lane (n % 8) * 4 + (t % 8) / 2, register 2 (n / 8) + t % 2
-  for (int i = threadIdx.x; i < NT * 128; i += blockDim.x) {
-    const int nl = i & 15, tl = i >> 4, t = t0 + tl, n = blockIdx.x * 16 + nl;
+  // element (row n, token t) of a tile: lane (n % 8) * 4 + (t % 8) / 2, register 2 (n / 8) + t % 2
+  for (int i = threadIdx.x; i < RT * NT * 128; i += blockDim.x) {
+    const int nl = i & 15, r = (i >> 4) % RT, tl = i / (16 * RT), t = t0 + tl, n = (blockIdx.x * RT + r) * 16 + nl;
     if (t >= p.T || n >= p.N) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kQ4LinWarps; ++w) v += red[w][tl >> 3][2 * (nl >> 3) + (tl & 1)][(nl & 7) * 4 + ((tl & 7) >> 1)];
+    for (int w = 0; w < kQ4LinWarps; ++w)
+      v += red[w][r][tl >> 3][2 * (nl >> 3) + (tl & 1)][(nl & 7) * 4 + ((tl & 7) >> 1)];
     v *= p.ts;
     if (p.res) v += __bfloat162float(p.res[static_cast<int64_t>(t) * p.res_st + n]);
     p.out[static_cast<int64_t>(t) * p.o_st + n] = __float2bfloat16_rn(v);
   }
 }
 
-template <int NT>
+template <int NT, int RT>
 static int launch_few(const Q4LinearParams& p, cudaStream_t s) {
-  q4_linear_few_kernel<NT><<<dim3((p.N + 15) / 16, (p.T + 8 * NT - 1) / (8 * NT)), kQ4LinWarps * 32, 0, s>>>(p);
+  q4_linear_few_kernel<NT, RT><<<dim3((p.N + 16 * RT - 1) / (16 * RT), (p.T + 8 * NT - 1) / (8 * NT)), kQ4LinWarps * 32, 0,
+                                 s>>>(p);
   return cuda_status(cudaGetLastError(), "q4_linear_few_kernel launch");
 }
 
@@ -101,10 +118,11 @@ static int launch_few(const Q4LinearParams& p, cudaStream_t s) {
 template <int BN>
 struct Q4Many {
   static constexpr int A_BYTES = 128 * 64 * 2, B_BYTES = BN * 64 * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 64 ? 4 : 4;
+  static constexpr int STAGES = 4;
   static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
-  static constexpr int PER = BN / 128 > 0 ? BN / 128 : 1;  // 16-row tiles a dequantising warp takes per stage
-  static constexpr int DQ = BN / 16 / PER;                 // dequantising warps: 4 (BN 64) or 8
+  static constexpr int DQ = BN / 16;      // dequantising warps, one 16-row tile of the stage each
+  static constexpr int RED = BN + 4;      // floats per row of the partial tile that a cluster's CTAs exchange
+  static_assert(128 * RED * 4 <= STAGES * STAGE || BN > 64, "partial tile");
   static constexpr uint32_t COLS = BN;
 };
 
@@ -126,6 +144,55 @@ __device__ __forceinline__ void tma_load_rows(void* dst, const void* tmap, uint6
       : "memory");
 }
 
+// out[t, n .. n + 15] from the fp32 sums (columns past N left out).
+__device__ __forceinline__ void store16(const Q4LinearParams& p, int t, int n, float (&v)[16]) {
+  __nv_bfloat16* dst = p.out + static_cast<int64_t>(t) * p.o_st + n;
+  const __nv_bfloat16* rs = p.res ? p.res + static_cast<int64_t>(t) * p.res_st + n : nullptr;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] *= p.ts;
+  if (p.vec && n + 16 <= p.N) {
+    if (rs) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint4 u = reinterpret_cast<const uint4*>(rs)[q];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[8 * q + 2 * e] += __uint_as_float(w[e] << 16);
+          v[8 * q + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      reinterpret_cast<uint4*>(dst)[q] =
+          make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                     pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (n + e < p.N) dst[e] = __float2bfloat16_rn(v[e] + (rs ? __bfloat162float(rs[e]) : 0.f));
+  }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// 16 bytes of another CTA's shared memory, at the address `p` has in this one.
+__device__ __forceinline__ float4 ld_cluster(const void* p, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n"
+      ".reg .b32 a;\n"
+      "mapa.shared::cluster.u32 a, %4, %5;\n"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n"
+      "}\n"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(smem_u32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // warps 0 .. DQ-1 dequantise, then write the output; warp DQ: TMA of x; warp DQ + 1: products.
 template <int BN>
 __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kernel(
@@ -140,7 +207,11 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.y * 128, n0 = blockIdx.x * BN, NK = (p.K + 63) / 64, kt_n = (p.K + 127) / 128;
+  const int m0 = blockIdx.y * 128, n0 = blockIdx.x * BN, kt_n = (p.K + 127) / 128;
+  // this CTA's blocks of 64 columns of K
+  const int nk_all = (p.K + 63) / 64;
+  const int kfirst = static_cast<int>(stream_start(blockIdx.z, nk_all, p.split));
+  const int NK = static_cast<int>(stream_start(blockIdx.z + 1, nk_all, p.split)) - kfirst;
 
   if (warp == DQ) tc::alloc(tmem_slot, C::COLS);
   if (threadIdx.x == (DQ + 1) * 32) {
@@ -163,48 +234,50 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
     // lane: row 8 half + g of a 16-row tile, columns 32 c .. of the stage's 64
     const int half = lane >> 4, g = (lane >> 1) & 7, c = lane & 1, row = 8 * half + g;
     const int64_t tile_row = static_cast<int64_t>(kt_n) * kQ4WeightTile;
-    const uint8_t* base = p.w + (n0 / 16 + warp * C::PER) * tile_row;
-    const int n_tiles = (p.N + 15) / 16;
-    bool there[C::PER];
-#pragma unroll
-    for (int i = 0; i < C::PER; ++i) there[i] = n0 / 16 + warp * C::PER + i < n_tiles;
-    constexpr int AHEAD = 3;  // stages whose codes are in flight
-    uint4 code[AHEAD][C::PER];
-    uint32_t sb[AHEAD][C::PER];
-    auto fetch = [&](int kb, uint4 (&cd)[C::PER], uint32_t (&s)[C::PER]) {
-#pragma unroll
-      for (int i = 0; i < C::PER; ++i) {
-        const uint8_t* tile = base + i * tile_row + static_cast<int64_t>(kb >> 1) * kQ4WeightTile;
-        const int cc = 2 * (kb & 1) + c;
-        const bool ok = there[i] && kb < NK;
-        cd[i] = ok ? __ldg(reinterpret_cast<const uint4*>(tile + half * 512 + (g * 4 + cc) * 16)) : make_uint4(0u, 0u, 0u, 0u);
-        s[i] = ok ? __ldg(tile + 1024 + (g * 4 + cc) * 2 + half) : 0u;
+    const bool there = n0 / 16 + warp < (p.N + 15) / 16;
+    // a block of 64 columns is half a tile; pairs of blocks advance by a tile
+    const uint8_t* src = p.w + (n0 / 16 + warp) * tile_row + static_cast<int64_t>(kfirst >> 1) * kQ4WeightTile;
+    const uint32_t code_at = half * 512 + (g * 4 + c) * 16, scale_at = 1024 + (g * 4 + c) * 2 + half;
+    constexpr int AHEAD = 4;  // blocks whose codes are in flight
+    uint4 code[AHEAD];
+    uint32_t sb[AHEAD];
+    int kf = kfirst;                     // next block to fetch
+    const int kend = there ? kfirst + NK : 0;
+    auto fetch = [&](uint4& cd, uint32_t& s) {
+      cd = make_uint4(0u, 0u, 0u, 0u);
+      s = 0u;
+      if (kf < kend) {
+        const uint8_t* at = src + (kf & 1) * 32;
+        cd = __ldg(reinterpret_cast<const uint4*>(at + code_at));
+        s = __ldg(src + (kf & 1) * 4 + scale_at);
       }
+      if (kf & 1) src += kQ4WeightTile;
+      ++kf;
     };
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) fetch(a, code[a], sb[a]);
-    for (int kb0 = 0; kb0 < NK; kb0 += AHEAD) {
+    for (int a = 0; a < AHEAD; ++a) fetch(code[a], sb[a]);
+    // the four 16-byte chunks of this thread's row in stage 0 (SWIZZLE_128B)
+    uint8_t* const b0 = smem + C::A_BYTES + (warp * 16 + row) * 128;
+    uint32_t off[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) off[j] = ((4 * c + j) ^ g) << 4;
+    static_assert(AHEAD == C::STAGES, "one fetched block per stage");
+    uint32_t phase = 1;
+    for (int kb0 = 0; kb0 < NK; kb0 += AHEAD, phase ^= 1) {
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const int kb = kb0 + a;
-        if (kb >= NK) break;
-        const int s = kb % C::STAGES;
-        if (kb >= C::STAGES) wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty);
-        uint8_t* b = smem + s * C::STAGE + C::A_BYTES;
+        if (kb0 + a >= NK) break;
+        wait(&empty[a], phase, kErrWaitEmpty);
+        const Q4Scale sc(e4m3x2_to_bf2(sb[a] | (sb[a] << 8)));
+        const uint32_t w[4] = {code[a].x, code[a].y, code[a].z, code[a].w};
 #pragma unroll
-        for (int i = 0; i < C::PER; ++i) {
-          const int r = (warp * C::PER + i) * 16 + row;
-          const Q4Scale sc(e4m3x2_to_bf2(sb[a][i] | (sb[a][i] << 8)));
-          const uint32_t w[4] = {code[a][i].x, code[a][i].y, code[a][i].z, code[a][i].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(b + r * 128 + (((4 * c + j) ^ (r & 7)) << 4)) =
-                make_uint4(q4_pair<0>(w[j], sc), q4_pair<1>(w[j], sc), q4_pair<2>(w[j], sc), q4_pair<3>(w[j], sc));
-        }
-        fetch(kb + AHEAD, code[a], sb[a]);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(b0 + a * C::STAGE + off[j]) =
+              make_uint4(q4_pair<0>(w[j], sc), q4_pair<1>(w[j], sc), q4_pair<2>(w[j], sc), q4_pair<3>(w[j], sc));
+        fetch(code[a], sb[a]);
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
+        if (lane == 0) mbar_arrive(&full[a]);
       }
     }
     // ---- output: this warp's 32 rows (tokens), its share of the columns
@@ -220,36 +293,20 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
       uint32_t r[16];
       tc::ld16(acc + c0, r);
       tc::wait_ld();
+      if (BN == 64 && p.split > 1) {  // this CTA's part of the sum, for the cluster
+        float4* dst = reinterpret_cast<float4*>(smem + ((warp & 3) * 32 + lane) * C::RED * 4 + (cw + c0) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          dst[e] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]),
+                               __uint_as_float(r[4 * e + 3]));
+        continue;
+      }
       const int n = n0 + cw + c0;
       if (t >= p.T || n >= p.N) continue;
-      __nv_bfloat16* dst = p.out + static_cast<int64_t>(t) * p.o_st + n;
-      const __nv_bfloat16* rs = p.res ? p.res + static_cast<int64_t>(t) * p.res_st + n : nullptr;
       float v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) * p.ts;
-      if (p.vec && n + 16 <= p.N) {
-        if (rs) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint4 u = reinterpret_cast<const uint4*>(rs)[q];
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[8 * q + 2 * e] += __uint_as_float(w[e] << 16);
-              v[8 * q + 2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
-            }
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          reinterpret_cast<uint4*>(dst)[q] =
-              make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                         pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (n + e < p.N) dst[e] = __float2bfloat16_rn(v[e] + (rs ? __bfloat162float(rs[e]) : 0.f));
-      }
+      for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]);
+      store16(p, t, n, v);
     }
   } else if (warp == DQ) {
     if (lane == 0) {
@@ -258,7 +315,7 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
         const int s = kb % C::STAGES;
         if (kb >= C::STAGES) wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty);
         mbar_arrive_expect_tx(&full[s], C::A_BYTES);
-        tma_load_rows(smem + s * C::STAGE, &tmap_x, &full[s], kb * 64, m0);  // rows and columns past x are zeros
+        tma_load_rows(smem + s * C::STAGE, &tmap_x, &full[s], (kfirst + kb) * 64, m0);  // rows and columns past x are zeros
       }
       // the last copies land before the CTA ends, also when a wait has given up
       for (int kb = max(0, NK - C::STAGES); kb < NK; ++kb) mbar_wait(&full[kb % C::STAGES], (kb / C::STAGES) & 1, p.wait_ns);
@@ -277,6 +334,32 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
     tc::commit(done);
     mbar_wait(done, 0, p.wait_ns);
   }
+  if constexpr (BN == 64) {
+    if (p.split > 1) {
+      // the cluster's CTAs hold a part of the sum each; CTA k adds up and writes every split-th row from k
+      cluster_sync();
+      const int rows = min(128, p.T - m0);
+      for (int u = threadIdx.x; u < ((rows - static_cast<int>(blockIdx.z) + p.split - 1) / p.split) * (BN / 4); u += blockDim.x) {
+        const int r = u / (BN / 4) * p.split + blockIdx.z, c0 = u % (BN / 4) * 4, t = m0 + r, n = n0 + c0;
+        if (n >= p.N) continue;
+        float4 part[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) part[k] = k < p.split ? ld_cluster(smem + (r * C::RED + c0) * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // in order: the sum does not depend on which CTA adds
+          v[0] += part[k].x; v[1] += part[k].y; v[2] += part[k].z; v[3] += part[k].w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (n + e >= p.N) break;
+          const float rs = p.res ? __bfloat162float(p.res[static_cast<int64_t>(t) * p.res_st + n + e]) : 0.f;
+          p.out[static_cast<int64_t>(t) * p.o_st + n + e] = __float2bfloat16_rn(v[e] * p.ts + rs);
+        }
+      }
+      cluster_sync();  // no CTA's memory goes before the others have read it
+    }
+  }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -291,8 +374,19 @@ static int launch_many(const Q4LinearParams& p, cudaStream_t s) {
   if (rc) return rc;
   static unsigned attr_mask = 0;
   ensure_smem_limit(q4_linear_many_kernel<BN>, C::SMEM, attr_mask);
-  q4_linear_many_kernel<BN><<<dim3((p.N + BN - 1) / BN, (p.T + 127) / 128), (C::DQ + 2) * 32, C::SMEM, s>>>(tx, p);
-  return cuda_status(cudaGetLastError(), "q4_linear_many_kernel launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.N + BN - 1) / BN, (p.T + 127) / 128, p.split);
+  cfg.blockDim = dim3((C::DQ + 2) * 32);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = p.split;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, q4_linear_many_kernel<BN>, tx, p), "q4_linear_many_kernel launch");
 }
 
 }  // namespace hla
@@ -331,11 +425,16 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
   p.vec = a16(out, out_stride_t) && (!residual || a16(residual, residual_stride_t));
   p.wait_ns = wait_limit_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (num_tokens <= 8) return launch_few<1>(p, s);
-  if (num_tokens <= 16) return launch_few<2>(p, s);
-  if (num_tokens <= 32) return launch_few<4>(p, s);
-  const int64_t wide = static_cast<int64_t>((num_tokens + 127) / 128) * ((out_features + 255) / 256);
-  return wide >= 64 ? launch_many<256>(p, s) : launch_many<64>(p, s);
+  if (num_tokens <= 8) return out_features >= 16384 ? launch_few<1, 2>(p, s) : launch_few<1, 1>(p, s);
+  if (num_tokens <= 16) return launch_few<2, 1>(p, s);
+  if (num_tokens <= kQ4FewTokens) return launch_few<4, 2>(p, s);
+  const int64_t mt = (num_tokens + 127) / 128, wide = mt * ((out_features + 255) / 256);
+  p.split = 1;
+  if (wide >= 64) return launch_many<256>(p, s);
+  // K is split over a cluster while the CTAs still fit two to an SM and each keeps at least 4 blocks of it
+  const int64_t tiles = mt * ((out_features + 63) / 64);
+  while (p.split < 8 && tiles * p.split * 2 <= 296 && (in_features + 63) / 64 >= 8 * p.split) p.split *= 2;
+  return launch_many<64>(p, s);
 }
 
 }  // extern "C"

@@ -57,28 +57,56 @@ def new_cache(num_blocks, page, width, device='cuda'):
     return torch.zeros(num_blocks, 1, page, row_bytes(width), dtype=torch.uint8, device=device)
 
 
-def _on_device(*tensors):
-    """Every tensor on one CUDA device, which is made current for the launch."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != dev):
-            raise ValueError('S6 4-bit ops take CUDA tensors of one device (no CPU path exists)')
-    return torch.cuda.device(dev)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _device_of(first, *rest):
+    """The index of the one CUDA device that every tensor is on."""
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError('S6 4-bit ops take CUDA tensors of one device (no CPU path exists)')
+    return index
+
+
+def _launch(index, name, *args):
+    """Entry point ``name`` with ``args`` and the current stream of device ``index``, which is made current for the
+    launch.  (Plain ints and the raw stream handle: the calls of one token's step cost more on the host than on the
+    device.)"""
+    fn = getattr(_lib.load(), name)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _cache_geometry(cache, width):
     """``(num_blocks, block stride in bytes, page)`` of a 4-bit cache of latent width ``width``."""
-    if cache.dim() != 4 or cache.shape[1] != 1 or cache.shape[-1] != row_bytes(width) or cache.dtype != torch.uint8:
-        raise ValueError(f'a 4-bit latent cache of width {width} must be uint8 [num_blocks, 1, page, '
-                         f'{row_bytes(width)}], got {cache.dtype} {tuple(cache.shape)}')
-    if cache.stride(-1) != 1 or cache.stride(2) != cache.shape[-1]:
+    shape, bytes_ = cache.shape, 17 * width // 16
+    if len(shape) != 4 or shape[1] != 1 or shape[3] != bytes_ or cache.dtype != torch.uint8:
+        raise ValueError(f'a 4-bit latent cache of width {width} must be uint8 [num_blocks, 1, page, {bytes_}], got '
+                         f'{cache.dtype} {tuple(shape)}')
+    stride = cache.stride()
+    if stride[3] != 1 or stride[2] != bytes_:
         raise ValueError('the bytes of a 4-bit cache page must be contiguous')
-    return cache.shape[0], cache.stride(0), cache.shape[2]
+    return shape[0], stride[0], shape[2]
 
 
 def _block_table(table):
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(-1) != 1:
+    """``(row stride, rows, columns)`` of a block table."""
+    shape, stride = table.shape, table.stride()
+    if table.dtype != torch.int32 or len(shape) != 2 or stride[1] != 1:
         raise ValueError('block_table must be int32 [rows, max_blocks] with a unit last-dim stride')
+    return stride[0], shape[0], shape[1]
 
 
 def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, k_scale=1.0, v_scale=1.0,
@@ -86,30 +114,29 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
     """``s6_ops.history_attention`` over a 4-bit cache: ``(o [T, H, W] bf16, lse [H, T] fp32)`` of the softmax of
     ``q_lat [T, H, W]`` over the first ``ctx[t]`` rows; empty rows give ``o = 0``, ``lse = -inf``.
     ``error_flag`` (int32 [1], optional) receives 5 for a block-table entry outside the cache."""
-    if q_lat.dim() != 3 or q_lat.stride(-1) != 1 or q_lat.dtype != BF16:
+    if q_lat.dim() != 3 or q_lat.dtype != BF16 or q_lat.stride(2) != 1:
         raise ValueError('q_lat must be bf16 [T, H, W] with a unit last-dim stride')
     T, H, W = q_lat.shape
     nb, sb, page = _cache_geometry(cache, W)
-    _block_table(block_table)
-    if ctx.dtype != torch.int32 or ctx.shape != (T,) or block_table.shape[0] < T:
+    bt_stride, bt_rows, bt_cols = _block_table(block_table)
+    if ctx.dtype != torch.int32 or ctx.shape != (T,) or bt_rows < T:
         raise ValueError('ctx must be int32 [T] and block_table hold a row per token')
     if empty is not None:
         if empty.shape != (T,):
             raise ValueError('empty must be [T]')
         empty = empty.contiguous() if empty.dtype in (torch.bool, torch.uint8) else (empty != 0)
-    with _on_device(q_lat, cache, block_table, ctx, empty, error_flag):
-        need = T * H * num_kv_splits * (W + 1)
-        buffer = workspace.ensure(q_lat.device)
-        if need > buffer.numel():
-            raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {buffer.numel()}')
-        o = torch.empty(T, H, W, dtype=BF16, device=q_lat.device)
-        lse = torch.empty(H, T, dtype=torch.float32, device=q_lat.device)
-        ctx = ctx.contiguous()
-        _lib.call('hla_s6_history_attention_q4', q_lat.data_ptr(), q_lat.stride(0), q_lat.stride(1), cache.data_ptr(),
-                  nb, sb, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], ctx.data_ptr(),
-                  _lib.ptr(empty), T, H, W, page, float(scale), int(num_kv_splits), buffer.data_ptr(), need,
-                  float(k_scale), float(v_scale), o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(),
-                  _lib.ptr(error_flag), _lib.stream_of(q_lat))
+    buffer = workspace.ensure(q_lat.device)
+    index = _device_of(q_lat, cache, block_table, ctx, empty, error_flag, buffer)
+    need = T * H * num_kv_splits * (W + 1)
+    if need > buffer.numel():
+        raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {buffer.numel()}')
+    o = q_lat.new_empty((T, H, W))
+    lse = q_lat.new_empty((H, T), dtype=torch.float32)
+    ctx = ctx.contiguous()
+    _launch(index, 'hla_s6_history_attention_q4', q_lat.data_ptr(), q_lat.stride(0), q_lat.stride(1), cache.data_ptr(),
+            nb, sb, block_table.data_ptr(), bt_stride, bt_cols, ctx.data_ptr(),
+            _address(empty), T, H, W, page, scale, num_kv_splits, buffer.data_ptr(), need, k_scale, v_scale,
+            o.data_ptr(), H * W, W, lse.data_ptr(), _address(error_flag))
     return o, lse
 
 
@@ -118,24 +145,25 @@ def commit_rows(row, positions, table, cache, block_table, query_start_loc, k_sc
     ``positions [T]`` (int64), both halves quantised and stored at ``block_table[request, pos // page] * page +
     pos % page``.  Returns the slots (int64 [T]); padding tokens (``t >= query_start_loc[-1]``) and positions
     without a block in the cache are skipped, their slot is -1.  Two tokens of one call must not share a slot."""
-    if row.dim() != 2 or row.dtype != BF16 or row.stride(-1) != 1:
+    if row.dim() != 2 or row.dtype != BF16 or row.stride(1) != 1:
         raise ValueError('row must be bf16 [T, 2 * width] with a unit last-dim stride')
-    T, W = row.shape[0], row.shape[1] // 2
+    T, W = row.shape
+    W //= 2
     nb, sb, page = _cache_geometry(cache, W)
-    if table.dim() != 2 or table.dtype != BF16 or table.stride(-1) != 1 or table.shape[1] != W:
+    if table.dim() != 2 or table.dtype != BF16 or table.stride(1) != 1 or table.shape[1] != W:
         raise ValueError(f'table must be bf16 [max_position, {W}] = [cos | sin]')
-    _block_table(block_table)
+    bt_stride, bt_rows, bt_cols = _block_table(block_table)
+    requests = query_start_loc.numel() - 1
     if (positions.dtype != torch.int64 or positions.shape != (T,) or query_start_loc.dtype != torch.int32
-            or query_start_loc.dim() != 1 or block_table.shape[0] < query_start_loc.shape[0] - 1):
+            or query_start_loc.dim() != 1 or bt_rows < requests):
         raise ValueError('positions must be int64 [T], query_start_loc int32 [R + 1], block_table [R, max_blocks]')
-    with _on_device(row, positions, table, cache, block_table, query_start_loc):
-        positions, query_start_loc = positions.contiguous(), query_start_loc.contiguous()
-        slots = torch.empty(T, dtype=torch.int64, device=row.device)
-        _lib.call('hla_s6_commit_rows_q4', row.data_ptr(), row.stride(0), W, positions.data_ptr(), table.data_ptr(),
-                  table.stride(0), table.shape[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
-                  block_table.stride(0), block_table.shape[1], query_start_loc.data_ptr(),
-                  query_start_loc.shape[0] - 1, T, float(k_scale), float(v_scale), slots.data_ptr(),
-                  _lib.stream_of(row))
+    index = _device_of(row, positions, table, cache, block_table, query_start_loc)
+    positions, query_start_loc = positions.contiguous(), query_start_loc.contiguous()
+    slots = positions.new_empty((T,))
+    _launch(index, 'hla_s6_commit_rows_q4', row.data_ptr(), row.stride(0), W, positions.data_ptr(), table.data_ptr(),
+            table.stride(0), table.shape[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
+            bt_stride, bt_cols, query_start_loc.data_ptr(), requests, T, k_scale, v_scale,
+            slots.data_ptr())
     return slots
 
 
@@ -149,15 +177,15 @@ def _gather(cache, blocks, slots, rows, k_scale, v_scale, out, error_flag):
         raise IndexError('the block list does not cover the rows')
     if out is not None and (out.shape != (rows, 2 * W) or out.dtype != BF16 or out.stride(-1) != 1):
         raise ValueError(f'out must be bf16 [{rows}, {2 * W}] with a unit last-dim stride')
-    with _on_device(cache, index, out, error_flag):
-        index = index.contiguous()
-        if out is None:
-            out = torch.empty(rows, 2 * W, dtype=BF16, device=cache.device)
-        if rows:
-            _lib.call('hla_s6_gather_rows_q4', cache.data_ptr(), nb, sb, W, page,
-                      index.data_ptr() if slots is None else None, None if slots is None else index.data_ptr(), rows,
-                      float(k_scale), float(v_scale), out.data_ptr(), out.stride(0), _lib.ptr(error_flag),
-                      _lib.stream_of(cache))
+    device = _device_of(cache, index, out, error_flag)
+    index = index.contiguous()
+    if out is None:
+        out = cache.new_empty((rows, 2 * W), dtype=BF16)
+    if rows:
+        at = index.data_ptr()
+        _launch(device, 'hla_s6_gather_rows_q4', cache.data_ptr(), nb, sb, W, page, at if slots is None else None,
+                None if slots is None else at, rows, k_scale, v_scale, out.data_ptr(), out.stride(0),
+                _address(error_flag))
     return out
 
 
@@ -185,13 +213,17 @@ def quantize_weight(weight, scale=None):
     N, K = weight.shape
     if K < GROUP or K % GROUP or N < 1:
         raise ValueError('a 4-bit weight needs in_features a multiple of 32')
-    with _on_device(weight):
-        if scale is None:
-            scale = tensor_scale(float(weight.abs().amax()))
-        packed = torch.empty(weight_tiles(N, K), dtype=torch.uint8, device=weight.device)
-        _lib.call('hla_s6_quantize_weight_q4', weight.data_ptr(), weight.stride(0), N, K, float(scale),
-                  packed.data_ptr(), _lib.stream_of(weight))
+    index = _device_of(weight)
+    if scale is None:
+        scale = tensor_scale(float(weight.abs().amax()))
+    packed = weight.new_empty(weight_tiles(N, K), dtype=torch.uint8)
+    _launch(index, 'hla_s6_quantize_weight_q4', weight.data_ptr(), weight.stride(0), N, K, scale, packed.data_ptr())
     return packed, float(scale)
+
+
+def _check_rows(y, T, N):
+    if y.shape != (T, N) or y.dtype != BF16 or y.stride(1) != 1:
+        raise ValueError(f'residual and out must be bf16 [{T}, {N}] with a unit last-dim stride')
 
 
 def linear(x, packed, out_features, scale, residual=None, out=None):
@@ -200,17 +232,20 @@ def linear(x, packed, out_features, scale, residual=None, out=None):
     if x.dim() != 2 or x.dtype != BF16 or x.stride(-1) != 1:
         raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
     T, K = x.shape
-    N = int(out_features)
-    if packed.dtype != torch.uint8 or packed.shape != weight_tiles(N, K) or not packed.is_contiguous():
+    N = out_features
+    if (packed.dtype != torch.uint8 or packed.shape != (-(-N // 16), -(-K // 128), WEIGHT_TILE_BYTES)
+            or not packed.is_contiguous()):
         raise ValueError(f'packed must be contiguous uint8 {list(weight_tiles(N, K))}, got {packed.dtype} '
                          f'{list(packed.shape)}')
-    for y in (residual, out):
-        if y is not None and (y.shape != (T, N) or y.dtype != BF16 or y.stride(-1) != 1):
-            raise ValueError(f'residual and out must be bf16 [{T}, {N}] with a unit last-dim stride')
-    with _on_device(x, packed, residual, out):
-        if out is None:
-            out = torch.empty(T, N, dtype=BF16, device=x.device)
-        _lib.call('hla_s6_linear_q4', x.data_ptr(), x.stride(0), packed.data_ptr(), T, N, K, float(scale),
-                  _lib.ptr(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
-                  _lib.stream_of(x))
+    if x.stride(0) < K and T > 1:
+        x = x.contiguous()   # rows that overlap (an expanded x)
+    if residual is not None:
+        _check_rows(residual, T, N)
+    if out is not None:
+        _check_rows(out, T, N)
+    index = _device_of(x, packed, residual, out)
+    if out is None:
+        out = x.new_empty((T, N))
+    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x.stride(0), packed.data_ptr(), T, N, K, scale,
+            _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0))
     return out
