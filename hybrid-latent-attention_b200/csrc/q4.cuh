@@ -124,22 +124,37 @@ __device__ __forceinline__ uint32_t q4_scale_byte(float amax, float ts) {
 __device__ __forceinline__ float q4_scale_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }
-// Code of x in a group whose step is s * ts (0: a group of zeros).  |x| / step < 7.5 except where the scale
-// saturated or was rounded in e4m3's subnormal range, hence the clamp; an infinity takes
-// the group's largest code, a NaN code 1 (the stored rows hold no NaN).
-__device__ __forceinline__ uint32_t q4_code(float x, float step) {
-  if (!(step > 0.f)) return 8u;
-  return static_cast<uint32_t>(8 + static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x, step)), -7.f), 7.f)));
-}
+// Codes of a group whose step is s * ts: 8 + x / step rounded to nearest, ties to even, clamped to 1..15 (by
+// clamping x to 7 steps: |x| / step < 7.5 except where the scale saturated or was rounded in e4m3's subnormal range).
+// An infinity takes the group's largest code, a NaN code 1 (the stored rows hold no NaN); a step of 0 gives 8.
+// No division: z = x * inv + 1.5 * 2^23 + 8 has the rounded sum in its low bits.  inv = 1 / step is itself rounded, so
+// where x / step is (almost) half way z may have gone the wrong way; the remainder x - q step, exact for power-of-two
+// tensor scales (8 bits minus 3 x 4 bits), tells: more than half a step, or half a step from an odd code, moves the
+// code by one towards it.
+struct Q4Coder {
+  float step, inv, lim;
+  uint32_t half;  // bits of step / 2
+  __device__ __forceinline__ explicit Q4Coder(float step_) {
+    step = step_;
+    inv = step_ > 0.f ? __frcp_rn(step_) : 0.f;
+    lim = 7.f * step_;
+    half = step_ > 0.f ? __float_as_uint(0.5f * step_) : 0x7f800000u;
+  }
+  __device__ __forceinline__ uint32_t operator()(float x) const {
+    constexpr float kMagic = 12582912.f + 8.f;
+    x = fminf(fmaxf(x, -lim), lim);
+    const uint32_t z = __float_as_uint(fmaf(x, inv, kMagic));
+    const uint32_t r = __float_as_uint(fmaf(kMagic - __uint_as_float(z), step, x));
+    const uint32_t towards = static_cast<uint32_t>(static_cast<int32_t>(r) >> 31) | 1u;
+    return (z + ((r & 0x7fffffffu) + (z & 1u) > half ? towards : 0u)) & 15u;
+  }
+};
 // The word of 8 columns' codes.
 __device__ __forceinline__ uint32_t q4_word(const uint32_t (&n)[8]) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w |= (n[2 * i] << (4 * i)) | (n[2 * i + 1] << (16 + 4 * i));
   return w;
-}
-__device__ __forceinline__ int q4_code_at(uint32_t w, int col) {
-  return static_cast<int>((w >> (4 * (col >> 1) + 16 * (col & 1))) & 15u) - 8;
 }
 
 }  // namespace hla

@@ -26,10 +26,10 @@ __device__ __forceinline__ uint32_t quantize8(const float (&f)[8], float ts, uin
   a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
   a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
   scale = q4_scale_byte(a, ts);
-  const float step = q4_scale_value(scale) * ts;
+  const Q4Coder code(q4_scale_value(scale) * ts);
   uint32_t n[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = q4_code(f[i], step);
+  for (int i = 0; i < 8; ++i) n[i] = code(f[i]);
   return q4_word(n);
 }
 
@@ -62,23 +62,21 @@ __global__ void __launch_bounds__(kQ4CommitThreads) q4_commit_kernel(const Q4Com
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (kQ4CommitThreads / PER) + threadIdx.x / PER;
   const int k = threadIdx.x % PER;
   const bool in = t < a.T;
+  // every load that does not need the slot goes out before the chain of lookups that finds it
+  uint4 raw[6] = {};
   int64_t slot = -1;
-  int64_t pos = 0;
   if (in) {
-    pos = a.positions[t];
+    const __nv_bfloat16* src = a.row + t * a.row_st + 8 * k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * (W / 2)));
+    const int64_t pos = a.positions[t];
+    const __nv_bfloat16* tab = a.table + clamp_pos(pos, a.max_pos) * a.tab_st + 8 * k;
+    raw[4] = __ldg(reinterpret_cast<const uint4*>(tab));
+    raw[5] = __ldg(reinterpret_cast<const uint4*>(tab + W / 2));
     slot = token_slot(qsl, a.R, static_cast<int>(t), pos, a.bt, a.bt_st, a.max_blocks, a.page, a.num_blocks);
     if (a.slot_out && k == 0) a.slot_out[t] = slot;
   }
   const bool live = slot >= 0;
-  uint4 raw[6] = {};
-  if (live) {
-    const __nv_bfloat16* src = a.row + t * a.row_st + 8 * k;
-    const __nv_bfloat16* tab = a.table + clamp_pos(pos, a.max_pos) * a.tab_st + 8 * k;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * (W / 2)));
-    raw[4] = __ldg(reinterpret_cast<const uint4*>(tab));
-    raw[5] = __ldg(reinterpret_cast<const uint4*>(tab + W / 2));
-  }
   float x[4][8], c[8], s[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) unpack8(raw[i], x[i]);
@@ -124,47 +122,53 @@ struct Q4GatherArgs {
   int* err;
 };
 
-// The 8 values of a word, times scale s (a float) and the tensor scale, in bf16.
+// The 8 values of a word in bf16: (n - 8) s is exact, the tensor scale is applied in fp32 and rounded once.
 __device__ __forceinline__ uint4 q4_values(uint32_t w, uint32_t scale, float ts) {
-  const float s = q4_scale_value(scale);
-  float f[8];
+  const Q4Scale s(e4m3x2_to_bf2(scale | (scale << 8)));
+  const uint32_t v[4] = {q4_pair<0>(w, s), q4_pair<1>(w, s), q4_pair<2>(w, s), q4_pair<3>(w, s)};
+  uint32_t r[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (static_cast<float>(q4_code_at(w, i)) * s) * ts;
-  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  for (int i = 0; i < 4; ++i) r[i] = pack_bf16(__uint_as_float(v[i] << 16) * ts, __uint_as_float(v[i] & 0xffff0000u) * ts);
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// W / 8 threads per row: thread k takes octet k of the K and of the V half.
 template <int W>
-__global__ void __launch_bounds__(128) q4_gather_kernel(const Q4GatherArgs a) {
-  constexpr int PER = W / 4;  // octets of a row, K and V
+__global__ void __launch_bounds__(256) q4_gather_kernel(const Q4GatherArgs a) {
+  constexpr int PER = W / 8;
   const Q4Tile tl(W);
-  for (int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; idx < a.rows * PER;
-       idx += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t i = idx / PER;
-    const int oc = static_cast<int>(idx % PER);
-    int64_t blk, off;
+  const int octet = threadIdx.x % PER, group = octet / 4;
+  const uint32_t page = a.page, cache_rows = static_cast<uint32_t>(a.num_blocks) * page;  // < 2^31 (checked)
+  for (uint32_t i = blockIdx.x * (256 / PER) + threadIdx.x / PER; i < a.rows; i += gridDim.x * (256 / PER)) {
+    uint32_t blk, off;
+    bool ok, skip = false;
     if (a.slots) {
       const int64_t s = a.slots[i];
-      blk = s < 0 ? -1 : s / a.page;
-      off = s < 0 ? 0 : s % a.page;
+      skip = s < 0;  // a padding token: zeros, no error
+      ok = !skip && s < cache_rows;
+      blk = ok ? static_cast<uint32_t>(s) / page : 0u;
+      off = ok ? static_cast<uint32_t>(s) - blk * page : 0u;
     } else {
-      blk = a.blocks[i / a.page];
-      off = i % a.page;
+      const uint32_t b = i / page;
+      blk = a.blocks[b];
+      off = i - b * page;
+      ok = blk < static_cast<uint32_t>(a.num_blocks);  // a negative id is a large one
     }
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (blk >= 0 && blk < a.num_blocks) {
-      const uint8_t* tile = a.cache + blk * a.c_sb + (off / 16) * tl.bytes();
+    uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
+    if (ok) {
+      const uint8_t* tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
       const int r = static_cast<int>(off % 16);
-      const int octet = oc < W / 8 ? oc : oc - W / 8, group = octet / 4;
-      if (oc < W / 8)
-        v = q4_values(__ldg(reinterpret_cast<const uint32_t*>(tile + tl.k_codes(group, r) + 4 * (octet & 3))),
-                      __ldg(tile + tl.k_scale(r, group)), a.k_ts);
-      else
-        v = q4_values(__ldg(reinterpret_cast<const uint32_t*>(tile + tl.v_codes(octet, r))),
-                      __ldg(tile + tl.v_scale(group, r)), a.v_ts);
-    } else if (oc == 0 && !(a.slots && blk < 0)) {
+      const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.k_codes(group, r) + 4 * (octet & 3)));
+      const uint32_t vw = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.v_codes(octet, r)));
+      const uint32_t ks = __ldg(tile + tl.k_scale(r, group)), vs = __ldg(tile + tl.v_scale(group, r));
+      k = q4_values(kw, ks, a.k_ts);
+      v = q4_values(vw, vs, a.v_ts);
+    } else if (octet == 0 && !skip) {
       record_error(a.err, kErrBlock);
     }
-    *reinterpret_cast<uint4*>(a.out + i * a.o_st + 8 * oc) = v;
+    __nv_bfloat16* out = a.out + static_cast<int64_t>(i) * a.o_st + 8 * octet;
+    *reinterpret_cast<uint4*>(out) = k;
+    *reinterpret_cast<uint4*>(out + W) = v;
   }
 }
 
@@ -262,9 +266,11 @@ int hla_s6_gather_rows_q4(const void* cache, int64_t num_blocks, int64_t cache_s
   if (!q4_cache_ok(cache, cache_stride_block, width, page, "gather rows (4 bit)") ||
       !q4_ts_ok(k_scale, v_scale, "gather rows (4 bit)"))
     return kStatusInvalid;
-  if (num_rows < 0 || (!blocks == !slots && num_rows > 0) || (out_stride % 8) || out_stride < 2 * width ||
+  if (num_rows < 0 || num_rows >= (int64_t(1) << 31) || num_blocks < 0 || num_blocks * page >= (int64_t(1) << 31) ||
+      (!blocks == !slots && num_rows > 0) || (out_stride % 8) || out_stride < 2 * width ||
       (reinterpret_cast<uintptr_t>(out) % 16)) {
-    set_error("gather rows (4 bit) needs a block list or slots (one of them) and 16-byte aligned output rows");
+    set_error("gather rows (4 bit) needs a block list or slots (one of them), fewer than 2^31 rows and 16-byte aligned "
+              "output rows");
     return kStatusInvalid;
   }
   if (num_rows == 0) return kStatusOk;
@@ -281,12 +287,12 @@ int hla_s6_gather_rows_q4(const void* cache, int64_t num_blocks, int64_t cache_s
   a.out = static_cast<__nv_bfloat16*>(out);
   a.o_st = out_stride;
   a.err = error_flag;
-  const int64_t want = (num_rows * (width / 4) + 127) / 128;
+  const int64_t per = 256 / (width / 8), want = (num_rows + per - 1) / per;
   const int grid = static_cast<int>(std::min<int64_t>(want, 148 * 64));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (width == 256) q4_gather_kernel<256><<<grid, 128, 0, s>>>(a);
-  else if (width == 512) q4_gather_kernel<512><<<grid, 128, 0, s>>>(a);
-  else q4_gather_kernel<1024><<<grid, 128, 0, s>>>(a);
+  if (width == 256) q4_gather_kernel<256><<<grid, 256, 0, s>>>(a);
+  else if (width == 512) q4_gather_kernel<512><<<grid, 256, 0, s>>>(a);
+  else q4_gather_kernel<1024><<<grid, 256, 0, s>>>(a);
   return cuda_status(cudaGetLastError(), "q4_gather_kernel launch");
 }
 
