@@ -64,7 +64,9 @@ __global__ void __launch_bounds__(kQ4CommitThreads) q4_commit_kernel(const Q4Com
   const bool in = t < a.T;
   // every load that does not need the slot goes out before the chain of lookups that finds it
   uint4 raw[6] = {};
-  int64_t slot = -1;
+  const Q4Tile tl(W);
+  uint8_t* tile = nullptr;  // NULL: no slot
+  int r = 0;
   if (in) {
     const __nv_bfloat16* src = a.row + t * a.row_st + 8 * k;
 #pragma unroll
@@ -73,26 +75,41 @@ __global__ void __launch_bounds__(kQ4CommitThreads) q4_commit_kernel(const Q4Com
     const __nv_bfloat16* tab = a.table + clamp_pos(pos, a.max_pos) * a.tab_st + 8 * k;
     raw[4] = __ldg(reinterpret_cast<const uint4*>(tab));
     raw[5] = __ldg(reinterpret_cast<const uint4*>(tab + W / 2));
-    slot = token_slot(qsl, a.R, static_cast<int>(t), pos, a.bt, a.bt_st, a.max_blocks, a.page, a.num_blocks);
+    // token_slot (decode_ops.cuh) with 32-bit divisions: a position inside the table is below 2^31 (checked)
+    int req;
+    int64_t slot = -1;
+    if (token_request(qsl, a.R, static_cast<int>(t), req) && pos >= 0 && pos < static_cast<int64_t>(a.max_blocks) * a.page) {
+      const uint32_t p32 = static_cast<uint32_t>(pos), page = a.page, col = p32 / page, off = p32 - col * page;
+      const int blk = a.bt[static_cast<int64_t>(req) * a.bt_st + col];
+      if (blk >= 0 && blk < a.num_blocks) {
+        slot = static_cast<int64_t>(blk) * a.page + off;
+        tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
+        r = static_cast<int>(off % 16);
+      }
+    }
     if (a.slot_out && k == 0) a.slot_out[t] = slot;
   }
-  const bool live = slot >= 0;
-  float x[4][8], c[8], s[8];
+  const bool live = tile != nullptr;
+  // latent RoPE of the K half in packed bf16 arithmetic: every operation rounds its exact result once, which on bf16
+  // inputs is the fp32 operation rounded to bf16 (a product is exact in fp32; a sum's first rounding is innocuous)
+  float x[4][8];
+  {
+    uint32_t* lo = reinterpret_cast<uint32_t*>(&raw[0]);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(&raw[1]);
+    const uint32_t* cs = reinterpret_cast<const uint32_t*>(&raw[4]);
+    const uint32_t* sn = reinterpret_cast<const uint32_t*>(&raw[5]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 x1 = *reinterpret_cast<const __nv_bfloat162*>(lo + i), x2 = *reinterpret_cast<const __nv_bfloat162*>(hi + i);
+      const __nv_bfloat162 c = *reinterpret_cast<const __nv_bfloat162*>(cs + i), s = *reinterpret_cast<const __nv_bfloat162*>(sn + i);
+      const __nv_bfloat162 y1 = __hadd2_rn(__hmul2_rn(x1, c), __hneg2(__hmul2_rn(x2, s)));
+      const __nv_bfloat162 y2 = __hadd2_rn(__hmul2_rn(x2, c), __hmul2_rn(x1, s));
+      lo[i] = *reinterpret_cast<const uint32_t*>(&y1);
+      hi[i] = *reinterpret_cast<const uint32_t*>(&y2);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) unpack8(raw[i], x[i]);
-  unpack8(raw[4], c);
-  unpack8(raw[5], s);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) rope_pair_torch(x[0][i], x[1][i], c[i], s[i], x[0][i], x[1][i]);
-  const Q4Tile tl(W);
-  uint8_t* tile = nullptr;
-  int r = 0;
-  if (live) {
-    const int64_t blk = slot / a.page;
-    const int off = static_cast<int>(slot - blk * a.page);
-    tile = a.cache + blk * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
-    r = off % 16;
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t sb;
@@ -225,10 +242,11 @@ int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, 
   if (!q4_cache_ok(cache, cache_stride_block, width, page, "commit rows (4 bit)") ||
       !q4_ts_ok(k_scale, v_scale, "commit rows (4 bit)"))
     return kStatusInvalid;
-  if (num_tokens < 0 || num_reqs < 1 || max_position < 1 || table_stride < width || (table_stride % 8) ||
+  if (num_tokens < 0 || num_reqs < 1 || max_position < 1 || table_stride < width || max_blocks < 0 ||
+      static_cast<int64_t>(max_blocks) * page >= (int64_t(1) << 31) || (table_stride % 8) ||
       (row_stride_t % 8) || (reinterpret_cast<uintptr_t>(row) % 16) || (reinterpret_cast<uintptr_t>(table) % 16)) {
-    set_error("commit rows (4 bit) needs >= 1 request, a [max_position, width] table and 16-byte aligned row and "
-              "table rows");
+    set_error("commit rows (4 bit) needs >= 1 request, a [max_position, width] table, a block table of fewer than 2^31 "
+              "positions and 16-byte aligned row and table rows");
     return kStatusInvalid;
   }
   if (num_tokens == 0) return kStatusOk;
