@@ -404,6 +404,10 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
               "weight");
     return kStatusInvalid;
   }
+  if (out_stride_t < out_features && num_tokens > 1) {
+    set_error("linear (4 bit): output rows overlap (stride %lld)", static_cast<long long>(out_stride_t));
+    return kStatusInvalid;
+  }
   if (!(scale > 0.f && scale <= 3.0e38f)) {
     set_error("linear (4 bit): the weight's tensor scale must be positive and finite");
     return kStatusInvalid;

@@ -41,13 +41,23 @@ def rope_theta(config) -> float:
 
 
 def check_latent_caches(caches: dict) -> dict:
-    """``{width: cache}`` of the latent caches (vLLM TRITON_ATTN layout ``[num_blocks, 1, block, 2 * width]``)
-    -> the runtime-check record the reference prints (ouro_latent.py:243-246).  Raises RuntimeError for a
+    """``{width: cache}`` of the latent caches (vLLM TRITON_ATTN layout ``[num_blocks, 1, block, 2 * width]``,
+    or the 4-bit one of ``q4.new_cache``, uint8 ``[num_blocks, 1, block, 17 * width / 16]``) -> the runtime-check record the reference prints (ouro_latent.py:243-246).  Raises RuntimeError for a
     layout the reference rejects (block not a multiple of 16, last dim != 2 * width) or the B200 kernels
     cannot read (width / block size outside their instantiations, non-bf16, misaligned rows)."""
     record = {}
     for w, c in caches.items():
         shape, stride = tuple(c.shape), tuple(c.stride())
+        if str(c.dtype) == 'torch.uint8':
+            row = 17 * w // 16
+            if len(shape) != 4 or shape[1] != 1 or shape[2] % 16 or shape[-1] != row:
+                raise RuntimeError(f'unexpected 4-bit latent cache geometry: {shape}')
+            if w not in KERNEL_WIDTHS:
+                raise RuntimeError(f'B200 4-bit history kernel has no instance for width {w}')
+            if stride[-1] != 1 or stride[2] != row or stride[0] % 16:
+                raise RuntimeError(f'B200 4-bit latent cache pages must be contiguous and 16-byte aligned: {stride}')
+            record[w] = [list(shape), list(stride), str(c.dtype)]
+            continue
         if len(shape) != 4 or shape[1] != 1 or shape[2] % 16 or shape[-1] != 2 * w:
             raise RuntimeError(f'unexpected latent cache geometry: {shape}')
         if w not in KERNEL_WIDTHS or shape[2] not in KERNEL_PAGES[w]:

@@ -13,6 +13,8 @@ import math
 import torch
 from torch import nn
 
+from . import q4
+
 ARCHITECTURE = 's6-block-v1'
 
 
@@ -29,8 +31,14 @@ class LatentLayer(nn.Module):
         self.out_absorb = nn.Parameter(torch.empty(loops - 1, heads, rank_v, head_dim))
         self.q_absorb1 = nn.Parameter(torch.empty(heads, head_dim, rank1))
         self.out_absorb1 = nn.Parameter(torch.empty(heads, rank1, head_dim))
+        self.packed_writers = None
         for p in (self.q_absorb, self.out_absorb, self.q_absorb1, self.out_absorb1):
             nn.init.normal_(p, std=1 / math.sqrt(hidden))
+
+    def pack_writers(self):
+        """From now on the writers run on 4-bit copies of their weights, made here (on CUDA, bf16).  The parameters
+        stay as they are, as does the state dict; a copy is not made again when they change."""
+        self.packed_writers = [q4.Weight.of(w.weight.detach()) for w in (self.cand1, *self.cand_s)]
 
     def readers(self, loop):
         """``(A, B, width)`` of a loop: loop 0 reads the loop-1 latent, later loops the main latent."""
@@ -39,7 +47,10 @@ class LatentLayer(nn.Module):
         return self.q_absorb[loop - 1], self.out_absorb[loop - 1], self.rank
 
     def writer(self, loop):
-        """The projection weight written at ``loop`` (E_1' at loop 0, E_{loop+1} after)."""
+        """The projection weight written at ``loop`` (E_1' at loop 0, E_{loop+1} after): bf16, or a ``q4.Weight``
+        after ``pack_writers``."""
+        if self.packed_writers is not None:
+            return self.packed_writers[loop]
         return self.cand1.weight if loop == 0 else self.cand_s[loop - 1].weight
 
 

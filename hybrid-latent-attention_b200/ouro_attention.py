@@ -8,8 +8,9 @@ and metadata through its forward context (``get_attention_context``); here the c
 ``PagedCaches`` record, so the same per-layer sequence runs in tests over a simulated paged cache, and in
 any host that owns its KV memory.
 
-Per (layer, loop) the launches are this package's kernels except the two dense projections (cuBLAS via
-torch, as vLLM's ``QKVParallelLinear`` / ``RowParallelLinear``):
+Per (layer, loop) the launches are this package's kernels except the two dense projections with bf16 weights
+(cuBLAS via torch, as vLLM's ``QKVParallelLinear`` / ``RowParallelLinear``; with ``q4.Weight``s they are
+``hla_s6_linear_q4``, and latent caches in the 4-bit format take its commit and its history split):
 
   writer            s6_layer.write_rows                         (ouro_latent.py:108)
   qkv               F.linear                                    (:109-110)
@@ -33,7 +34,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import _lib, s6_layer
+from . import _lib, q4, s6_layer
 
 
 @dataclass
@@ -44,18 +45,29 @@ class PagedCaches:
     (one cache group geometry, as the reference's serving test uses); ``exact[t]`` is loop t's exact
     cache in vLLM's TRITON_ATTN physical layout ``[nb, page, H, 2 * head_dim]`` with ``exact_table``
     (a sliding window of W + 1 rows needs only the pages it touches).  ``exact`` may be empty when the
-    model has no window (W = 0)."""
+    model has no window (W = 0).
+
+    ``main`` and ``l1`` may each be a 4-bit cache (``q4.new_cache``, uint8) instead of a bf16 one;
+    ``main_scale`` and ``l1_scale`` are then its tensor scales ``(k, v)``."""
     main: torch.Tensor
     l1: torch.Tensor
     latent_table: torch.Tensor
     exact: list
     exact_table: torch.Tensor | None
+    main_scale: tuple = (1.0, 1.0)
+    l1_scale: tuple = (1.0, 1.0)
+
+
+def _project(x, weight):
+    """``x . weight^T`` with a bf16 weight or a packed one (``q4.Weight``)."""
+    return weight.linear(x) if isinstance(weight, q4.Weight) else F.linear(x, weight)
 
 
 class LatentAttention:
     """The S6 attention of one Ouro layer: frozen ``qkv_weight [3 H d, hidden]`` / ``o_weight [hidden, H d]``,
     the layer's ``LatentLayer`` student, the exact RoPE table ``cos_sin [max_position, d]`` (``[cos | sin]``
-    fp32, neox pairs ``(i, i + d/2)``) and the window W."""
+    fp32, neox pairs ``(i, i + d/2)``) and the window W.  ``qkv_weight`` and ``o_weight`` may each be a
+    ``q4.Weight``, the student's writers too (``LatentLayer.pack_writers``)."""
 
     def __init__(self, latent, qkv_weight, o_weight, cos_sin, window):
         self.latent, self.qkv_weight, self.o_weight = latent, qkv_weight, o_weight
@@ -69,9 +81,9 @@ class LatentAttention:
         T, sl = hidden_states.shape[0], self.latent
         H, d = self.heads, self.head_dim
         state = s6_layer.write_rows(sl, current_ut, hidden_states, state)
-        qkv = F.linear(hidden_states, self.qkv_weight)
+        qkv = _project(hidden_states, self.qkv_weight)
         q, k, v = (x.view(T, H, d) for x in qkv.split(H * d, -1))
-        cache = caches.l1 if current_ut == 0 else caches.main
+        cache, scales = (caches.l1, caches.l1_scale) if current_ut == 0 else (caches.main, caches.main_scale)
         md = ctx.md_present
         if self.window and md and ctx.max_query_len == 1:
             # decode batch: latent query, exact RoPE and exact-cache append in one launch, and the history
@@ -83,13 +95,13 @@ class LatentAttention:
             q_lat, q_rope = self._prepare(current_ut, q, k, v, positions, cache_e, caches.exact_table, ctx)
             ctx.history_after_query = True
             try:
-                out = s6_layer.attend(sl, current_ut, q_lat, q_rope, None, v, cache, caches.latent_table, None,
-                                      None, ctx, (cache_e, caches.exact_table))
+                out = s6_layer.attend(sl, current_ut, q_lat, q_rope, None, v, cache, caches.latent_table,
+                                      *scales, ctx, (cache_e, caches.exact_table))
             finally:
                 ctx.history_after_query = False
             if current_ut == 0 or current_ut == sl.loops - 1:
-                self._commit(current_ut, state, positions, cache, caches.latent_table, ctx)
-            output = F.linear(out.reshape(T, H * d), self.o_weight)
+                self._commit(current_ut, state, positions, cache, caches.latent_table, ctx, scales)
+            output = _project(out.reshape(T, H * d), self.o_weight)
             return (output, state, out) if return_attention else (output, state)
         q_lat = ctx.latent_query(sl, current_ut, q)            # before the in-place exact RoPE
         k_rope = torch.empty(T, H, d, dtype=k.dtype, device=k.device)
@@ -101,10 +113,10 @@ class LatentAttention:
         else:
             self._exact_append(q, k, v, k_rope, positions, None, None, ctx)
         out = s6_layer.attend(sl, current_ut, q_lat, q, k_rope, v, cache if md else None,
-                              caches.latent_table if md else None, None, None, ctx, window)
+                              caches.latent_table if md else None, *scales, ctx, window)
         if md and (current_ut == 0 or current_ut == sl.loops - 1):
-            self._commit(current_ut, state, positions, cache, caches.latent_table, ctx)
-        output = F.linear(out.reshape(T, H * d), self.o_weight)
+            self._commit(current_ut, state, positions, cache, caches.latent_table, ctx, scales)
+        output = _project(out.reshape(T, H * d), self.o_weight)
         return (output, state, out) if return_attention else (output, state)
 
     def _prepare(self, loop, q, k, v, positions, cache, table, ctx):
@@ -148,15 +160,19 @@ class LatentAttention:
                   _lib.ptr(cache), nb, sb, sh, sr, page, _lib.ptr(table), bt_stride, max_blocks, _lib.ptr(qsl),
                   qsl.shape[0] - 1, T, H, d, None, _lib.stream_of(q))
 
-    def _commit(self, loop, state, positions, cache, table, ctx):
+    def _commit(self, loop, state, positions, cache, table, ctx, scales=(1.0, 1.0)):
         """The committed latent row of ``loop`` (loop-1 row at loop 0, main row at the last loop): K half
         latent-RoPE'd in the torch bf16 order of LatentLayer.pack and the row stored at the token's slot -
-        committed_row + unified_kv_cache_update in one launch."""
+        committed_row + unified_kv_cache_update in one launch.  A 4-bit cache takes the row quantised
+        (``q4.commit_rows``)."""
         sl = self.latent
         row, width = (state.first, sl.rank1) if loop == 0 else (state.reg, sl.rank)
         tab = ctx.tables[width]
         pos = positions if positions.dtype == torch.int64 else positions.long()
         qsl = ctx.query_start_loc
+        if cache.dtype == torch.uint8:
+            q4.commit_rows(row, pos, tab, cache, table, qsl, *scales)
+            return
         _lib.call('hla_s6_commit_rows', _lib.ptr(row), row.stride(0), width, _lib.ptr(pos), _lib.ptr(tab),
                   tab.stride(0), tab.shape[0], _lib.ptr(cache), cache.shape[0], cache.stride(0), cache.stride(2),
                   cache.shape[2], _lib.ptr(table), table.stride(0), table.shape[1], _lib.ptr(qsl), qsl.shape[0] - 1,

@@ -10,7 +10,8 @@ column instead of 4 (544 bytes for a 512-wide latent, bf16 2048), weights of 17/
                          cache, ``s6_layer.attend`` and ``ouro_attention`` take such caches too
 * ``gather_rows`` / ``gather_slots``  rows back as bf16 (the export's gather, cache_export.py:160-174)
 * ``quantize_weight`` / ``linear``    packed weights, and ``x . w^T`` with them (register.py:45-61,
-                         ouro_latent.py:109-110, 130)
+                         ouro_latent.py:109-110, 130); ``Weight`` holds one for ``ouro_attention`` and
+                         ``LatentLayer.pack_writers``
 
 Format: a group of 32 consecutive columns shares one e4m3 scale ``s``; a value is ``(n - 8) * s * ts`` with a
 code ``n`` in 1..15 and one tensor scale ``ts``: ``s = e4m3(amax / (7 ts))``, ``n = 8 + rint(x / (s ts))``.  The
@@ -24,6 +25,7 @@ synchronise and can be captured in CUDA graphs.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 
 import torch
 
@@ -249,3 +251,21 @@ def linear(x, packed, out_features, scale, residual=None, out=None):
     _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x.stride(0), packed.data_ptr(), T, N, K, scale,
             _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0))
     return out
+
+
+@dataclass(frozen=True)
+class Weight:
+    """A packed weight with what its calls need: the weights of ``ouro_attention.LatentAttention`` and of
+    ``latent.LatentLayer``'s writers may be of this kind."""
+    packed: torch.Tensor
+    out_features: int
+    scale: float
+
+    @classmethod
+    def of(cls, weight, scale=None):
+        """The 4-bit copy of a bf16 weight ``[N, K]`` (``quantize_weight``)."""
+        packed, scale = quantize_weight(weight, scale)
+        return cls(packed, weight.shape[0], scale)
+
+    def linear(self, x, residual=None, out=None):
+        return linear(x, self.packed, self.out_features, self.scale, residual, out)

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, s6_ops
+from . import _lib, q4, s6_ops
 
 
 def latent_inv_freq(head_dim, theta):
@@ -99,6 +99,9 @@ def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_sc
     then one fused combine (split reduce, B up-projection, window over the exact cache incl. the
     current token, merge).  Other steps: causal chunk attention, merged with the window history when
     there is a window, then history split + combine taking that exact part.
+
+    A uint8 ``cache`` is a 4-bit one (``q4``) with the tensor scales ``k_scale`` / ``v_scale`` (None: 1);
+    a bf16 cache has none.
     """
     s6_ops._require(ctx.backends.history, 'history')
     T, H, d = q_rope.shape
@@ -120,16 +123,27 @@ def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_sc
     use_history = cache is not None and ctx.md_present and ctx.history_needed
     ws_ptr, ws_floats, splits, lpage = None, 0, ctx.num_kv_splits, 16
     if use_history:
-        nb, lpage, sb, sr = s6_ops._latent_cache_geometry(cache, width)
+        four_bit = cache.dtype == torch.uint8
+        if four_bit:
+            nb, sb, lpage = q4._cache_geometry(cache, width)
+        else:
+            nb, lpage, sb, sr = s6_ops._latent_cache_geometry(cache, width)
         ws = ctx.workspace.attn_logits(T, H, splits, width, q_lat.device)
         ws_ptr, ws_floats = ctx.workspace.buffer, ws.numel()
         bt = ctx.block_table(block_table)
         # a caller whose last launch wrote q_lat (ouro_attention's fused prepare) sets history_after_query:
         # the split then streams pages while that launch runs
         after_query = _lib.PARTIALS_AFTER_QUERY if getattr(ctx, 'history_after_query', False) else 0
-        _lib.call('hla_s6_history_partials', _lib.ptr(q_lat), q_lat.stride(0), q_lat.stride(1), _lib.ptr(cache), nb,
-                  sb, sr, _lib.ptr(bt), bt.stride(0), bt.shape[1], _lib.ptr(ctx.ctx_latent), T, H, width, lpage,
-                  float(ctx.scale), int(splits), _lib.ptr(ws_ptr), ws_floats, None, after_query, stream)
+        if four_bit:
+            _lib.call('hla_s6_history_partials_q4', _lib.ptr(q_lat), q_lat.stride(0), q_lat.stride(1), _lib.ptr(cache),
+                      nb, sb, _lib.ptr(bt), bt.stride(0), bt.shape[1], _lib.ptr(ctx.ctx_latent), T, H, width, lpage,
+                      float(ctx.scale), int(splits), _lib.ptr(ws_ptr), ws_floats,
+                      1.0 if k_scale is None else float(k_scale), 1.0 if v_scale is None else float(v_scale), None,
+                      after_query, stream)
+        else:
+            _lib.call('hla_s6_history_partials', _lib.ptr(q_lat), q_lat.stride(0), q_lat.stride(1), _lib.ptr(cache),
+                      nb, sb, sr, _lib.ptr(bt), bt.stride(0), bt.shape[1], _lib.ptr(ctx.ctx_latent), T, H, width,
+                      lpage, float(ctx.scale), int(splits), _lib.ptr(ws_ptr), ws_floats, None, after_query, stream)
         z_in = lse_in = None
         empty = ctx.empty_latent
     else:
@@ -162,12 +176,16 @@ class WriterState:
 
 def write_rows(sl, loop, h, state=None):
     """Writer accumulation on the attention input ``h[T, hidden]`` (reference s6_layer.py:124-132):
-    loop 0 gives ``first = E_1' h``; later loops ``reg = reg + E_t h`` with a bf16 add."""
+    loop 0 gives ``first = E_1' h``; later loops ``reg = reg + E_t h`` with a bf16 add.  A packed writer
+    (``LatentLayer.pack_writers``) runs as ``q4.linear``, which rounds the sum once."""
     weight = sl.writer(loop) if hasattr(sl, 'writer') else (sl.cand1.weight if loop == 0 else sl.cand_s[loop - 1].weight)
+    reg_in = None if loop == 0 or state is None else state.reg
+    if isinstance(weight, q4.Weight):
+        out = weight.linear(h, reg_in)
+        return WriterState(None, out) if loop == 0 else WriterState(out, None)
     T, K = h.shape
     N = weight.shape[0]
     out = torch.empty(T, N, dtype=h.dtype, device=h.device)
-    reg_in = None if loop == 0 or state is None else state.reg
     _lib.call('hla_s6_writer_project', _lib.ptr(h), h.stride(0), _lib.ptr(weight), weight.stride(0),
               _lib.ptr(reg_in), 0 if reg_in is None else reg_in.stride(0), _lib.ptr(out), out.stride(0), T, N, K,
               _lib.stream_of(h))

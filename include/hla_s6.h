@@ -460,7 +460,7 @@ int hla_s6_history_partials_q4(const void* q_lat, int64_t q_stride_t, int64_t q_
 /* hla_s6_commit_rows into a 4-bit cache: the K half latent-RoPE'd in the torch bf16 order, then both halves
  * quantised.  Padding tokens and tokens without a slot in the cache are skipped (slot_out -1).  Infinite
  * values take their group's largest code.  Two tokens of one call must not share a slot.  row and table rows
- * 16-byte aligned. */
+ * 16-byte aligned, max_blocks * page < 2^31. */
 int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, const int64_t* positions,
                           const void* table, int64_t table_stride, int64_t max_position, void* cache,
                           int64_t num_blocks, int64_t cache_stride_block, int32_t page, const int32_t* block_table,
@@ -471,7 +471,7 @@ int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, 
 /* Rows of a 4-bit cache as bf16 [num_rows, 2 * width] (K | V, row stride out_stride elements, 16-byte aligned
  * rows): row i is row i % page of block blocks[i / page] (blocks int32, ceil(num_rows / page) entries), or -
  * with slots (int64 [num_rows]) instead - cache row slots[i] (block * page + offset; negative: zeros).  A block
- * outside the cache gives zeros and sets error_flag (5).  The rows hla_s6_export_rows gathers from a bf16
+ * outside the cache gives zeros and sets error_flag (5).  Fewer than 2^31 rows.  The rows hla_s6_export_rows gathers from a bf16
  * cache (hla/vllm_latent/cache_export.py:160-174). */
 int hla_s6_gather_rows_q4(const void* cache, int64_t num_blocks, int64_t cache_stride_block, int32_t width,
                           int32_t page, const int32_t* blocks, const int64_t* slots, int64_t num_rows, float k_scale,
