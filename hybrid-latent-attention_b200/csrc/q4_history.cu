@@ -55,7 +55,7 @@ struct Q4HistoryParams {
   float* ws_o;
   float* ws_lse;
   int2* meta;
-  int32_t slots_cap, parts, stream_mode;  // parts: CTAs of the page partition (stream mode)
+  int32_t slots_cap, parts, stream_mode;  // parts: CTAs of the partition (stream mode)
   uint32_t sixteen;  // 16 (q4_word_h)
   int* err;
   uint64_t wait_ns;
@@ -132,10 +132,18 @@ __device__ __forceinline__ bool named_bar_or(int id, int threads, bool pred) {
   return r != 0;
 }
 
+// The partition over the CTAs (stream mode) counts half steps: a row costs 2 a step of 128 rows and 1 for what its
+// segment takes to begin and end, and is only cut between steps (a cut one costs its CTAs a step each).  Cut at pages
+// and without that 1, short rows piled up in a CTA, up to 5 segments and 8 steps where 5 were due (37 rows of 0 to
+// 16384, width 256: 31 -> 25 us; 64 rows of 8160, width 512: 104 -> 97).
+__device__ __forceinline__ int q4_cost(int ctx) { return ctx > 0 ? 2 * ((ctx - 1) / 128 + 1) + 1 : 0; }
+// The step at cost x of a row: a CTA that starts there begins with it, one that ends there ends before it.
+__device__ __forceinline__ int q4_step_at(int x) { return x > 0 ? (x - 1) >> 1 : 0; }
+
 // The steps of a CTA: up to 8 consecutive tiles of one row's segment.  Every role walks them by itself.
 struct Q4Walk {
   const Q4HistoryParams& p;
-  const int* pref;  // page prefix (stream mode)
+  const int* pref;  // prefix of the rows' costs (stream mode)
   int r, pg, p1, tile, tend, n, ctx, slot;
   bool first, last;
   __device__ Q4Walk(const Q4HistoryParams& p_, const int* pref_, int r0, int p0, int p1_)
@@ -145,14 +153,16 @@ struct Q4Walk {
     first = tile >= tend;
     if (first) {
       if (p.stream_mode) {
-        if (pg >= p1) return false;
-        while (pg >= pref[r + 1]) ++r;
-        const int base = pref[r], end = min(p1, pref[r + 1]);
-        ctx = p.ctx[r];
-        tile = (pg - base) * p.tpp;
-        tend = min((end - base) * p.tpp, (ctx + 15) >> 4);
-        pg = end;
-        slot = blockIdx.x + r;
+        do {
+          if (pg >= p1) return false;
+          while (pg >= pref[r + 1]) ++r;
+          const int base = pref[r], end = min(p1, pref[r + 1]);
+          ctx = p.ctx[r];
+          tile = 8 * q4_step_at(pg - base);
+          tend = min(8 * q4_step_at(end - base), (ctx + 15) >> 4);
+          pg = end;
+          slot = blockIdx.x + r;
+        } while (tile >= tend);  // the range ends before the row's next step
       } else {
         for (r = pg; r < p.T; r += gridDim.x) {
           ctx = p.ctx[r];
@@ -203,8 +213,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   int r0 = 0, p0 = 0, p1 = 0;
   int P = 0, G = 1;
   if (p.stream_mode) {
-    const int page = 16 * p.tpp;
-    for (int t = tid; t < p.T; t += blockDim.x) pref[t + 1] = (max(p.ctx[t], 0) + page - 1) / page;
+    for (int t = tid; t < p.T; t += blockDim.x) pref[t + 1] = q4_cost(p.ctx[t]);
     if (tid == 0) pref[0] = 0;
     __syncthreads();
     if (warp == 0) {
@@ -222,8 +231,8 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     }
     __syncthreads();
     P = pref[p.T];
-    G = min(p.parts, P);
-    if (static_cast<int>(blockIdx.x) >= G) {
+    G = min(p.parts, max(P / 2, 1));  // ranges of 2 or more: a CTA between the first and the last of a row has a step
+    if (P == 0 || static_cast<int>(blockIdx.x) >= G) {
       if (blockIdx.x == 0) {  // no rows at all: every slot range is empty
         griddep_wait();
         for (int t = tid; t < p.T; t += blockDim.x) p.meta[t] = make_int2(0, 0);
@@ -232,7 +241,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     }
     p0 = static_cast<int>(stream_start(blockIdx.x, P, G));
     p1 = static_cast<int>(stream_start(blockIdx.x + 1, P, G));
-    int lo = 0, hi = p.T;  // the row holding page p0
+    int lo = 0, hi = p.T;  // the row that p0 is in
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pref[mid] <= p0) lo = mid; else hi = mid;
@@ -442,7 +451,8 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     if (p.stream_mode && blockIdx.x == 0) {
       for (int t = tid - 512; t < p.T; t += 256) {
         const int a = pref[t], b = pref[t + 1];
-        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a, P, G)) + t,
+        // the CTAs of the row's first and last step (its step s ends at cost 2 s + 2)
+        p.meta[t] = b > a ? make_int2(static_cast<int>(stream_owner(a + 2, P, G)) + t,
                                       static_cast<int>(stream_owner(b - 1, P, G)) + t + 1)
                           : make_int2(0, 0);
       }
