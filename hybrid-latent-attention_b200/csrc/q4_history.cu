@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   using C = Q4Cfg<W>;
   constexpr int NB = C::NB, UT = C::UT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // (an offset, not a rounded pointer: the compiler then knows that these are shared-memory addresses)
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   uint8_t* qs = smem;
   uint8_t* ps = qs + C::Q_BYTES;
   uint8_t* units = ps + C::P_BYTES;

@@ -200,7 +200,8 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
   using C = Q4Many<BN>;
   constexpr int DQ = C::DQ;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // (an offset, not a rounded pointer: the compiler then knows that these are shared-memory addresses)
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);  // x copied and weights written
   uint64_t* empty = full + C::STAGES;
   uint64_t* done = empty + C::STAGES;

@@ -33,7 +33,7 @@ from . import _lib
 
 GROUP = 32
 WEIGHT_TILE_BYTES = 1088   # HLA_S6_Q4_WEIGHT_TILE_BYTES
-BF16 = torch.bfloat16
+BF16, U8, I32, I64 = torch.bfloat16, torch.uint8, torch.int32, torch.int64
 
 
 def row_bytes(width):
@@ -56,7 +56,7 @@ def new_cache(num_blocks, page, width, device='cuda'):
     """A zeroed 4-bit latent cache (every row reads as zeros)."""
     if width not in (256, 512, 1024) or page < 16 or page % 16:
         raise ValueError('a 4-bit latent cache has width 256, 512 or 1024 and a page of a multiple of 16 rows')
-    return torch.zeros(num_blocks, 1, page, row_bytes(width), dtype=torch.uint8, device=device)
+    return torch.zeros(num_blocks, 1, page, row_bytes(width), dtype=U8, device=device)
 
 
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
@@ -73,11 +73,16 @@ def _device_of(first, *rest):
     return index
 
 
+_entries = {}   # the library's functions by name, looked up once
+
+
 def _launch(index, name, *args):
     """Entry point ``name`` with ``args`` and the current stream of device ``index``, which is made current for the
-    launch.  (Plain ints and the raw stream handle: the calls of one token's step cost more on the host than on the
-    device.)"""
-    fn = getattr(_lib.load(), name)
+    launch.  (Plain ints and the raw stream handle, and outputs by the quickest of torch's constructors: the calls of
+    one token's step cost more on the host than on the device.)"""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
     if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
@@ -94,7 +99,7 @@ def _address(t):
 def _cache_geometry(cache, width):
     """``(num_blocks, block stride in bytes, page)`` of a 4-bit cache of latent width ``width``."""
     shape, bytes_ = cache.shape, 17 * width // 16
-    if len(shape) != 4 or shape[1] != 1 or shape[3] != bytes_ or cache.dtype != torch.uint8:
+    if len(shape) != 4 or shape[1] != 1 or shape[3] != bytes_ or cache.dtype is not U8:
         raise ValueError(f'a 4-bit latent cache of width {width} must be uint8 [num_blocks, 1, page, {bytes_}], got '
                          f'{cache.dtype} {tuple(shape)}')
     stride = cache.stride()
@@ -106,7 +111,7 @@ def _cache_geometry(cache, width):
 def _block_table(table):
     """``(row stride, rows, columns)`` of a block table."""
     shape, stride = table.shape, table.stride()
-    if table.dtype != torch.int32 or len(shape) != 2 or stride[1] != 1:
+    if table.dtype is not I32 or len(shape) != 2 or stride[1] != 1:
         raise ValueError('block_table must be int32 [rows, max_blocks] with a unit last-dim stride')
     return stride[0], shape[0], shape[1]
 
@@ -116,12 +121,13 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
     """``s6_ops.history_attention`` over a 4-bit cache: ``(o [T, H, W] bf16, lse [H, T] fp32)`` of the softmax of
     ``q_lat [T, H, W]`` over the first ``ctx[t]`` rows; empty rows give ``o = 0``, ``lse = -inf``.
     ``error_flag`` (int32 [1], optional) receives 5 for a block-table entry outside the cache."""
-    if q_lat.dim() != 3 or q_lat.dtype != BF16 or q_lat.stride(2) != 1:
+    stride = q_lat.stride()
+    if len(stride) != 3 or q_lat.dtype is not BF16 or stride[2] != 1:
         raise ValueError('q_lat must be bf16 [T, H, W] with a unit last-dim stride')
     T, H, W = q_lat.shape
     nb, sb, page = _cache_geometry(cache, W)
     bt_stride, bt_rows, bt_cols = _block_table(block_table)
-    if ctx.dtype != torch.int32 or ctx.shape != (T,) or bt_rows < T:
+    if ctx.dtype is not I32 or ctx.shape != (T,) or bt_rows < T:
         raise ValueError('ctx must be int32 [T] and block_table hold a row per token')
     if empty is not None:
         if empty.shape != (T,):
@@ -132,13 +138,13 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
     need = T * H * num_kv_splits * (W + 1)
     if need > buffer.numel():
         raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {buffer.numel()}')
-    o = q_lat.new_empty((T, H, W))
-    lse = q_lat.new_empty((H, T), dtype=torch.float32)
+    o = q_lat.new_empty(T, H, W)
+    lse = buffer.new_empty(H, T)
     ctx = ctx.contiguous()
-    _launch(index, 'hla_s6_history_attention_q4', q_lat.data_ptr(), q_lat.stride(0), q_lat.stride(1), cache.data_ptr(),
-            nb, sb, block_table.data_ptr(), bt_stride, bt_cols, ctx.data_ptr(),
-            _address(empty), T, H, W, page, scale, num_kv_splits, buffer.data_ptr(), need, k_scale, v_scale,
-            o.data_ptr(), H * W, W, lse.data_ptr(), _address(error_flag))
+    _launch(index, 'hla_s6_history_attention_q4', q_lat.data_ptr(), stride[0], stride[1], cache.data_ptr(), nb,
+            sb, block_table.data_ptr(), bt_stride, bt_cols, ctx.data_ptr(), _address(empty), T, H, W, page, scale,
+            num_kv_splits, buffer.data_ptr(), need, k_scale, v_scale, o.data_ptr(), H * W, W, lse.data_ptr(),
+            _address(error_flag))
     return o, lse
 
 
@@ -147,42 +153,44 @@ def commit_rows(row, positions, table, cache, block_table, query_start_loc, k_sc
     ``positions [T]`` (int64), both halves quantised and stored at ``block_table[request, pos // page] * page +
     pos % page``.  Returns the slots (int64 [T]); padding tokens (``t >= query_start_loc[-1]``) and positions
     without a block in the cache are skipped, their slot is -1.  Two tokens of one call must not share a slot."""
-    if row.dim() != 2 or row.dtype != BF16 or row.stride(1) != 1:
+    stride = row.stride()
+    if len(stride) != 2 or row.dtype is not BF16 or stride[1] != 1:
         raise ValueError('row must be bf16 [T, 2 * width] with a unit last-dim stride')
     T, W = row.shape
     W //= 2
     nb, sb, page = _cache_geometry(cache, W)
-    if table.dim() != 2 or table.dtype != BF16 or table.stride(1) != 1 or table.shape[1] != W:
+    tab_rows, tab_stride = table.shape, table.stride()
+    if len(tab_stride) != 2 or table.dtype is not BF16 or tab_stride[1] != 1 or tab_rows[1] != W:
         raise ValueError(f'table must be bf16 [max_position, {W}] = [cos | sin]')
     bt_stride, bt_rows, bt_cols = _block_table(block_table)
     requests = query_start_loc.numel() - 1
-    if (positions.dtype != torch.int64 or positions.shape != (T,) or query_start_loc.dtype != torch.int32
+    if (positions.dtype is not I64 or positions.shape != (T,) or query_start_loc.dtype is not I32
             or query_start_loc.dim() != 1 or bt_rows < requests):
         raise ValueError('positions must be int64 [T], query_start_loc int32 [R + 1], block_table [R, max_blocks]')
     index = _device_of(row, positions, table, cache, block_table, query_start_loc)
     positions, query_start_loc = positions.contiguous(), query_start_loc.contiguous()
-    slots = positions.new_empty((T,))
-    _launch(index, 'hla_s6_commit_rows_q4', row.data_ptr(), row.stride(0), W, positions.data_ptr(), table.data_ptr(),
-            table.stride(0), table.shape[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
+    slots = positions.new_empty(T)
+    _launch(index, 'hla_s6_commit_rows_q4', row.data_ptr(), stride[0], W, positions.data_ptr(), table.data_ptr(),
+            tab_stride[0], tab_rows[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
             bt_stride, bt_cols, query_start_loc.data_ptr(), requests, T, k_scale, v_scale,
             slots.data_ptr())
     return slots
 
 
 def _gather(cache, blocks, slots, rows, k_scale, v_scale, out, error_flag):
-    W = cache_width(cache)
+    W = cache.shape[-1] * 16 // 17
     nb, sb, page = _cache_geometry(cache, W)
     index = blocks if slots is None else slots
-    if index.dim() != 1 or index.dtype != (torch.int32 if slots is None else torch.int64):
+    if index.dim() != 1 or index.dtype is not (I32 if slots is None else I64):
         raise ValueError('blocks must be int32 [n], slots int64 [n]')
     if rows < 0 or (slots is None and -(-rows // page) > blocks.shape[0]):
         raise IndexError('the block list does not cover the rows')
-    if out is not None and (out.shape != (rows, 2 * W) or out.dtype != BF16 or out.stride(-1) != 1):
+    if out is not None and (out.shape != (rows, 2 * W) or out.dtype is not BF16 or out.stride(-1) != 1):
         raise ValueError(f'out must be bf16 [{rows}, {2 * W}] with a unit last-dim stride')
     device = _device_of(cache, index, out, error_flag)
     index = index.contiguous()
     if out is None:
-        out = cache.new_empty((rows, 2 * W), dtype=BF16)
+        out = torch.empty_strided((rows, 2 * W), (2 * W, 1), dtype=BF16, device=cache.device)
     if rows:
         at = index.data_ptr()
         _launch(device, 'hla_s6_gather_rows_q4', cache.data_ptr(), nb, sb, W, page, at if slots is None else None,
@@ -210,7 +218,7 @@ def weight_tiles(out_features, in_features):
 def quantize_weight(weight, scale=None):
     """``(packed, scale)`` of a bf16 weight ``[N, K]``, K a multiple of 32.  ``scale`` defaults to
     ``tensor_scale`` of its largest value (which reads it back: call this once, at load time)."""
-    if weight.dim() != 2 or weight.dtype != BF16 or weight.stride(-1) != 1:
+    if weight.dim() != 2 or weight.dtype is not BF16 or weight.stride(-1) != 1:
         raise ValueError('weight must be bf16 [N, K] with a unit last-dim stride')
     N, K = weight.shape
     if K < GROUP or K % GROUP or N < 1:
@@ -218,38 +226,42 @@ def quantize_weight(weight, scale=None):
     index = _device_of(weight)
     if scale is None:
         scale = tensor_scale(float(weight.abs().amax()))
-    packed = weight.new_empty(weight_tiles(N, K), dtype=torch.uint8)
+    packed = weight.new_empty(weight_tiles(N, K), dtype=U8)
     _launch(index, 'hla_s6_quantize_weight_q4', weight.data_ptr(), weight.stride(0), N, K, scale, packed.data_ptr())
     return packed, float(scale)
 
 
 def _check_rows(y, T, N):
-    if y.shape != (T, N) or y.dtype != BF16 or y.stride(1) != 1:
+    if y.shape != (T, N) or y.dtype is not BF16 or y.stride(1) != 1:
         raise ValueError(f'residual and out must be bf16 [{T}, {N}] with a unit last-dim stride')
 
 
 def linear(x, packed, out_features, scale, residual=None, out=None):
     """``bf16(scale * x . w^T + residual)`` for ``x [T, K]`` bf16 and the packed weight ``[N, K]``: fp32 sums, one
     rounding.  ``residual`` and ``out`` are bf16 ``[T, N]``; ``out`` may be ``residual``."""
-    if x.dim() != 2 or x.dtype != BF16 or x.stride(-1) != 1:
+    stride = x.stride()
+    if len(stride) != 2 or x.dtype is not BF16 or stride[1] != 1:
         raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
     T, K = x.shape
     N = out_features
-    if (packed.dtype != torch.uint8 or packed.shape != (-(-N // 16), -(-K // 128), WEIGHT_TILE_BYTES)
+    if (packed.dtype is not U8 or packed.shape != (-(-N // 16), -(-K // 128), WEIGHT_TILE_BYTES)
             or not packed.is_contiguous()):
         raise ValueError(f'packed must be contiguous uint8 {list(weight_tiles(N, K))}, got {packed.dtype} '
                          f'{list(packed.shape)}')
-    if x.stride(0) < K and T > 1:
-        x = x.contiguous()   # rows that overlap (an expanded x)
+    x_stride = stride[0]
+    if x_stride < K and T > 1:   # rows that overlap (an expanded x)
+        x, x_stride = x.contiguous(), K
     if residual is not None:
         _check_rows(residual, T, N)
     if out is not None:
         _check_rows(out, T, N)
     index = _device_of(x, packed, residual, out)
-    if out is None:
-        out = x.new_empty((T, N))
-    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x.stride(0), packed.data_ptr(), T, N, K, scale,
-            _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0))
+    fresh = out is None
+    if fresh:
+        out = x.new_empty(T, N)
+    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x_stride, packed.data_ptr(), T, N, K, scale,
+            _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(),
+            N if fresh else out.stride(0))
     return out
 
 

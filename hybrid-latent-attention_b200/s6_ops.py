@@ -158,10 +158,10 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
     signature compatibility.
     """
     _require(backend, 'history')
-    _check_cuda(q_lat, cache, block_table, ctx)
-    if cache.dtype == torch.uint8:
+    if cache.dtype is torch.uint8:
         return q4.history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace,
                                     1.0 if k_scale is None else k_scale, 1.0 if v_scale is None else v_scale, empty)
+    _check_cuda(q_lat, cache, block_table, ctx)
     if q_lat.dim() != 3 or q_lat.stride(-1) != 1:
         raise ValueError('q_lat must be [T, H, W] with a unit last-dim stride')
     if q_lat.dtype != torch.bfloat16:
