@@ -665,35 +665,39 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     // ------------------------------------------------------------------ tile copies
     // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
     const uint64_t policy = l2_policy_evict_first();
+    // The lanes look up 32 tiles at once: a lookup per unit, when its slot was free, kept this warp busy for longer
+    // than the others took to use the unit up (64 x 8160 rows: 95 -> XX us).
     int unit = 0;
     while (st.next()) {
-      for (int t0 = 0; t0 < st.n; t0 += UT, ++unit) {
-        const int ring = unit % C::UNITS, n = min(UT, st.n - t0);
-        const int t = st.tile + t0 + lane;
-        const int lp = t / p.tpp;
+      for (int b = st.tile; b < st.tend; b += 32) {
+        const int t = b + lane, lp = t / p.tpp;
         int blk = -1;
-        if (lane < n) {
+        if (t < st.tend) {
           if (lp < p.max_blocks) blk = p.bt[static_cast<int64_t>(st.r) * p.bt_st + lp];
           if (blk < 0 || blk >= p.num_blocks) {
             record_error(p.err, kErrBlock);
             blk = -1;
           }
         }
-        if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
-        __syncwarp();
-        uint8_t* dst = units + ring * C::UNIT + lane * C::TILE;
-        const unsigned absent = __ballot_sync(0xffffffffu, lane < n && blk < 0);
-        if (lane < n && blk < 0) {  // a page outside the table or the cache reads as zeros
-          for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async();
+        const uint8_t* src = p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE;
+        const unsigned absent = __ballot_sync(0xffffffffu, t < st.tend && blk < 0);
+        for (int k = 0; k < 32 && b + k < st.tend; k += UT, ++unit) {
+          const int ring = unit % C::UNITS, n = min(UT, st.tend - b - k);
+          const bool mine = lane >= k && lane < k + n;
+          if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
+          __syncwarp();
+          uint8_t* dst = units + ring * C::UNIT + (lane - k) * C::TILE;
+          if (mine && blk < 0) {  // a page outside the table or the cache reads as zeros
+            for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc((absent >> k) & ((1u << n) - 1u))) * C::TILE);
+          __syncwarp();
+          if (mine && blk >= 0) tc::bulk_load(dst, src, C::TILE, &full[ring], policy);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc(absent)) * C::TILE);
-        __syncwarp();
-        if (lane < n && blk >= 0)
-          tc::bulk_load(dst, p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE,
-                        C::TILE, &full[ring], policy);
       }
+      st.n = st.tend - st.tile;  // the segment's steps are all taken
     }
     // after an abort no role may have waited for the last copies: they must land before the CTA ends
     if (wait.aborted() && lane == 0)
