@@ -1,13 +1,21 @@
 // Linear layer with 4-bit weights (format: q4.cuh): y[t, n] = ts sum_k x[t, k] w[n, k] (+ residual[t, n]),
-// fp32 accumulation, one rounding to bf16.  Two kernels, by the number of tokens:
+// fp32 accumulation, one rounding to bf16.  Three kernels, by the number of tokens and tiles:
 //
 // q4_linear_few: the weight tile is the A operand of mma.m16n8k16 (16 output features), the tokens are N = 8, so one
 // token costs no more tensor work than eight.  What bounds it is the stream of weight bytes; codes go from global
 // memory to registers in 16-byte loads and are dequantised there (exact).
 //
-// q4_linear_many: tokens are the M = 128 rows of tcgen05.mma, x comes by TMA, and eight warps dequantise the weight
-// block of the stage into shared memory in the operand's swizzled layout, one 16-byte load of codes per thread and 16
-// rows, three stages ahead.  One launch and no workspace; the weight is dequantised once per 128 tokens.
+// q4_linear_many: tokens are the M = 128 rows of tcgen05.mma, 64 output features its N; x comes by TMA, and four warps
+// dequantise the stage's 64 columns of weights into shared memory in the operand's swizzled layout, their codes fetched
+// four stages ahead.  With few tiles K is split over a cluster, whose CTAs add up over distributed shared memory.
+//
+// q4_linear_wide: with enough tiles the products bound it, and shared memory their operands: with x and 256 outputs'
+// weights there an SM moves 96 KB for 512 clocks of products (28 us for 4096 x 2048 -> 1024).  So the weights are the
+// A operand in tensor memory, 128 outputs, written there by the dequantising warps, and 256 tokens of x the B operand:
+// 64 KB per 512 clocks, half of the dequantisation, 550 clocks a stage (16.2 us; 1059 TFLOP/s).  What is left is
+// mostly the start and the output of the one tile a CTA has (about 5.7 us).
+//
+// None has a workspace or a second launch.
 #include <cudaTypedefs.h>
 
 #include "../../include/hla_s6.h"
@@ -115,14 +123,14 @@ static int launch_few(const Q4LinearParams& p, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ many tokens
-template <int BN>
 struct Q4Many {
+  static constexpr int BN = 64;           // outputs of a tile
   static constexpr int A_BYTES = 128 * 64 * 2, B_BYTES = BN * 64 * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 4;
   static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
   static constexpr int DQ = BN / 16;      // dequantising warps, one 16-row tile of the stage each
   static constexpr int RED = BN + 4;      // floats per row of the partial tile that a cluster's CTAs exchange
-  static_assert(128 * RED * 4 <= STAGES * STAGE || BN > 64, "partial tile");
+  static_assert(128 * RED * 4 <= STAGES * STAGE, "partial tile");
   static constexpr uint32_t COLS = BN;
 };
 
@@ -144,8 +152,8 @@ __device__ __forceinline__ void tma_load_rows(void* dst, const void* tmap, uint6
       : "memory");
 }
 
-// out[t, n .. n + 15] from the fp32 sums (columns past N left out).
-__device__ __forceinline__ void store16(const Q4LinearParams& p, int t, int n, float (&v)[16]) {
+// out[t, n .. n + 15] from the fp32 sums (columns past N left out); `pre`: the residual, where it has been loaded.
+__device__ __forceinline__ void store16(const Q4LinearParams& p, int t, int n, float (&v)[16], const uint4* pre = nullptr) {
   __nv_bfloat16* dst = p.out + static_cast<int64_t>(t) * p.o_st + n;
   const __nv_bfloat16* rs = p.res ? p.res + static_cast<int64_t>(t) * p.res_st + n : nullptr;
 #pragma unroll
@@ -154,7 +162,7 @@ __device__ __forceinline__ void store16(const Q4LinearParams& p, int t, int n, f
     if (rs) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const uint4 u = reinterpret_cast<const uint4*>(rs)[q];
+        const uint4 u = pre ? pre[q] : reinterpret_cast<const uint4*>(rs)[q];
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -194,11 +202,10 @@ __device__ __forceinline__ float4 ld_cluster(const void* p, uint32_t rank) {
 }
 
 // warps 0 .. DQ-1 dequantise, then write the output; warp DQ: TMA of x; warp DQ + 1: products.
-template <int BN>
-__global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kernel(
+__global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
     const __grid_constant__ CUtensorMap tmap_x, const Q4LinearParams p) {
-  using C = Q4Many<BN>;
-  constexpr int DQ = C::DQ;
+  using C = Q4Many;
+  constexpr int DQ = C::DQ, BN = C::BN;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // (an offset, not a rounded pointer: the compiler then knows that these are shared-memory addresses)
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
@@ -294,7 +301,7 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
       uint32_t r[16];
       tc::ld16(acc + c0, r);
       tc::wait_ld();
-      if (BN == 64 && p.split > 1) {  // this CTA's part of the sum, for the cluster
+      if (p.split > 1) {  // this CTA's part of the sum, for the cluster
         float4* dst = reinterpret_cast<float4*>(smem + ((warp & 3) * 32 + lane) * C::RED * 4 + (cw + c0) * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -335,31 +342,29 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
     tc::commit(done);
     mbar_wait(done, 0, p.wait_ns);
   }
-  if constexpr (BN == 64) {
-    if (p.split > 1) {
-      // the cluster's CTAs hold a part of the sum each; CTA k adds up and writes every split-th row from k
-      cluster_sync();
-      const int rows = min(128, p.T - m0);
-      for (int u = threadIdx.x; u < ((rows - static_cast<int>(blockIdx.z) + p.split - 1) / p.split) * (BN / 4); u += blockDim.x) {
-        const int r = u / (BN / 4) * p.split + blockIdx.z, c0 = u % (BN / 4) * 4, t = m0 + r, n = n0 + c0;
-        if (n >= p.N) continue;
-        float4 part[8];
+  if (p.split > 1) {
+    // the cluster's CTAs hold a part of the sum each; CTA k adds up and writes every split-th row from k
+    cluster_sync();
+    const int rows = min(128, p.T - m0);
+    for (int u = threadIdx.x; u < ((rows - static_cast<int>(blockIdx.z) + p.split - 1) / p.split) * (BN / 4); u += blockDim.x) {
+      const int r = u / (BN / 4) * p.split + blockIdx.z, c0 = u % (BN / 4) * 4, t = m0 + r, n = n0 + c0;
+      if (n >= p.N) continue;
+      float4 part[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) part[k] = k < p.split ? ld_cluster(smem + (r * C::RED + c0) * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < 8; ++k) part[k] = k < p.split ? ld_cluster(smem + (r * C::RED + c0) * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {  // in order: the sum does not depend on which CTA adds
-          v[0] += part[k].x; v[1] += part[k].y; v[2] += part[k].z; v[3] += part[k].w;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (n + e >= p.N) break;
-          const float rs = p.res ? __bfloat162float(p.res[static_cast<int64_t>(t) * p.res_st + n + e]) : 0.f;
-          p.out[static_cast<int64_t>(t) * p.o_st + n + e] = __float2bfloat16_rn(v[e] * p.ts + rs);
-        }
+      for (int k = 0; k < 8; ++k) {  // in order: the sum does not depend on which CTA adds
+        v[0] += part[k].x; v[1] += part[k].y; v[2] += part[k].z; v[3] += part[k].w;
       }
-      cluster_sync();  // no CTA's memory goes before the others have read it
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= p.N) break;
+        const float rs = p.res ? __bfloat162float(p.res[static_cast<int64_t>(t) * p.res_st + n + e]) : 0.f;
+        p.out[static_cast<int64_t>(t) * p.o_st + n + e] = __float2bfloat16_rn(v[e] * p.ts + rs);
+      }
     }
+    cluster_sync();  // no CTA's memory goes before the others have read it
   }
   tc::fence_before();
   __syncthreads();
@@ -367,16 +372,205 @@ __global__ void __launch_bounds__((Q4Many<BN>::DQ + 2) * 32) q4_linear_many_kern
   if (warp == DQ) tc::dealloc(tmem, C::COLS);
 }
 
-template <int BN>
-static int launch_many(const Q4LinearParams& p, cudaStream_t s) {
-  using C = Q4Many<BN>;
+// ------------------------------------------------------------------ very many tokens
+// From this many tiles on.  A tile takes as long as K has columns, however few there are: 24 tiles (384 x 2048 -> 2048)
+// 15.4 us here and 14.7 with the kernel before, 32 (512 x 2048 -> 2048) 15.0 with either, 48 (256 x 2048 -> 6144) 15.4
+// and 18.7, 64 (1024 x 2048 -> 2048) 15.5 and 27.
+constexpr int kWideTiles = 40;
+constexpr int kWideTokens = 256, kWideOut = 128;          // a CTA's tile of the output
+constexpr int kWideStages = 6, kWideStage = kWideTokens * 128;  // 64 columns of x, bf16
+constexpr int kWideSmem = 1024 + kWideStages * kWideStage + 256;
+static_assert(kWideTokens * kWideOut * 4 <= kWideStages * kWideStage, "the output tile replaces the stages");
+static_assert(kWideTokens + kWideStages * 32 <= 512, "tensor memory");
+
+// warps 0-7 dequantise (groups of four take turns), then write the output; warp 8: TMA of x; warp 9: products.
+__global__ void __launch_bounds__(320, 1) q4_linear_wide_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                                                                const Q4LinearParams p) {
+  constexpr int S = kWideStages, AHEAD = S / 2;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + S * kWideStage);  // x of a stage copied
+  uint64_t* a_full = x_full + S;                                          // its weights in tensor memory
+  uint64_t* empty = a_full + S;                                           // its products done
+  uint64_t* done = empty + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * kWideOut, m0 = blockIdx.y * kWideTokens, NK = (p.K + 63) / 64;
+  if (warp == 8) tc::alloc(tmem_slot, 512);
+  if (threadIdx.x == 9 * 32) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&a_full[s], 4);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;  // columns: the output's 256 tokens, then a stage's 64 weight columns each
+  const tc::Waits wait{abort_flag, nullptr, p.wait_ns};
+
+  if (warp < 8) {
+    const int grp = warp >> 2, w = warp & 3, row = 32 * w + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    // group 0 takes the first halves of the weight tiles (64 of 128 columns), group 1 the second
+    const int own = (NK - grp + 1) / 2, h = (row >> 3) & 1, g = row & 7;
+    const bool there = n0 / 16 + row / 16 < (p.N + 15) / 16;
+    const uint8_t* src = p.w + (n0 / 16 + row / 16) * (static_cast<int64_t>((p.K + 127) / 128) * kQ4WeightTile);
+    const uint8_t *codes = src + h * 512 + g * 64 + grp * 32, *scales = src + 1024 + g * 8 + grp * 4 + h;
+    uint4 code[AHEAD][2];
+    uint32_t sb[AHEAD][2];
+    int next = 0;
+    auto fetch = [&](uint4 (&cd)[2], uint32_t (&s)[2]) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        cd[q] = make_uint4(0u, 0u, 0u, 0u);
+        s[q] = 0u;
+        if (there && next < own) {
+          cd[q] = __ldg(reinterpret_cast<const uint4*>(codes + 16 * q));
+          s[q] = __ldg(scales + 2 * q);
+        }
+      }
+      codes += kQ4WeightTile;
+      scales += kQ4WeightTile;
+      ++next;
+    };
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) fetch(code[a], sb[a]);
+    uint32_t phase = 1;
+    for (int i0 = 0; i0 < own; i0 += AHEAD, phase ^= 1) {
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        if (i0 + a >= own) break;
+        const int s = 2 * a + grp;
+        wait(&empty[s], phase, kErrWaitEmpty);
+        __syncwarp();
+        tc::fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const Q4Scale sc(e4m3x2_to_bf2(sb[a][q] | (sb[a][q] << 8)));
+          const uint32_t x[4] = {code[a][q].x, code[a][q].y, code[a][q].z, code[a][q].w};
+          uint32_t v[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[4 * j] = q4_pair<0>(x[j], sc);
+            v[4 * j + 1] = q4_pair<1>(x[j], sc);
+            v[4 * j + 2] = q4_pair<2>(x[j], sc);
+            v[4 * j + 3] = q4_pair<3>(x[j], sc);
+          }
+          tc::st16(lane_base + kWideTokens + s * 32 + q * 16, v);
+        }
+        fetch(code[a], sb[a]);
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_full[s]);
+      }
+    }
+    // ---- output: through shared memory, where a token's 128 columns lie side by side (16-byte chunks swizzled)
+    const int tid = threadIdx.x & 127, seg = tid & 7;  // 16 columns of every 16th token
+    uint4 pre[8][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = m0 + grp * 128 + (tid >> 3) + 16 * i, n = n0 + 16 * seg;
+      pre[i][0] = pre[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.res && p.vec && t < p.T && n + 16 <= p.N) {
+        const uint4* r = reinterpret_cast<const uint4*>(p.res + static_cast<int64_t>(t) * p.res_st + n);
+        pre[i][0] = r[0];
+        pre[i][1] = r[1];
+      }
+    }
+    wait(done, 0, kErrWaitFull);
+    __syncwarp();
+    tc::fence_after();
+    uint8_t* tile = smem + grp * 128 * 512;
+    {
+      const uint32_t at = (8 * w + ((lane >> 2) ^ w)) * 16 + (lane & 3) * 4;
+#pragma unroll 2
+      for (int c0 = 0; c0 < 128; c0 += 16) {
+        uint32_t r[16];
+        tc::ld16(lane_base + grp * 128 + c0, r);
+        tc::wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) *reinterpret_cast<uint32_t*>(tile + (c0 + e) * 512 + at) = r[e];
+      }
+    }
+    named_bar_sync(1 + grp, 128);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int tl = (tid >> 3) + 16 * i, t = m0 + grp * 128 + tl, n = n0 + 16 * seg;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = 4 * seg + e;
+        const float4 f = *reinterpret_cast<const float4*>(tile + tl * 512 + ((q & ~7) | ((q & 7) ^ (q >> 3))) * 16);
+        v[4 * e] = f.x; v[4 * e + 1] = f.y; v[4 * e + 2] = f.z; v[4 * e + 3] = f.w;
+      }
+      if (t < p.T && n < p.N) store16(p, t, n, v, pre[i]);
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      prefetch_tmap(&tmap_x);
+      for (int kb = 0; kb < NK; ++kb) {
+        const int s = kb % S;
+        if (kb >= S) wait(&empty[s], ((kb / S) - 1) & 1, kErrWaitEmpty);
+        mbar_arrive_expect_tx(&x_full[s], kWideStage);  // rows and columns past x are zeros
+        tma_load_rows(smem + s * kWideStage, &tmap_x, &x_full[s], kb * 64, m0);
+        tma_load_rows(smem + s * kWideStage + kWideStage / 2, &tmap_x, &x_full[s], kb * 64, m0 + 128);
+      }
+      // the last copies land before the CTA ends, also when a wait has given up
+      for (int kb = max(0, NK - S); kb < NK; ++kb) mbar_wait(&x_full[kb % S], (kb / S) & 1, p.wait_ns);
+    }
+  } else if (tc::elect()) {
+    uint32_t phase = 0;
+    for (int kb0 = 0; kb0 < NK; kb0 += S, phase ^= 1) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (kb0 + s >= NK) break;
+        wait(&a_full[s], phase, kErrWaitFull);
+        wait(&x_full[s], phase, kErrWaitFull);
+        tc::fence_after();
+        const uint64_t xd = tc::desc_sw128(smem_u32(smem + s * kWideStage));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc::mma_ts(tmem, tmem + kWideTokens + s * 32 + k * 8, xd + 2 * k, tc::idesc(1, 128, kWideTokens), kb0 + s + k > 0);
+        tc::commit(&empty[s]);
+      }
+    }
+    tc::commit(done);
+    mbar_wait(done, 0, p.wait_ns);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::dealloc(tmem, 512);
+}
+
+static int launch_wide(const Q4LinearParams& p, cudaStream_t s) {
   CUtensorMap tx;
   int rc = rows_tmap(&tx, p.x, p.T, p.K, p.x_st);
   if (rc) return rc;
   static unsigned attr_mask = 0;
-  ensure_smem_limit(q4_linear_many_kernel<BN>, C::SMEM, attr_mask);
+  ensure_smem_limit(q4_linear_wide_kernel, kWideSmem, attr_mask);
+  const dim3 grid((p.N + kWideOut - 1) / kWideOut, (p.T + kWideTokens - 1) / kWideTokens);
+  q4_linear_wide_kernel<<<grid, 320, kWideSmem, s>>>(tx, p);
+  return cuda_status(cudaGetLastError(), "q4_linear_wide_kernel launch");
+}
+
+static int launch_many(const Q4LinearParams& p, cudaStream_t s) {
+  using C = Q4Many;
+  CUtensorMap tx;
+  int rc = rows_tmap(&tx, p.x, p.T, p.K, p.x_st);
+  if (rc) return rc;
+  static unsigned attr_mask = 0;
+  ensure_smem_limit(q4_linear_many_kernel, C::SMEM, attr_mask);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N + BN - 1) / BN, (p.T + 127) / 128, p.split);
+  cfg.gridDim = dim3((p.N + C::BN - 1) / C::BN, (p.T + 127) / 128, p.split);
   cfg.blockDim = dim3((C::DQ + 2) * 32);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
@@ -387,7 +581,7 @@ static int launch_many(const Q4LinearParams& p, cudaStream_t s) {
   attr[0].val.clusterDim.z = p.split;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 1 : 0;
-  return cuda_status(cudaLaunchKernelEx(&cfg, q4_linear_many_kernel<BN>, tx, p), "q4_linear_many_kernel launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, q4_linear_many_kernel, tx, p), "q4_linear_many_kernel launch");
 }
 
 }  // namespace hla
@@ -433,13 +627,14 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
   if (num_tokens <= 8) return out_features >= 16384 ? launch_few<1, 2>(p, s) : launch_few<1, 1>(p, s);
   if (num_tokens <= 16) return launch_few<2, 1>(p, s);
   if (num_tokens <= kQ4FewTokens) return launch_few<4, 2>(p, s);
-  const int64_t mt = (num_tokens + 127) / 128, wide = mt * ((out_features + 255) / 256);
+  const int64_t mt = (num_tokens + 127) / 128;
+  const int64_t wide = static_cast<int64_t>((num_tokens + kWideTokens - 1) / kWideTokens) * ((out_features + kWideOut - 1) / kWideOut);
+  if (wide >= kWideTiles) return launch_wide(p, s);
   p.split = 1;
-  if (wide >= 64) return launch_many<256>(p, s);
   // K is split over a cluster while the CTAs still fit two to an SM and each keeps at least 4 blocks of it
   const int64_t tiles = mt * ((out_features + 63) / 64);
   while (p.split < 8 && tiles * p.split * 2 <= 296 && (in_features + 63) / 64 >= 8 * p.split) p.split *= 2;
-  return launch_many<64>(p, s);
+  return launch_many(p, s);
 }
 
 }  // extern "C"

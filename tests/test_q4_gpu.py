@@ -420,6 +420,15 @@ def test_linear(T, N, K, residual):
     check_linear(y, x, wq, scale, res if residual else None, K)
 
 
+# enough tiles for the kernel of the largest calls: ends inside a tile in every direction, the shortest K, one block of K
+# more than a whole number of stages, and rows of outputs that are not 16-byte aligned
+@pytest.mark.parametrize('T,N,K', [(1030, 2001, 416), (4096, 512, 128), (8200, 130, 32), (2100, 1000, 2048),
+                                   (1025, 1800, 832), (4000, 400, 64)])
+@pytest.mark.parametrize('residual', [False, True])
+def test_linear_wide(T, N, K, residual):
+    test_linear(T, N, K, residual)
+
+
 @pytest.mark.parametrize('T', [2, 20, 300])
 def test_linear_strides_in_place_residual_and_zero_tokens(T):
     q4 = pkg('q4')
