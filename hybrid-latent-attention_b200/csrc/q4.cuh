@@ -156,15 +156,33 @@ __device__ __forceinline__ uint32_t q4_word(const uint32_t (&n)[8]) {
   for (int i = 0; i < 4; ++i) w |= (n[2 * i] << (4 * i)) | (n[2 * i + 1] << (16 + 4 * i));
   return w;
 }
-// The same word for bf16 values and a power-of-two tensor scale, in 6 instructions a value instead of 16.  A quotient
-// of 8 by 4 significant bits that is not half way between two integers is at least 1/1000 away from that, so rounding
-// x * inv is right for it with either neighbour of inv; half way the two neighbours give the two integers, of which the
-// even one is (a + b + ((a + b) / 2) % 2) / 2, for two columns in a register.  amax: the group's largest value, which
-// says whether anything has to be clamped (see above).
+// Scale byte and codes of bf16 values for a power-of-two tensor scale (2^-124 .. 2^123), without divisions and in 6
+// instructions a value instead of 16:
+// * amax / 7 has at most 5 significant bits where it is half way between two e4m3 numbers, and is otherwise 2^-11 or
+//   more away from that, relative; so amax * (1 / 7), right to 2^-23, is rounded to 16 bits and falls as the quotient.
+// * a quotient of 8 by 4 significant bits that is not half way between two integers is at least 1/1000 away from that,
+//   so x * inv rounds like it for an inv within 2^-20; half way a value below and one above 1 / step give the two
+//   integers, of which the even one is (a + b + ((a + b) / 2) % 2) / 2, computed for two columns in a register.
+// amax: the group's largest value, which says whether anything has to be clamped (see above).
+__device__ __forceinline__ bool q4_pow2(float ts) {
+  const uint32_t b = __float_as_uint(ts);
+  return (b & 0x7fffffu) == 0 && b - (3u << 23) <= (247u << 23);
+}
+__device__ __forceinline__ uint32_t q4_scale_byte_pow2(float amax, float ts) {
+  const float seventh = __uint_as_float(__float_as_uint(1.f / 7.f) + (127u << 23) - __float_as_uint(ts));  // 1 / (7 ts)
+  const float q = __uint_as_float((__float_as_uint(amax * seventh) + 0x80u) & 0xffffff00u);
+  return __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float rcp_approx(float x) {  // to 1 ulp (0 is infinite)
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t q4_word_pow2(const float (&f)[8], float amax, float step) {
   constexpr float kMagic = 12582912.f + 8.f;
-  const uint32_t inv = step > 0.f ? __float_as_uint(fminf(__frcp_rn(step), 1e38f)) : 0u;
-  const float lo = inv ? __uint_as_float(inv - 1u) : 0.f, hi = inv ? __uint_as_float(inv + 1u) : 0.f;
+  // a step of 0 (every value below 2^-10 * 7 ts) leaves the codes at 8
+  const uint32_t inv = __float_as_uint(rcp_approx(step));
+  const float lo = step > 0.f ? __uint_as_float(inv - 2u) : 0.f, hi = step > 0.f ? __uint_as_float(inv + 2u) : 0.f;
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = f[i];

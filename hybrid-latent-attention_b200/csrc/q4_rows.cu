@@ -25,10 +25,12 @@ __device__ __forceinline__ uint32_t quantize8(const float (&f)[8], float ts, uin
   for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
   a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
   a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+  if (q4_pow2(ts)) {
+    scale = q4_scale_byte_pow2(a, ts);
+    return q4_word_pow2(f, a, q4_scale_value(scale) * ts);
+  }
   scale = q4_scale_byte(a, ts);
-  const float step = q4_scale_value(scale) * ts;
-  if ((__float_as_uint(ts) & 0x7fffffu) == 0) return q4_word_pow2(f, a, step);
-  const Q4Coder code(step);
+  const Q4Coder code(q4_scale_value(scale) * ts);
   uint32_t n[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) n[i] = code(f[i]);
