@@ -53,79 +53,94 @@ struct Q4CommitArgs {
   int R, T;
   float k_ts, v_ts;
   int64_t* slot_out;
+  int rounds;
 };
 
 // W / 16 threads per row; thread k holds columns 8k .. and W/2 + 8k .. of both halves, i.e. whole RoPE
 // pairs and quarters of groups, so the amax of a group is two shuffles.
 constexpr int kQ4CommitThreads = 128;
+constexpr int kQ4CommitRounds = 4;  // rows of a thread group, one after the other, with many tokens
 template <int W>
 __global__ void __launch_bounds__(kQ4CommitThreads) q4_commit_kernel(const Q4CommitArgs a) {
   constexpr int PER = W / 16;
   __shared__ int32_t qsl_s[kQslCap];
   const int32_t* qsl = stage_qsl(a.qsl, a.R, qsl_s);
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kQ4CommitThreads / PER) + threadIdx.x / PER;
-  const int k = threadIdx.x % PER;
-  const bool in = t < a.T;
-  // every load that does not need the slot goes out before the chain of lookups that finds it
-  uint4 raw[6] = {};
+  constexpr int ROWS = kQ4CommitThreads / PER;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS * a.rounds;
   const Q4Tile tl(W);
-  uint8_t* tile = nullptr;  // NULL: no slot
-  int r = 0;
-  if (in) {
-    const __nv_bfloat16* src = a.row + t * a.row_st + 8 * k;
+  // One thread looks a row up (token_slot of decode_ops.cuh with 32-bit divisions: a position inside the table is below
+  // 2^31, checked).  The row's own threads did it at first, a third of their instructions.
+  __shared__ uint8_t* tile_s[ROWS * kQ4CommitRounds];  // NULL: no slot
+  __shared__ int row_s[ROWS * kQ4CommitRounds];
+  if (threadIdx.x < ROWS * a.rounds) {
+    const int64_t t = first + threadIdx.x;
+    uint8_t* tile = nullptr;
+    if (t < a.T) {
+      const int64_t pos = a.positions[t];
+      int req;
+      int64_t slot = -1;
+      if (token_request(qsl, a.R, static_cast<int>(t), req) && pos >= 0 && pos < static_cast<int64_t>(a.max_blocks) * a.page) {
+        const uint32_t p32 = static_cast<uint32_t>(pos), page = a.page, col = p32 / page, off = p32 - col * page;
+        const int blk = a.bt[static_cast<int64_t>(req) * a.bt_st + col];
+        if (blk >= 0 && blk < a.num_blocks) {
+          slot = static_cast<int64_t>(blk) * a.page + off;
+          tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
+          row_s[threadIdx.x] = static_cast<int>(off % 16);
+        }
+      }
+      if (a.slot_out) a.slot_out[t] = slot;
+    }
+    tile_s[threadIdx.x] = tile;
+  }
+  const int k = threadIdx.x % PER;
+  for (int round = 0; round < a.rounds; ++round) {
+    const int at = round * ROWS + threadIdx.x / PER;
+    const int64_t t = first + at;
+    uint4 raw[6] = {};
+    if (t < a.T) {
+      const __nv_bfloat16* src = a.row + t * a.row_st + 8 * k;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * (W / 2)));
-    const int64_t pos = a.positions[t];
-    const __nv_bfloat16* tab = a.table + clamp_pos(pos, a.max_pos) * a.tab_st + 8 * k;
-    raw[4] = __ldg(reinterpret_cast<const uint4*>(tab));
-    raw[5] = __ldg(reinterpret_cast<const uint4*>(tab + W / 2));
-    // token_slot (decode_ops.cuh) with 32-bit divisions: a position inside the table is below 2^31 (checked)
-    int req;
-    int64_t slot = -1;
-    if (token_request(qsl, a.R, static_cast<int>(t), req) && pos >= 0 && pos < static_cast<int64_t>(a.max_blocks) * a.page) {
-      const uint32_t p32 = static_cast<uint32_t>(pos), page = a.page, col = p32 / page, off = p32 - col * page;
-      const int blk = a.bt[static_cast<int64_t>(req) * a.bt_st + col];
-      if (blk >= 0 && blk < a.num_blocks) {
-        slot = static_cast<int64_t>(blk) * a.page + off;
-        tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
-        r = static_cast<int>(off % 16);
+      for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * (W / 2)));
+      const __nv_bfloat16* tab = a.table + clamp_pos(a.positions[t], a.max_pos) * a.tab_st + 8 * k;
+      raw[4] = __ldg(reinterpret_cast<const uint4*>(tab));
+      raw[5] = __ldg(reinterpret_cast<const uint4*>(tab + W / 2));
+    }
+    if (round == 0) __syncthreads();  // the lookups, behind the first row's loads
+    uint8_t* const tile = tile_s[at];
+    const int r = tile ? row_s[at] : 0;
+    // latent RoPE of the K half in packed bf16 arithmetic: every operation rounds its exact result once, which on bf16
+    // inputs is the fp32 operation rounded to bf16 (a product is exact in fp32; a sum's first rounding is innocuous)
+    float x[4][8];
+    {
+      uint32_t* lo = reinterpret_cast<uint32_t*>(&raw[0]);
+      uint32_t* hi = reinterpret_cast<uint32_t*>(&raw[1]);
+      const uint32_t* cs = reinterpret_cast<const uint32_t*>(&raw[4]);
+      const uint32_t* sn = reinterpret_cast<const uint32_t*>(&raw[5]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 x1 = *reinterpret_cast<const __nv_bfloat162*>(lo + i), x2 = *reinterpret_cast<const __nv_bfloat162*>(hi + i);
+        const __nv_bfloat162 c = *reinterpret_cast<const __nv_bfloat162*>(cs + i), s = *reinterpret_cast<const __nv_bfloat162*>(sn + i);
+        const __nv_bfloat162 y1 = __hadd2_rn(__hmul2_rn(x1, c), __hneg2(__hmul2_rn(x2, s)));
+        const __nv_bfloat162 y2 = __hadd2_rn(__hmul2_rn(x2, c), __hmul2_rn(x1, s));
+        lo[i] = *reinterpret_cast<const uint32_t*>(&y1);
+        hi[i] = *reinterpret_cast<const uint32_t*>(&y2);
       }
     }
-    if (a.slot_out && k == 0) a.slot_out[t] = slot;
-  }
-  const bool live = tile != nullptr;
-  // latent RoPE of the K half in packed bf16 arithmetic: every operation rounds its exact result once, which on bf16
-  // inputs is the fp32 operation rounded to bf16 (a product is exact in fp32; a sum's first rounding is innocuous)
-  float x[4][8];
-  {
-    uint32_t* lo = reinterpret_cast<uint32_t*>(&raw[0]);
-    uint32_t* hi = reinterpret_cast<uint32_t*>(&raw[1]);
-    const uint32_t* cs = reinterpret_cast<const uint32_t*>(&raw[4]);
-    const uint32_t* sn = reinterpret_cast<const uint32_t*>(&raw[5]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack8(raw[i], x[i]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 x1 = *reinterpret_cast<const __nv_bfloat162*>(lo + i), x2 = *reinterpret_cast<const __nv_bfloat162*>(hi + i);
-      const __nv_bfloat162 c = *reinterpret_cast<const __nv_bfloat162*>(cs + i), s = *reinterpret_cast<const __nv_bfloat162*>(sn + i);
-      const __nv_bfloat162 y1 = __hadd2_rn(__hmul2_rn(x1, c), __hneg2(__hmul2_rn(x2, s)));
-      const __nv_bfloat162 y2 = __hadd2_rn(__hmul2_rn(x2, c), __hmul2_rn(x1, s));
-      lo[i] = *reinterpret_cast<const uint32_t*>(&y1);
-      hi[i] = *reinterpret_cast<const uint32_t*>(&y2);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) unpack8(raw[i], x[i]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t sb;
-    const uint32_t w = quantize8(x[i], i < 2 ? a.k_ts : a.v_ts, sb);  // warp-collective: every lane
-    if (!live) continue;
-    const int octet = k + (i & 1) * PER, group = octet / 4;
-    if (i < 2) {
-      *reinterpret_cast<uint32_t*>(tile + tl.k_codes(group, r) + 4 * (octet & 3)) = w;
-      if ((k & 3) == 0) tile[tl.k_scale(r, group)] = static_cast<uint8_t>(sb);
-    } else {
-      *reinterpret_cast<uint32_t*>(tile + tl.v_codes(octet, r)) = w;
-      if ((k & 3) == 0) tile[tl.v_scale(group, r)] = static_cast<uint8_t>(sb);
+      uint32_t sb;
+      const uint32_t w = quantize8(x[i], i < 2 ? a.k_ts : a.v_ts, sb);  // warp-collective: every lane
+      if (!tile) continue;
+      const int octet = k + (i & 1) * PER, group = octet / 4;
+      if (i < 2) {
+        *reinterpret_cast<uint32_t*>(tile + tl.k_codes(group, r) + 4 * (octet & 3)) = w;
+        if ((k & 3) == 0) tile[tl.k_scale(r, group)] = static_cast<uint8_t>(sb);
+      } else {
+        *reinterpret_cast<uint32_t*>(tile + tl.v_codes(octet, r)) = w;
+        if ((k & 3) == 0) tile[tl.v_scale(group, r)] = static_cast<uint8_t>(sb);
+      }
     }
   }
 }
@@ -274,7 +289,11 @@ int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, 
   a.k_ts = k_scale;
   a.v_ts = v_scale;
   a.slot_out = slot_out;
-  const int rows = kQ4CommitThreads / (width / 16), grid = (num_tokens + rows - 1) / rows;
+  // rounds only once every SM has its CTAs without them (their rows are then in flight together)
+  int rows = kQ4CommitThreads / (width / 16);
+  a.rounds = num_tokens >= rows * kQ4CommitRounds * 148 * 8 ? kQ4CommitRounds : 1;
+  rows *= a.rounds;
+  const int grid = (num_tokens + rows - 1) / rows;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (width == 256) q4_commit_kernel<256><<<grid, kQ4CommitThreads, 0, s>>>(a);
   else if (width == 512) q4_commit_kernel<512><<<grid, kQ4CommitThreads, 0, s>>>(a);

@@ -256,7 +256,8 @@ def commit_setup(share, W, page, seed, start=None, padding=0):
 
 
 COMMITS = [([1], 512, 16, 0), ([1, 1, 1], 256, 16, 0), ([5, 0, 17, 1], 512, 16, 3), ([40, 33], 1024, 32, 0),
-           ([7], 256, 48, 2), ([64] * 3, 512, 32, 1), ([1] * 130, 512, 16, 5)]
+           ([7], 256, 48, 2), ([64] * 3, 512, 32, 1), ([1] * 130, 512, 16, 5),
+           ([4000, 1, 5601], 1024, 16, 7)]    # enough tokens for several rows a thread
 
 
 @pytest.mark.parametrize('share,W,page,padding', COMMITS)
