@@ -28,6 +28,13 @@
 //   warp 26     bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
 // The dequantising loops are kept rolled: unrolled over a step they outgrew the instruction caches, and the warps
 // of a scheduler run different code (190 us unrolled with one group of each, 137 us rolled with a softmax group).
+//
+// Measured: 64 requests of 8160 rows, width 512: 91 us (3.15 TB/s, 188 TFLOP/s; the bytes alone 44); 4 of 65501:
+// 49 us (22); 37 of 0 to 16384, width 256: 28 us.  A step of 128 rows takes 6000 clocks and 14000 warp instructions,
+// 0.6 of the issue slots; without any dequantisation it would still take 4700, so what bounds it is the hand-over
+// between the roles (waits, barriers, instruction fetch) as much as the arithmetic.  Tried without a gain: two CTAs
+// of 13 warps (112 us), a ring each for K and V with a copy warp each (90.0 and 50.0 us), V chunks of two tiles (90.8
+// and 50.4), all on mma.sync (118).
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
 // of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
 // 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
     const uint64_t policy = l2_policy_evict_first();
     // The lanes look up 32 tiles at once: a lookup per unit, when its slot was free, kept this warp busy for longer
-    // than the others took to use the unit up (64 x 8160 rows: 95 -> XX us).
+    // than the others took to use the unit up (64 x 8160 rows: 95 -> 91 us).
     int unit = 0;
     while (st.next()) {
       for (int b = st.tile; b < st.tend; b += 32) {
