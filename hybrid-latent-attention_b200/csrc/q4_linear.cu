@@ -373,10 +373,6 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
 }
 
 // ------------------------------------------------------------------ very many tokens
-// From this many tiles on.  A tile takes as long as K has columns, however few there are: 24 tiles (384 x 2048 -> 2048)
-// 15.4 us here and 14.7 with the kernel before, 32 (512 x 2048 -> 2048) 15.0 with either, 48 (256 x 2048 -> 6144) 15.4
-// and 18.7, 64 (1024 x 2048 -> 2048) 15.5 and 27.
-constexpr int kWideTiles = 40;
 constexpr int kWideTokens = 256, kWideOut = 128;          // a CTA's tile of the output
 constexpr int kWideStages = 6, kWideStage = kWideTokens * 128;  // 64 columns of x, bf16
 constexpr int kWideSmem = 1024 + kWideStages * kWideStage + 256;
@@ -624,16 +620,25 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
   p.vec = a16(out, out_stride_t) && (!residual || a16(residual, residual_stride_t));
   p.wait_ns = wait_limit_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (num_tokens <= 8) return out_features >= 16384 ? launch_few<1, 2>(p, s) : launch_few<1, 1>(p, s);
-  if (num_tokens <= 16) return launch_few<2, 1>(p, s);
-  if (num_tokens <= kQ4FewTokens) return launch_few<4, 2>(p, s);
-  const int64_t mt = (num_tokens + 127) / 128;
-  const int64_t wide = static_cast<int64_t>((num_tokens + kWideTokens - 1) / kWideTokens) * ((out_features + kWideOut - 1) / kWideOut);
-  if (wide >= kWideTiles) return launch_wide(p, s);
+  // Few tokens: tiles of 16 outputs x 8 tokens.  One token tile: two row tiles a CTA once there are enough CTAs (1 x 2048
+  // -> 12288 5.0 us instead of 5.3; -> 6144 4.7 instead of 4.3).
+  if (num_tokens <= 8) return out_features >= 8192 ? launch_few<1, 2>(p, s) : launch_few<1, 1>(p, s);
+  // Then two token tiles share a row tile's codes, or four two row tiles' from 900 tiles on (48 tokens x 2048 -> 2048,
+  // 768 tiles: 6.5 and 6.4 us; 64, 1024 tiles: 8.0 and 6.5; 64 x 2048 -> 512, 256 tiles: 3.8 and 6.3).  From 32 tokens
+  // and 1280 tiles on the kernel for many tokens is as fast (32 x 2048 -> 6144: 11.2 and 11.2 us; 48: 14.4 and 11.3;
+  // 64 x 2048 -> 2048: 6.5 and 7.0); with fewer tokens it is not (24 x 2048 -> 49152: 54 and 78).
+  const int64_t few = static_cast<int64_t>((out_features + 15) / 16) * ((num_tokens + 7) / 8);
+  if (num_tokens < 32 || (num_tokens <= kQ4FewTokens && few <= 900)) return launch_few<2, 1>(p, s);
+  if (num_tokens <= kQ4FewTokens && few <= 1280) return launch_few<4, 2>(p, s);
+  // More tiles of 128 tokens x 64 outputs than SMs: the large tiles, which take the same time however few there are
+  // (512 x 2048 -> 2048, 128 of the small ones: 15.0 us with the large, 13.0 with the small; 256 x 2048 -> 6144, 192:
+  // 15.4 and 18.7)
+  const int64_t tiles = static_cast<int64_t>((num_tokens + 127) / 128) * ((out_features + 63) / 64);
+  if (tiles > 148) return launch_wide(p, s);
+  // K is split over a cluster while every SM has at most one CTA and each keeps at least 4 blocks of 64 (128 x 2048 ->
+  // 2048, 32 tiles: 9.5, 7.5 and 9.5 us split by 2, 4 and 8; -> 6144, 96 tiles: 11.7 whole, 13.2 split by 2)
   p.split = 1;
-  // K is split over a cluster while the CTAs still fit two to an SM and each keeps at least 4 blocks of it
-  const int64_t tiles = mt * ((out_features + 63) / 64);
-  while (p.split < 8 && tiles * p.split * 2 <= 296 && (in_features + 63) / 64 >= 8 * p.split) p.split *= 2;
+  while (p.split < 8 && tiles * p.split * 2 <= 148 && (in_features + 63) / 64 >= 8 * p.split) p.split *= 2;
   return launch_many(p, s);
 }
 

@@ -387,7 +387,8 @@ def test_round_trip_error_is_half_a_step():
 # ------------------------------------------------------------------------------------ linear
 LINEARS = [(1, 16, 32), (1, 1, 128), (3, 17, 160), (8, 100, 96), (9, 2048, 2048), (16, 33, 1024), (17, 48, 4096),
            (33, 512, 2048), (64, 1024, 128), (65, 250, 416), (127, 64, 2048), (128, 256, 128), (130, 512, 2048),
-           (257, 1024, 512), (300, 272, 192), (200, 100, 320), (1, 6144, 2048), (600, 768, 640)]
+           (257, 1024, 512), (300, 272, 192), (200, 100, 320), (1, 6144, 2048), (600, 768, 640),
+           (5, 8200, 64), (64, 2048, 160), (57, 2030, 96), (40, 5000, 64), (31, 5000, 64)]
 
 
 def linear_case(T, N, K, seed):
