@@ -36,8 +36,9 @@ class LatentLayer(nn.Module):
             nn.init.normal_(p, std=1 / math.sqrt(hidden))
 
     def pack_writers(self):
-        """From now on the writers run on 4-bit copies of their weights, made here (on CUDA, bf16).  The parameters
-        stay as they are, as does the state dict; a copy is not made again when they change."""
+        """From now on ``s6_layer.write_rows`` runs on 4-bit copies of the writers' weights (``packed_writers``, by
+        loop), made here (on CUDA, bf16).  ``writer`` and the state dict stay as they are; a copy is not made again
+        when its parameter changes."""
         self.packed_writers = [q4.Weight.of(w.weight.detach()) for w in (self.cand1, *self.cand_s)]
 
     def readers(self, loop):
@@ -47,10 +48,7 @@ class LatentLayer(nn.Module):
         return self.q_absorb[loop - 1], self.out_absorb[loop - 1], self.rank
 
     def writer(self, loop):
-        """The projection weight written at ``loop`` (E_1' at loop 0, E_{loop+1} after): bf16, or a ``q4.Weight``
-        after ``pack_writers``."""
-        if self.packed_writers is not None:
-            return self.packed_writers[loop]
+        """The projection weight written at ``loop`` (E_1' at loop 0, E_{loop+1} after)."""
         return self.cand1.weight if loop == 0 else self.cand_s[loop - 1].weight
 
 

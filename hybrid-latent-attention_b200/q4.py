@@ -96,6 +96,11 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
+def _check_flag(error_flag):
+    if error_flag is not None and (error_flag.dtype is not I32 or error_flag.numel() < 1):
+        raise ValueError('error_flag must be int32 [1]')
+
+
 def _cache_geometry(cache, width):
     """``(num_blocks, block stride in bytes, page)`` of a 4-bit cache of latent width ``width``."""
     shape, bytes_ = cache.shape, 17 * width // 16
@@ -133,18 +138,20 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
         if empty.shape != (T,):
             raise ValueError('empty must be [T]')
         empty = empty.contiguous() if empty.dtype in (torch.bool, torch.uint8) else (empty != 0)
-    buffer = workspace.ensure(q_lat.device)
-    index = _device_of(q_lat, cache, block_table, ctx, empty, error_flag, buffer)
+    _check_flag(error_flag)
+    index = _device_of(q_lat, cache, block_table, ctx, empty, error_flag)
+    buffer = workspace.ensure(q_lat.device)   # (after the check: a workspace keeps the device of its first use)
+    _device_of(q_lat, buffer)
     need = T * H * num_kv_splits * (W + 1)
     if need > buffer.numel():
         raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {buffer.numel()}')
     o = q_lat.new_empty(T, H, W)
     lse = buffer.new_empty(H, T)
     ctx = ctx.contiguous()
-    _launch(index, 'hla_s6_history_attention_q4', q_lat.data_ptr(), stride[0], stride[1], cache.data_ptr(), nb,
-            sb, block_table.data_ptr(), bt_stride, bt_cols, ctx.data_ptr(), _address(empty), T, H, W, page, scale,
-            num_kv_splits, buffer.data_ptr(), need, k_scale, v_scale, o.data_ptr(), H * W, W, lse.data_ptr(),
-            _address(error_flag))
+    _launch(index, 'hla_s6_history_attention_q4', q_lat.data_ptr(), stride[0], stride[1], cache.data_ptr(), nb, sb,
+            block_table.data_ptr(), bt_stride, bt_cols, ctx.data_ptr(), _address(empty), T, H, W, page, float(scale),
+            int(num_kv_splits), buffer.data_ptr(), need, float(k_scale), float(v_scale), o.data_ptr(), H * W, W,
+            lse.data_ptr(), _address(error_flag))
     return o, lse
 
 
@@ -172,8 +179,8 @@ def commit_rows(row, positions, table, cache, block_table, query_start_loc, k_sc
     slots = positions.new_empty(T)
     _launch(index, 'hla_s6_commit_rows_q4', row.data_ptr(), stride[0], W, positions.data_ptr(), table.data_ptr(),
             tab_stride[0], tab_rows[0], cache.data_ptr(), nb, sb, page, block_table.data_ptr(),
-            bt_stride, bt_cols, query_start_loc.data_ptr(), requests, T, k_scale, v_scale,
-            slots.data_ptr())
+            bt_stride, bt_cols, query_start_loc.data_ptr(), requests, T, float(k_scale),
+            float(v_scale), slots.data_ptr())
     return slots
 
 
@@ -187,6 +194,7 @@ def _gather(cache, blocks, slots, rows, k_scale, v_scale, out, error_flag):
         raise IndexError('the block list does not cover the rows')
     if out is not None and (out.shape != (rows, 2 * W) or out.dtype is not BF16 or out.stride(-1) != 1):
         raise ValueError(f'out must be bf16 [{rows}, {2 * W}] with a unit last-dim stride')
+    _check_flag(error_flag)
     device = _device_of(cache, index, out, error_flag)
     index = index.contiguous()
     if out is None:
@@ -194,8 +202,8 @@ def _gather(cache, blocks, slots, rows, k_scale, v_scale, out, error_flag):
     if rows:
         at = index.data_ptr()
         _launch(device, 'hla_s6_gather_rows_q4', cache.data_ptr(), nb, sb, W, page, at if slots is None else None,
-                None if slots is None else at, rows, k_scale, v_scale, out.data_ptr(), out.stride(0),
-                _address(error_flag))
+                None if slots is None else at, rows, float(k_scale), float(v_scale), out.data_ptr(),
+                out.stride(0), _address(error_flag))
     return out
 
 
@@ -225,7 +233,10 @@ def quantize_weight(weight, scale=None):
         raise ValueError('a 4-bit weight needs in_features a multiple of 32')
     index = _device_of(weight)
     if scale is None:
-        scale = tensor_scale(float(weight.abs().amax()))
+        amax = float(weight.abs().amax())
+        if not math.isfinite(amax):
+            raise ValueError('the weight holds values that are not finite')
+        scale = tensor_scale(amax)
     packed = weight.new_empty(weight_tiles(N, K), dtype=U8)
     _launch(index, 'hla_s6_quantize_weight_q4', weight.data_ptr(), weight.stride(0), N, K, scale, packed.data_ptr())
     return packed, float(scale)
@@ -238,7 +249,8 @@ def _check_rows(y, T, N):
 
 def linear(x, packed, out_features, scale, residual=None, out=None):
     """``bf16(scale * x . w^T + residual)`` for ``x [T, K]`` bf16 and the packed weight ``[N, K]``: fp32 sums, one
-    rounding.  ``residual`` and ``out`` are bf16 ``[T, N]``; ``out`` may be ``residual``."""
+    rounding.  ``residual`` and ``out`` are bf16 ``[T, N]``; ``out`` may be ``residual``, and overlaps no other input.
+    Rows of x start at 16-byte boundaries."""
     stride = x.stride()
     if len(stride) != 2 or x.dtype is not BF16 or stride[1] != 1:
         raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
@@ -248,8 +260,8 @@ def linear(x, packed, out_features, scale, residual=None, out=None):
             or not packed.is_contiguous()):
         raise ValueError(f'packed must be contiguous uint8 {list(weight_tiles(N, K))}, got {packed.dtype} '
                          f'{list(packed.shape)}')
-    x_stride = stride[0]
-    if x_stride < K and T > 1:   # rows that overlap (an expanded x)
+    x_stride = stride[0] if T > 1 else K
+    if x_stride < K:   # rows that overlap (an expanded x)
         x, x_stride = x.contiguous(), K
     if residual is not None:
         _check_rows(residual, T, N)
@@ -259,7 +271,7 @@ def linear(x, packed, out_features, scale, residual=None, out=None):
     fresh = out is None
     if fresh:
         out = x.new_empty(T, N)
-    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x_stride, packed.data_ptr(), T, N, K, scale,
+    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x_stride, packed.data_ptr(), T, N, K, float(scale),
             _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(),
             N if fresh else out.stride(0))
     return out

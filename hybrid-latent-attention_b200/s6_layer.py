@@ -178,11 +178,12 @@ def write_rows(sl, loop, h, state=None):
     """Writer accumulation on the attention input ``h[T, hidden]`` (reference s6_layer.py:124-132):
     loop 0 gives ``first = E_1' h``; later loops ``reg = reg + E_t h`` with a bf16 add.  A packed writer
     (``LatentLayer.pack_writers``) runs as ``q4.linear``, which rounds the sum once."""
-    weight = sl.writer(loop) if hasattr(sl, 'writer') else (sl.cand1.weight if loop == 0 else sl.cand_s[loop - 1].weight)
     reg_in = None if loop == 0 or state is None else state.reg
-    if isinstance(weight, q4.Weight):
-        out = weight.linear(h, reg_in)
+    packed = getattr(sl, 'packed_writers', None)
+    if packed is not None:
+        out = packed[loop].linear(h, reg_in)
         return WriterState(None, out) if loop == 0 else WriterState(out, None)
+    weight = sl.writer(loop) if hasattr(sl, 'writer') else (sl.cand1.weight if loop == 0 else sl.cand_s[loop - 1].weight)
     T, K = h.shape
     N = weight.shape[0]
     out = torch.empty(T, N, dtype=h.dtype, device=h.device)

@@ -96,10 +96,14 @@ def history_args(**kw):
     (dict(ctx=torch.zeros(2, dtype=I64)), 'ctx must be int32'),
     (dict(ctx=torch.zeros(3, dtype=I32)), 'ctx must be int32'),
     (dict(empty=torch.zeros(3, dtype=torch.bool)), 'empty must be'),
+    (dict(error_flag=torch.zeros(1, dtype=I64)), 'error_flag must be int32'),
+    (dict(error_flag=torch.zeros(0, dtype=I32)), 'error_flag must be int32'),
 ])
 def test_history_refusals(q4, kw, match):
+    args = history_args(**kw)
     with pytest.raises(ValueError, match=match):
-        q4.history_attention(**history_args(**kw))
+        q4.history_attention(**args)
+    assert args['workspace'].buffer is None      # a refused call leaves the workspace for its first use
 
 
 def commit_args(**kw):
@@ -146,6 +150,8 @@ def test_gather_refusals(q4):
         q4.gather_slots(cache, slots, out=torch.zeros(4, 512, dtype=BF16))
     with pytest.raises(ValueError, match='4-bit latent cache'):
         q4.gather_slots(cache[:, 0], slots)
+    with pytest.raises(ValueError, match='error_flag must be int32'):
+        q4.gather_slots(cache, slots, error_flag=torch.zeros(4, dtype=U8))
 
 
 def test_linear_refusals(q4):

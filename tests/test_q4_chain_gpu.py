@@ -114,7 +114,7 @@ class Layer:
             # projections and the writer: the 4-bit linear's own results
             assert torch.equal(out, self.o.linear(attn.reshape(T, H * D)))
             row = state.first if loop == 0 else state.reg
-            assert torch.equal(row, self.sl.writer(loop).linear(hidden, previous))
+            assert torch.equal(row, self.sl.packed_writers[loop].linear(hidden, previous))
             # the attention, against the bf16 path over the same values
             qkv = self.qkv.linear(hidden)
             q, k, v = (x.view(T, H, D) for x in qkv.split(H * D, -1))
