@@ -158,23 +158,33 @@ struct Q4GatherArgs {
   int* err;
 };
 
-// The 8 values of a word in bf16: (n - 8) s is exact, the tensor scale is applied in fp32 and rounded once.
-__device__ __forceinline__ uint4 q4_values(uint32_t w, uint32_t scale, float ts) {
-  const Q4Scale s(e4m3x2_to_bf2(scale | (scale << 8)));
+constexpr int kQ4GatherMany = 4096;  // rows from which a thread takes four octets
+
+// The 8 values of a word in bf16.  (n - 8) s is exact.  A power-of-two tensor scale goes into s (`folded`; the values
+// stay exact, to bf16's smallest numbers), any other is applied in fp32 and rounded once.
+__device__ __forceinline__ uint4 q4_values(uint32_t w, uint32_t scale, float ts, bool folded, uint32_t ts2) {
+  const uint32_t s2 = e4m3x2_to_bf2(scale | (scale << 8));
+  const Q4Scale s(folded ? bf2_mul(s2, ts2) : s2);
   const uint32_t v[4] = {q4_pair<0>(w, s), q4_pair<1>(w, s), q4_pair<2>(w, s), q4_pair<3>(w, s)};
+  if (folded) return make_uint4(v[0], v[1], v[2], v[3]);
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = pack_bf16(__uint_as_float(v[i] << 16) * ts, __uint_as_float(v[i] & 0xffff0000u) * ts);
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// W / 8 threads per row: thread k takes octet k of the K and of the V half.
-template <int W>
+// PER = W / (8 OCT) threads per row: thread k takes octets k, k + PER .. of the K and of the V half.  With one octet a
+// thread a row's look-up and the tensor scale in fp32 made 12 instructions a value, which bound it (32768 rows of width
+// 512: 17 us; 14.4 with four octets and the scale folded, 85 MB at 5.9 TB/s).  Few rows keep one octet a thread: they
+// need the threads (77 rows of width 256: 1.6 us, 2.2 with four).
+template <int W, int OCT>
 __global__ void __launch_bounds__(256) q4_gather_kernel(const Q4GatherArgs a) {
-  constexpr int PER = W / 8;
+  constexpr int PER = W / (8 * OCT);
   const Q4Tile tl(W);
-  const int octet = threadIdx.x % PER, group = octet / 4;
+  const int k = threadIdx.x % PER;
   const uint32_t page = a.page, cache_rows = static_cast<uint32_t>(a.num_blocks) * page;  // < 2^31 (checked)
+  const bool k_fold = q4_pow2(a.k_ts) && a.k_ts < 1e30f, v_fold = q4_pow2(a.v_ts) && a.v_ts < 1e30f;
+  const uint32_t k_ts2 = pack_bf16(a.k_ts, a.k_ts), v_ts2 = pack_bf16(a.v_ts, a.v_ts);
   for (uint32_t i = blockIdx.x * (256 / PER) + threadIdx.x / PER; i < a.rows; i += gridDim.x * (256 / PER)) {
     uint32_t blk, off;
     bool ok, skip = false;
@@ -190,21 +200,29 @@ __global__ void __launch_bounds__(256) q4_gather_kernel(const Q4GatherArgs a) {
       off = i - b * page;
       ok = blk < static_cast<uint32_t>(a.num_blocks);  // a negative id is a large one
     }
-    uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
-    if (ok) {
-      const uint8_t* tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
-      const int r = static_cast<int>(off % 16);
-      const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.k_codes(group, r) + 4 * (octet & 3)));
-      const uint32_t vw = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.v_codes(octet, r)));
-      const uint32_t ks = __ldg(tile + tl.k_scale(r, group)), vs = __ldg(tile + tl.v_scale(group, r));
-      k = q4_values(kw, ks, a.k_ts);
-      v = q4_values(vw, vs, a.v_ts);
-    } else if (octet == 0 && !skip) {
-      record_error(a.err, kErrBlock);
+    __nv_bfloat16* out = a.out + static_cast<int64_t>(i) * a.o_st + 8 * k;
+    if (!ok) {
+      if (k == 0 && !skip) record_error(a.err, kErrBlock);
+#pragma unroll
+      for (int j = 0; j < 2 * OCT; ++j) *reinterpret_cast<uint4*>(out + j * 8 * PER) = make_uint4(0u, 0u, 0u, 0u);
+      continue;
     }
-    __nv_bfloat16* out = a.out + static_cast<int64_t>(i) * a.o_st + 8 * octet;
-    *reinterpret_cast<uint4*>(out) = k;
-    *reinterpret_cast<uint4*>(out + W) = v;
+    const uint8_t* tile = a.cache + static_cast<int64_t>(blk) * a.c_sb + static_cast<int64_t>(off / 16) * tl.bytes();
+    const int r = static_cast<int>(off % 16);
+    uint32_t kw[OCT], vw[OCT], ks[OCT], vs[OCT];
+#pragma unroll
+    for (int j = 0; j < OCT; ++j) {
+      const int octet = k + j * PER;
+      kw[j] = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.k_codes(octet / 4, r) + 4 * (octet & 3)));
+      vw[j] = __ldg(reinterpret_cast<const uint32_t*>(tile + tl.v_codes(octet, r)));
+      ks[j] = __ldg(tile + tl.k_scale(r, octet / 4));
+      vs[j] = __ldg(tile + tl.v_scale(octet / 4, r));
+    }
+#pragma unroll
+    for (int j = 0; j < OCT; ++j) {
+      *reinterpret_cast<uint4*>(out + j * 8 * PER) = q4_values(kw[j], ks[j], a.k_ts, k_fold, k_ts2);
+      *reinterpret_cast<uint4*>(out + W + j * 8 * PER) = q4_values(vw[j], vs[j], a.v_ts, v_fold, v_ts2);
+    }
   }
 }
 
@@ -328,12 +346,14 @@ int hla_s6_gather_rows_q4(const void* cache, int64_t num_blocks, int64_t cache_s
   a.out = static_cast<__nv_bfloat16*>(out);
   a.o_st = out_stride;
   a.err = error_flag;
-  const int64_t per = 256 / (width / 8), want = (num_rows + per - 1) / per;
+  const int oct = num_rows >= kQ4GatherMany ? 4 : 1;
+  const int64_t per = 256 / (width / (8 * oct)), want = (num_rows + per - 1) / per;
   const int grid = static_cast<int>(std::min<int64_t>(want, 148 * 64));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (width == 256) q4_gather_kernel<256><<<grid, 256, 0, s>>>(a);
-  else if (width == 512) q4_gather_kernel<512><<<grid, 256, 0, s>>>(a);
-  else q4_gather_kernel<1024><<<grid, 256, 0, s>>>(a);
+  auto launch = [&](auto few, auto many) { (oct == 1 ? few : many)<<<grid, 256, 0, s>>>(a); };
+  if (width == 256) launch(q4_gather_kernel<256, 1>, q4_gather_kernel<256, 4>);
+  else if (width == 512) launch(q4_gather_kernel<512, 1>, q4_gather_kernel<512, 4>);
+  else launch(q4_gather_kernel<1024, 1>, q4_gather_kernel<1024, 4>);
   return cuda_status(cudaGetLastError(), "q4_gather_kernel launch");
 }
 

@@ -303,6 +303,20 @@ def test_commit_extreme_rows():
     assert got[5, W + 3] == 7 * 448 and got[5, W + 4] == -7 * 448 and (np.delete(got[5], [W + 3, W + 4]) == 0).all()
 
 
+def test_commit_tensor_scales_that_are_not_powers_of_two():
+    """3 / 8 and 5: steps of at most 7 significant bits, exact in fp32, so the codes are the formula's.  (No amax of 8
+    bits lies half way between two normal scales: 21 / 8 and 35 times an odd number of 5 bits has more than 8.)"""
+    q4 = pkg('q4')
+    c = commit_setup([70, 3], 512, 16, seed=4, start=[0, 9])
+    rotated = ref.rope(c['row'][:, :512], c['table'], c['pos'])
+    want = np.zeros((c['nb'], 1, 16, 544), dtype=np.uint8)
+    for t, s in enumerate(c['slots']):
+        ref.put_row(want, 512, 16, int(s), rotated[t], c['row'][t, 512:], 0.375, 5.0)
+    cache = dev(np.zeros_like(want))
+    q4.commit_rows(dev(c['row'], BF16), dev(c['pos']), dev(c['table'], BF16), cache, dev(c['bt']), dev(c['qsl']), 0.375, 5.0)
+    assert np.array_equal(cache.cpu().numpy(), want)
+
+
 def test_commit_skips_positions_without_a_block():
     q4 = pkg('q4')
     W, page = 256, 16
@@ -340,7 +354,7 @@ def test_commit_strided_rows_and_padded_blocks():
 
 
 @pytest.mark.parametrize('W,page,length', [(256, 16, 1), (256, 32, 33), (512, 16, 0), (512, 48, 100), (1024, 16, 250),
-                                           (512, 16, 16)])
+                                           (512, 16, 16), (256, 48, 4097), (512, 16, 4200), (1024, 16, 4111)])
 def test_gather_rows_is_exact(W, page, length):
     q4 = pkg('q4')
     rng = np.random.default_rng(length)
@@ -350,6 +364,19 @@ def test_gather_rows_is_exact(W, page, length):
     got = q4.gather_rows(dev(cache), dev(blocks), length, 0.5, 4.0).double().cpu().numpy()
     want = np.concatenate((k[blocks[:n]].reshape(-1, W)[:length] * 0.5, v[blocks[:n]].reshape(-1, W)[:length] * 4), 1)
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize('k_ts,v_ts', [(0.3, 7.0), (2.0 ** -120, 2.0 ** 110), (0.375, 2.0 ** -100)])
+def test_gather_tensor_scales(k_ts, v_ts):
+    """Any tensor scale: the exact (n - 8) s times the fp32 scale, rounded to fp32 and to bf16; in range, a power of two
+    of any size is exact."""
+    q4 = pkg('q4')
+    rng = np.random.default_rng(5)
+    cache, k, v = ref.random_cache(rng, 3, 16, 256)
+    got = q4.gather_rows(dev(cache), dev(np.array([2, 0], dtype=np.int32)), 30, k_ts, v_ts).double().cpu().numpy()
+    for half, x, ts in ((got[:, :256], k, k_ts), (got[:, 256:], v, v_ts)):
+        want = ref.bf16((x[[2, 0]].reshape(-1, 256)[:30].astype(np.float32) * np.float32(ts)).astype(np.float64))
+        assert np.array_equal(half, want)
 
 
 def test_gather_block_outside_the_cache():
