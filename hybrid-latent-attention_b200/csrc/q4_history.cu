@@ -25,16 +25,17 @@
 //               head only moves when a score passes it by 2^4 (a vote), so the output is rescaled rarely and the
 //               common step needs no reduction at all.  They also write the segment's output.
 //   warp 24, 25 one thread each issues the score and the value products.
-//   warp 26     bulk copies of whole tiles into a ring of 5 units of 34816 bytes (2, 4 or 8 tiles).
-// The dequantising loops are kept rolled: unrolled over a step they outgrew the instruction caches, and the warps
-// of a scheduler run different code (190 us unrolled with one group of each, 137 us rolled with a softmax group).
+//   warp 26, 27 bulk copies of the tiles' K and V halves into a ring each, of 5 units of 17408 bytes (2, 4 or 8 tiles):
+//               K is used a step or more before V, and in one ring of whole tiles its units waited for that.
+// Code size is what costs most after the arithmetic: the warps of a scheduler run different roles, whose loops share
+// its instruction caches.  The dequantising loops are kept rolled (unrolled over a step 190 us with one group of each,
+// 137 rolled with a softmax group; K by two chunks 99 instead of 91), and so are the issuing ones but for the MMAs of
+// one chunk (91 -> 85).
 //
-// Measured: 64 requests of 8160 rows, width 512: 91 us (3.15 TB/s, 188 TFLOP/s; the bytes alone 44); 4 of 65501:
-// 49 us (22); 37 of 0 to 16384, width 256: 28 us.  A step of 128 rows takes 6000 clocks and 14000 warp instructions,
-// 0.6 of the issue slots; without any dequantisation it would still take 4700, so what bounds it is the hand-over
-// between the roles (waits, barriers, instruction fetch) as much as the arithmetic.  Tried without a gain: two CTAs
-// of 13 warps (112 us), a ring each for K and V with a copy warp each (90.0 and 50.0 us), V chunks of two tiles (90.8
-// and 50.4), all on mma.sync (118).
+// Measured: 64 requests of 8160 rows, width 512: 79 us (3.6 TB/s, 215 TFLOP/s; the bytes alone 44); 4 of 65501: 45 us
+// (22); 37 of 0 to 16384, width 256: 27 us.  A step of 128 rows takes 5200 clocks and 14000 warp instructions; the
+// hand-over between the roles (waits, barriers, instruction fetch) bounds it as much as the arithmetic.  Without a
+// gain: two CTAs of 13 warps (112 us), all on mma.sync (118).
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
 // of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
 // 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
@@ -71,22 +72,25 @@ struct Q4HistoryParams {
 template <int W>
 struct Q4Cfg {
   static constexpr int NB = W / 128;             // blocks of 128 latent columns (output accumulators)
-  static constexpr int TILE = 17 * W;            // bytes of 16 rows
+  static constexpr int HALF = 17 * W / 2;        // bytes of a tile's K or V: codes [8 W], scales [W / 2]
+  static constexpr int SCALES = 8 * W;           // where the scales begin
   static constexpr int UT = 2048 / W;            // tiles per ring unit
-  static constexpr int UNIT = UT * TILE;         // 34816
+  static constexpr int UNIT = UT * HALF;         // 17408
   static constexpr int UNITS = 5;
-  static constexpr int VT = W == 256 ? 2 : 1;    // tiles per V chunk
+  // tiles per V chunk (width 512: with the rings apart 85.6, 80.3 and 79.4 us at 1, 2 and 4)
+  static constexpr int VT = W == 256 ? 2 : W == 512 ? 4 : 1;
   static constexpr int VCOLS = NB * VT * 8;      // its tensor-memory columns
-  static constexpr int BUFS = W == 1024 ? 2 : 4; // K chunks and V chunks in tensor memory
+  static constexpr int KB = 2;                   // K chunks in tensor memory (4 at width 256: no faster)
+  static constexpr int VB = W == 256 ? 4 : 2;    // V chunks
   static constexpr int Q_BYTES = 32 * W;
   static constexpr int P_BYTES = 2 * 4096;  // two steps
   // tensor-memory columns: K chunks (128 rows x 128 latent columns), V chunks, two score tiles, output
-  static constexpr uint32_t AK = 0, AV = AK + BUFS * 64, S = AV + BUFS * VCOLS, O = S + 32;
+  static constexpr uint32_t AK = 0, AV = AK + KB * 64, S = AV + VB * VCOLS, O = S + 32;
   static_assert(O + NB * 16 <= 512, "tensor memory");
-  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
+  static constexpr int SMEM = 1024 + Q_BYTES + P_BYTES + 2 * UNITS * UNIT + 1024;  // + 4 (T + 1) in stream mode
 };
 constexpr int kQSlots = 4;  // score factors of this many segments: the K warps run at most 3 segments ahead
-constexpr int kQ4HistThreads = 27 * 32;
+constexpr int kQ4HistThreads = 28 * 32;
 // log2 of how far a score may pass its head's exponent base before the base moves, and of the factor the
 // probabilities carry: together they end at 2^15, f16's largest power of two.  A small first term lets small
 // probabilities keep f16's precision, a large one makes rescales rare (each costs about one step).
@@ -142,7 +146,7 @@ __device__ __forceinline__ bool named_bar_or(int id, int threads, bool pred) {
 // The partition over the CTAs (stream mode) counts half steps: a row costs 2 a step of 128 rows and 1 for what its
 // segment takes to begin and end, and is only cut between steps (a cut one costs its CTAs a step each).  Cut at pages
 // and without that 1, short rows piled up in a CTA, up to 5 segments and 8 steps where 5 were due (37 rows of 0 to
-// 16384, width 256: 31 -> 25 us; 64 rows of 8160, width 512: 104 -> 97).
+// 16384, width 256: 35 -> 29 us; 64 rows of 8160, width 512: 102 -> 97).
 __device__ __forceinline__ int q4_cost(int ctx) { return ctx > 0 ? 2 * ((ctx - 1) / 128 + 1) + 1 : 0; }
 // The step at cost x of a row: a CTA that starts there begins with it, one that ends there ends before it.
 __device__ __forceinline__ int q4_step_at(int x) { return x > 0 ? (x - 1) >> 1 : 0; }
@@ -197,15 +201,18 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   uint8_t* qs = smem;
   uint8_t* ps = qs + C::Q_BYTES;
-  uint8_t* units = ps + C::P_BYTES;
-  uint8_t* ctl = units + C::UNITS * C::UNIT;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
-  uint64_t* empty = full + C::UNITS;                  // [UNITS] unit read
-  uint64_t* akf = empty + C::UNITS;                   // [BUFS] K chunk in tensor memory
-  uint64_t* ake = akf + C::BUFS;                      // [BUFS] its MMAs are done
-  uint64_t* avf = ake + C::BUFS;                      // [BUFS] V chunk
-  uint64_t* ave = avf + C::BUFS;
-  uint64_t* sf = ave + C::BUFS;                       // [2] scores of a step
+  uint8_t* k_units = ps + C::P_BYTES;
+  uint8_t* v_units = k_units + C::UNITS * C::UNIT;
+  uint8_t* ctl = v_units + C::UNITS * C::UNIT;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(ctl);  // [UNITS] unit copied
+  uint64_t* k_empty = k_full + C::UNITS;                // [UNITS] unit read
+  uint64_t* v_full = k_empty + C::UNITS;
+  uint64_t* v_empty = v_full + C::UNITS;
+  uint64_t* akf = v_empty + C::UNITS;                 // [KB] K chunk in tensor memory
+  uint64_t* ake = akf + C::KB;                        // [KB] its MMAs are done
+  uint64_t* avf = ake + C::KB;                        // [VB] V chunk
+  uint64_t* ave = avf + C::VB;
+  uint64_t* sf = ave + C::VB;                       // [2] scores of a step
   uint64_t* se = sf + 2;                              // [2] read
   uint64_t* qf = se + 2;                              // [kQSlots] score factors of a segment
   uint64_t* pf = qf + kQSlots;                        // [2] probabilities of a step written
@@ -213,7 +220,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   uint64_t* drain = pv + 2;                           // [2] every MMA of an issuer is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  float* qscale = reinterpret_cast<float*>(ctl + 384);  // [kQSlots][16] score factor of a head, by segment
+  float* qscale = reinterpret_cast<float*>(ctl + 512);  // [kQSlots][16] score factor of a head, by segment
   float* red = qscale + kQSlots * 16;                   // [2][4][8] per-warp maxima / sums
   int* pref = reinterpret_cast<int*>(ctl + 1024);       // [T + 1] (stream mode)
 
@@ -262,12 +269,16 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   if (warp == 24) tc::alloc(tmem_slot, 512);
   if (tid == 25 * 32) {
     for (int s = 0; s < C::UNITS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 8 + UT);  // the V warps, and the K warps of its tiles (one for two tiles in each group)
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], UT);  // the K warps of its tiles (one for two tiles in each group)
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 8);
     }
-    for (int b = 0; b < C::BUFS; ++b) {
+    for (int b = 0; b < C::KB; ++b) {
       mbar_init(&akf[b], 4);
       mbar_init(&ake[b], 1);
+    }
+    for (int b = 0; b < C::VB; ++b) {
       mbar_init(&avf[b], 4);
       mbar_init(&ave[b], 1);
     }
@@ -288,7 +299,6 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
   const tc::Waits wait{abort_flag, p.err, p.wait_ns};
-  const Q4Tile tl(W);
   const uint32_t sixteen = p.sixteen;
   Q4Walk st(p, pref, r0, p0, p1);
 
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     const int grp = warp >> 2, w = warp & 3;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
     const int u0 = 2 * w / UT, row = lane & 15;              // the unit of the step with this warp's two tiles
-    const int tile_off = (2 * w - u0 * UT + (lane >> 4)) * C::TILE;
+    const int tile_off = (2 * w - u0 * UT + (lane >> 4)) * C::HALF;
     int unit0 = 0;        // ring position of the step's first unit
     uint32_t chunk = 0;   // chunks before this step
     int seg = 0;
@@ -350,22 +360,22 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       }
       const int ring = (unit0 + u0) % C::UNITS;
       const bool unit_there = u0 * UT < st.n;
-      const uint8_t* tb = units + ring * C::UNIT + tile_off;
-      if (unit_there) wait(&full[ring], ((unit0 + u0) / C::UNITS) & 1, kErrWaitFull);
+      const uint8_t* tb = k_units + ring * C::UNIT + tile_off;
+      if (unit_there) wait(&k_full[ring], ((unit0 + u0) / C::UNITS) & 1, kErrWaitFull);
 #pragma unroll 1
       for (int kc = grp; kc < W / 128; kc += 2) {
-        const uint32_t c = chunk + kc, buf = c % C::BUFS;
-        wait(&ake[buf], ((c / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+        const uint32_t c = chunk + kc, buf = c % C::KB;
+        wait(&ake[buf], ((c / C::KB) & 1) ^ 1, kErrWaitEmpty);
         __syncwarp();
         tc::fence_after();
-        const uint32_t sc = *reinterpret_cast<const uint32_t*>(tb + tl.k_scale(row, 4 * kc));
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(tb + C::SCALES + row * (W / 32) + 4 * kc);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           Q4ScaleH s[2];
           q4_scales_h((sc >> (16 * hf)) & 0xffffu, s[0], s[1]);
 #pragma unroll
           for (int gi = 0; gi < 2; ++gi) {
-            const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.k_codes(4 * kc + 2 * hf + gi, row));
+            const uint4 x = *reinterpret_cast<const uint4*>(tb + (4 * kc + 2 * hf + gi) * 256 + row * 16);
             uint32_t v[16];
             q4_word_h(x.x, s[gi], sixteen, v[0], v[1], v[2], v[3]);
             q4_word_h(x.y, s[gi], sixteen, v[4], v[5], v[6], v[7]);
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         __syncwarp();
         if (lane == 0) mbar_arrive(&akf[buf]);
       }
-      if (lane == 0 && unit_there) mbar_arrive(&empty[ring]);
+      if (lane == 0 && unit_there) mbar_arrive(&k_empty[ring]);
       unit0 += (st.n + UT - 1) / UT;
       chunk += W / 128;
     }
@@ -394,21 +404,21 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     while (st.next()) {
       for (int ut = 0; ut < st.n; ut += UT, ++unit) {
         const int ring = unit % C::UNITS;
-        const uint8_t* ub = units + ring * C::UNIT;
-        wait(&full[ring], (unit / C::UNITS) & 1, kErrWaitFull);
+        const uint8_t* ub = v_units + ring * C::UNIT;
+        wait(&v_full[ring], (unit / C::UNITS) & 1, kErrWaitFull);
         const int tiles = min(UT, st.n - ut);
 #pragma unroll 1
         for (int t0 = ((chunk + ut / C::VT) & 1) == grp ? 0 : C::VT; t0 < tiles; t0 += 2 * C::VT) {
           // chunks alternate between the groups over all steps, so that a buffer always belongs to the same group:
           // a group that met a buffer's barrier out of turn could take an older phase for the one it waits for
-          const uint32_t ch = chunk + (ut + t0) / C::VT, buf = ch % C::BUFS;
-          wait(&ave[buf], ((ch / C::BUFS) & 1) ^ 1, kErrWaitEmpty);
+          const uint32_t ch = chunk + (ut + t0) / C::VT, buf = ch % C::VB;
+          wait(&ave[buf], ((ch / C::VB) & 1) ^ 1, kErrWaitEmpty);
           __syncwarp();
           tc::fence_after();
 #pragma unroll 1
           for (int ti = 0; ti < C::VT && t0 + ti < tiles; ++ti) {
-            const uint8_t* tb = ub + (t0 + ti) * C::TILE;
-            uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + tl.v_scale(col0 >> 5, 4 * c));
+            const uint8_t* tb = ub + (t0 + ti) * C::HALF;
+            uint32_t sb = *reinterpret_cast<const uint32_t*>(tb + C::SCALES + (col0 >> 5) * 16 + 4 * c);
             // rows past the context get a zero scale, whatever their bytes are
             if (st.last) {
               const int valid = st.ctx - ((st.tile + ut + t0 + ti) << 4) - 4 * c;
@@ -422,7 +432,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
               uint32_t v[8 * OH][2];  // [column][rows 4c, 4c+1 | 4c+2, 4c+3]
 #pragma unroll
               for (int oc = 0; oc < OH; ++oc) {
-                const uint4 x = *reinterpret_cast<const uint4*>(tb + tl.v_codes((col0 >> 3) + o0 + oc, 4 * c));
+                const uint4 x = *reinterpret_cast<const uint4*>(tb + ((col0 >> 3) + o0 + oc) * 64 + 16 * c);
                 uint32_t (*d)[2] = v + 8 * oc;
                 q4_word_h(__byte_perm(x.x, x.y, 0x5410), s01, sixteen, d[0][0], d[2][0], d[4][0], d[6][0]);
                 q4_word_h(__byte_perm(x.x, x.y, 0x7632), s01, sixteen, d[1][0], d[3][0], d[5][0], d[7][0]);
@@ -446,7 +456,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
           __syncwarp();
           if (lane == 0) mbar_arrive(&avf[buf]);
         }
-        if (lane == 0) mbar_arrive(&empty[ring]);
+        if (lane == 0) mbar_arrive(&v_empty[ring]);
       }
       chunk += (st.n + C::VT - 1) / C::VT;
     }
@@ -620,10 +630,10 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         }
         if (i >= 2) wait(&se[i & 1], ((i >> 1) - 1) & 1, kErrWaitEmpty);
         const uint32_t d = tmem + C::S + (i & 1) * 16;
-#pragma unroll
+#pragma unroll 1
         for (int kc = 0; kc < W / 128; ++kc, ++c) {
-          const uint32_t buf = c % C::BUFS;
-          wait(&akf[buf], (c / C::BUFS) & 1, kErrWaitFull);
+          const uint32_t buf = c % C::KB;
+          wait(&akf[buf], (c / C::KB) & 1, kErrWaitFull);
           tc::fence_after();
           const uint32_t a = tmem + C::AK + buf * 64;
 #pragma unroll
@@ -645,11 +655,11 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
         wait(&pf[i & 1], (i >> 1) & 1, kErrWaitFull);
         const uint64_t pd = tc::desc_sw128(smem_u32(ps) + (i & 1) * 4096);
         const uint32_t keep = !st.first;
-#pragma unroll
+#pragma unroll 1
         for (int t0 = 0; t0 < 8; t0 += C::VT, ++c) {
           if (t0 >= st.n) break;
-          const uint32_t buf = c % C::BUFS;
-          wait(&avf[buf], (c / C::BUFS) & 1, kErrWaitFull);
+          const uint32_t buf = c % C::VB;
+          wait(&avf[buf], (c / C::VB) & 1, kErrWaitFull);
           tc::fence_after();
           const uint32_t a = tmem + C::AV + buf * C::VCOLS;
 #pragma unroll
@@ -669,11 +679,16 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       if (!mbar_wait(&drain[1], 0, p.wait_ns)) record_error(p.err, kErrWaitFull);
     }
   } else {
-    // ------------------------------------------------------------------ tile copies
+    // ------------------------------------------------------------------ copies: warp 26 K, warp 27 V
     // codes are read once: evicted from L2 first, so that the partials and the combine's operands stay
     const uint64_t policy = l2_policy_evict_first();
+    const bool is_v = warp == 27;
+    uint8_t* units = is_v ? v_units : k_units;
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    const Q4Tile tl(W);
+    const int codes_at = is_v ? tl.v_codes(0, 0) : 0, scales_at = is_v ? tl.v_scale(0, 0) : tl.k_scale(0, 0);
     // The lanes look up 32 tiles at once: a lookup per unit, when its slot was free, kept this warp busy for longer
-    // than the others took to use the unit up (64 x 8160 rows: 95 -> 91 us).
+    // than the others took to use the unit up (64 x 8160 rows, then in one ring: 95 -> 91 us).
     int unit = 0;
     while (st.next()) {
       for (int b = st.tile; b < st.tend; b += 32) {
@@ -686,22 +701,25 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
             blk = -1;
           }
         }
-        const uint8_t* src = p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * C::TILE;
+        const uint8_t* src = p.cache + static_cast<int64_t>(blk) * p.c_sb + static_cast<int64_t>(t - lp * p.tpp) * tl.bytes();
         const unsigned absent = __ballot_sync(0xffffffffu, t < st.tend && blk < 0);
         for (int k = 0; k < 32 && b + k < st.tend; k += UT, ++unit) {
           const int ring = unit % C::UNITS, n = min(UT, st.tend - b - k);
           const bool mine = lane >= k && lane < k + n;
           if (unit >= C::UNITS) wait(&empty[ring], ((unit / C::UNITS) - 1) & 1, kErrWaitEmpty);
           __syncwarp();
-          uint8_t* dst = units + ring * C::UNIT + (lane - k) * C::TILE;
+          uint8_t* dst = units + ring * C::UNIT + (lane - k) * C::HALF;
           if (mine && blk < 0) {  // a page outside the table or the cache reads as zeros
-            for (int o = 0; o < C::TILE; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
+            for (int o = 0; o < C::HALF; o += 16) *reinterpret_cast<uint4*>(dst + o) = make_uint4(0u, 0u, 0u, 0u);
             fence_proxy_async();
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc((absent >> k) & ((1u << n) - 1u))) * C::TILE);
+          if (lane == 0) mbar_arrive_expect_tx(&full[ring], (n - __popc((absent >> k) & ((1u << n) - 1u))) * C::HALF);
           __syncwarp();
-          if (mine && blk >= 0) tc::bulk_load(dst, src, C::TILE, &full[ring], policy);
+          if (mine && blk >= 0) {
+            tc::bulk_load(dst, src + codes_at, C::SCALES, &full[ring], policy);
+            tc::bulk_load(dst + C::SCALES, src + scales_at, C::HALF - C::SCALES, &full[ring], policy);
+          }
         }
       }
       st.n = st.tend - st.tile;  // the segment's steps are all taken
