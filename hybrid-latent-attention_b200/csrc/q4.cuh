@@ -20,6 +20,8 @@
 namespace hla {
 
 constexpr int kQ4Group = 32;  // columns that share a scale
+constexpr uint32_t kQ4ScaleNaN = 0x7f;         // e4m3's NaN: the scale of a group that holds one
+constexpr uint32_t kQ4Zeros = 0x88888888u;     // a word of codes 8
 
 // A packed weight [N, K] is [N / 16][K / 128] tiles (zero padded) of 16 rows x 128 columns: codes
 // [2][32 lanes][16 B], scales [32 lanes][2], lane 4 g + c and half h holding row 8 h + g, columns 32 c .. -
@@ -50,6 +52,13 @@ __device__ __forceinline__ uint32_t bf2_fma(uint32_t a, uint32_t b, uint32_t c) 
 __device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// The larger value, or NaN where one is NaN (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 
@@ -126,7 +135,7 @@ __device__ __forceinline__ float q4_scale_value(uint32_t byte) {
 }
 // Codes of a group whose step is s * ts: 8 + x / step rounded to nearest, ties to even, clamped to 1..15 (by
 // clamping x to 7 steps: |x| / step < 7.5 except where the scale saturated or was rounded in e4m3's subnormal range).
-// An infinity takes the group's largest code, a NaN code 1 (the stored rows hold no NaN); a step of 0 gives 8.
+// An infinity takes the group's largest code; a step of 0 gives 8.  (Groups with a NaN take kQ4ScaleNaN and kQ4Zeros.)
 // No division: z = x * inv + 1.5 * 2^23 + 8 has the rounded sum in its low bits.  inv = 1 / step is itself rounded, so
 // where x / step is (almost) half way z may have gone the wrong way; the remainder x - q step, exact for power-of-two
 // tensor scales (8 bits minus 3 x 4 bits), tells: more than half a step, or half a step from an odd code, moves the

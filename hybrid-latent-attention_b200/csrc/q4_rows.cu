@@ -18,23 +18,25 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
 }
 
 // Quantise 8 columns of a group whose 32 columns sit in 4 neighbouring lanes: the word, and the scale byte
-// (the same in the 4 lanes).
+// (the same in the 4 lanes).  The maximum carries a NaN on, and a group that holds one takes the scale NaN.
 __device__ __forceinline__ uint32_t quantize8(const float (&f)[8], float ts, uint32_t& scale) {
   float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
-  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+  for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(f[i]));
+  a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+  a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+  const bool number = a == a;
   if (q4_pow2(ts)) {
-    scale = q4_scale_byte_pow2(a, ts);
-    return q4_word_pow2(f, a, q4_scale_value(scale) * ts);
+    scale = number ? q4_scale_byte_pow2(a, ts) : kQ4ScaleNaN;
+    const uint32_t w = q4_word_pow2(f, a, q4_scale_value(scale) * ts);
+    return number ? w : kQ4Zeros;
   }
-  scale = q4_scale_byte(a, ts);
+  scale = number ? q4_scale_byte(a, ts) : kQ4ScaleNaN;
   const Q4Coder code(q4_scale_value(scale) * ts);
   uint32_t n[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) n[i] = code(f[i]);
-  return q4_word(n);
+  return number ? q4_word(n) : kQ4Zeros;
 }
 
 struct Q4CommitArgs {

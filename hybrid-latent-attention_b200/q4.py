@@ -14,8 +14,8 @@ column instead of 4 (544 bytes for a 512-wide latent, bf16 2048), weights of 17/
                          ``LatentLayer.pack_writers``
 
 Format: a group of 32 consecutive columns shares one e4m3 scale ``s``; a value is ``(n - 8) * s * ts`` with a
-code ``n`` in 1..15 and one tensor scale ``ts``: ``s = e4m3(amax / (7 ts))``, ``n = 8 + rint(x / (s ts))``.  The
-byte layout is in include/hla_s6.h.  The tensor scales (``k_scale`` / ``v_scale`` of a cache, ``scale`` of a
+code ``n`` in 1..15 and one tensor scale ``ts``: ``s = e4m3(amax / (7 ts))``, ``n = 8 + rint(x / (s ts))``.  An
+infinity takes the largest code of its group; a group that holds a NaN reads back as NaN throughout.  The byte layout is in include/hla_s6.h.  The tensor scales (``k_scale`` / ``v_scale`` of a cache, ``scale`` of a
 weight) are not stored with the codes: every call on the same data passes the same values.  A scale covers groups
 with amax between 0.11 ts and 3136 ts at full precision; ``tensor_scale`` picks one.
 
@@ -225,7 +225,8 @@ def weight_tiles(out_features, in_features):
 
 def quantize_weight(weight, scale=None):
     """``(packed, scale)`` of a bf16 weight ``[N, K]``, K a multiple of 32.  ``scale`` defaults to
-    ``tensor_scale`` of its largest value (which reads it back: call this once, at load time)."""
+    ``tensor_scale`` of its largest value (which reads it back: call this once, at load time; a weight with values
+    that are not finite is then refused)."""
     if weight.dim() != 2 or weight.dtype is not BF16 or weight.stride(-1) != 1:
         raise ValueError('weight must be bf16 [N, K] with a unit last-dim stride')
     N, K = weight.shape

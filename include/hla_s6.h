@@ -427,7 +427,8 @@ int hla_s6_export_rows(const void* const* main_caches, const void* const* l1_cac
  * A group of 32 consecutive columns shares one e4m3 scale s; a value is (n - 8) * s * ts with a code n
  * in 1..15 and one tensor scale ts > 0 (k_scale, v_scale of a cache; scale of a weight).  Quantising:
  * s = e4m3(amax / (7 ts)), saturated at 448; n = 8 + rint(x / (s ts)) clamped to 1..15; a group whose
- * scale rounds to 0 stores zeros.  Codes travel in 32-bit words of 8 columns: nibble i holds column 2i,
+ * scale rounds to 0 stores zeros.  An infinity takes its group's largest code; a group that holds a NaN gets
+ * the scale NaN (0x7f), so all of it reads back as NaN.  Codes travel in 32-bit words of 8 columns: nibble i holds column 2i,
  * nibble i + 4 column 2i + 1.
  *
  * A 4-bit latent cache is uint8 [num_blocks, 1, page, 17 * width / 16], width 256, 512 or 1024, page a
@@ -458,9 +459,8 @@ int hla_s6_history_partials_q4(const void* q_lat, int64_t q_stride_t, int64_t q_
                                int* error_flag, int32_t flags, void* stream);
 
 /* hla_s6_commit_rows into a 4-bit cache: the K half latent-RoPE'd in the torch bf16 order, then both halves
- * quantised.  Padding tokens and tokens without a slot in the cache are skipped (slot_out -1).  Infinite
- * values take their group's largest code.  Two tokens of one call must not share a slot.  row and table rows
- * 16-byte aligned, max_blocks * page < 2^31. */
+ * quantised.  Padding tokens and tokens without a slot in the cache are skipped (slot_out -1).  Two tokens
+ * of one call must not share a slot.  row and table rows 16-byte aligned, max_blocks * page < 2^31. */
 int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, const int64_t* positions,
                           const void* table, int64_t table_stride, int64_t max_position, void* cache,
                           int64_t num_blocks, int64_t cache_stride_block, int32_t page, const int32_t* block_table,
