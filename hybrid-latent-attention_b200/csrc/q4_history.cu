@@ -580,10 +580,13 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
       const bool room = st.slot < p.slots_cap;
       if (!room && lane == 0) record_error(p.err, kErrSlots);
       if (room && w == 0) {
+        // A partial that is NaN says so by an lse of +inf: the reduces and the combine drop a NaN from their maximum and
+        // would take a row of such partials alone for one without history; +inf outweighs the others, as exp(inf - inf).
+        // (fminf drops it too; as a comparison and a choice this cost 1.2 us of 80 in registers.)
 #pragma unroll
         for (int h = 0; h < 8; ++h)
           if (lane == h && h0 + h < p.H)
-            p.ws_lse[static_cast<int64_t>(st.slot) * p.H + h0 + h] = (mm[h] + log2f(t[h])) * 0.6931471805599453f;
+            p.ws_lse[static_cast<int64_t>(st.slot) * p.H + h0 + h] = fminf((mm[h] + log2f(t[h])) * 0.6931471805599453f, INFINITY);
       }
 #pragma unroll
       for (int h = 0; h < 8; ++h) t[h] = t[h] == 0.f ? 0.f : p.v_ts / t[h];  // 0: every score is -inf

@@ -125,6 +125,7 @@ def history_attention(q_lat, cache, block_table, ctx, scale, num_kv_splits, work
                       empty=None, error_flag=None):
     """``s6_ops.history_attention`` over a 4-bit cache: ``(o [T, H, W] bf16, lse [H, T] fp32)`` of the softmax of
     ``q_lat [T, H, W]`` over the first ``ctx[t]`` rows; empty rows give ``o = 0``, ``lse = -inf``.
+    A NaN in a query or in a key makes the rows that meet it NaN, ``lse`` too.
     ``error_flag`` (int32 [1], optional) receives 5 for a block-table entry outside the cache."""
     stride = q_lat.stride()
     if len(stride) != 3 or q_lat.dtype is not BF16 or stride[2] != 1:

@@ -1,5 +1,5 @@
-"""The 4-bit operators (``q4``) where a mistake would hide: not-a-number and infinities in rows and weights.  The
-references are q4_reference's.
+"""The 4-bit operators (``q4``) where a mistake would hide: not-a-number and infinities in rows, weights and
+queries.  The references are q4_reference's; the bounds are counted as in test_q4_gpu.
 """
 import numpy as np
 import pytest
@@ -7,7 +7,7 @@ import torch
 
 import q4_reference as ref
 from conftest import pkg
-from test_q4_gpu import BF16, bf, commit_setup, dev
+from test_q4_gpu import CUDA, BF16, History, bf, commit_setup, dev
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,101 @@ def test_a_nan_in_a_weight_is_kept(T):
     assert torch.isfinite(y[:, keep]).all()
     clean, _ = q4.quantize_weight(dev(np.nan_to_num(w), BF16), 0.0078125)
     assert torch.equal(y[:, keep], q4.linear(dev(x, BF16), clean, N, scale)[:, keep])
+
+
+# ------------------------------------------------------------------------------------ the reader and values not finite
+def check_but(h, o, lse, touched):
+    """``History.check`` with the (token, head) pairs of ``touched`` taken from a run with the queries ``h.q``."""
+    clean_o, clean_lse = h.run(q=dev(h.q, BF16))
+    for t, hd in touched:
+        o[t, hd], lse[hd, t] = clean_o[t, hd], clean_lse[hd, t]
+    h.check(o, lse)
+
+
+@pytest.mark.parametrize('ctxs,splits', [([40], 64), ([5000], 64), ([900, 0, 17], 1), ([300] * 20 + [0, 1], 16)])
+@pytest.mark.parametrize('W', [256, 512])
+def test_history_nan_in_a_query_stays_in_its_head(W, ctxs, splits):
+    """A NaN query is a NaN row, one partial or many; rows without history are empty all the same."""
+    h = History(ctxs, W=W, seed=7)
+    touched = [(t, hd) for t, hd in ((0, 3), (0, 12), (len(ctxs) - 1, 0), (1, 5)) if t < len(ctxs)]
+    for t, hd in touched:
+        h.qd[t, hd, 9 * hd] = float('nan')
+    o, lse = h.run(splits=splits)
+    for t, hd in touched:
+        if ctxs[t]:
+            assert torch.isnan(o[t, hd]).all() and torch.isnan(lse[hd, t]), (t, hd)
+        else:
+            assert (o[t, hd] == 0).all() and torch.isneginf(lse[hd, t])
+    check_but(h, o, lse, touched)
+
+
+@pytest.mark.parametrize('splits', [1, 64])
+def test_history_infinite_queries(splits):
+    """Scores of +inf make a NaN row, as in exp(s - max) of the formula; a row whose scores are all -inf is empty."""
+    ctxs = [200, 1500, 70]
+    h = History(ctxs, W=256, seed=3)
+    flat = h.cache.reshape(-1).cpu().numpy().copy()
+    codes = ref.tile_views(flat, 256)[0][:, 0, :, 0]
+    codes[:] = (codes & 0xf0) | 3                                # column 0 of every key: code 3, below zero
+    h.cache.copy_(dev(flat).view(h.cache.shape))
+    k, _ = ref.unpack_cache(h.cache.cpu().numpy(), 256)
+    for t, n in enumerate(ctxs):
+        rows = k[h.table[t, :-(-n // 16)]].reshape(-1, 256)[:n] * h.k_ts
+        assert (rows[:, 0] < 0).all()
+        h.rows[t] = (rows, h.rows[t][1])
+    touched = [(0, 2), (1, 9), (1, 0), (2, 15)]
+    for (t, hd), v in zip(touched, (np.inf, np.inf, -np.inf, -np.inf)):
+        h.qd[t, hd, 0] = v
+    o, lse = h.run(splits=splits)
+    for t, hd in ((0, 2), (1, 9)):
+        assert (o[t, hd] == 0).all() and torch.isneginf(lse[hd, t]), (t, hd)
+    for t, hd in ((1, 0), (2, 15)):
+        assert torch.isnan(o[t, hd]).all() and torch.isnan(lse[hd, t]), (t, hd)
+    check_but(h, o, lse, touched)
+
+
+@pytest.mark.parametrize('ctxs,splits', [([40, 64], 64), ([3000, 500], 64), ([700, 130], 1)])
+def test_history_nan_in_a_cached_row_stays_in_its_request(ctxs, splits):
+    """A NaN key makes its request's rows NaN in every head, a NaN group of a value row that group's columns."""
+    W = 512
+    h = History(ctxs, W=W, seed=2)
+    clean = h.run(splits=splits)
+    at = ctxs[0] // 2
+    flat = h.cache.reshape(-1).cpu().numpy().copy()
+    views = ref.tile_views(flat, W)
+    tile, r = h.table[0, at // 16], at % 16
+    old = views[3][tile, 4, r]
+    views[3][tile, 4, r] = 0x7f                                 # V columns 128 .. 159
+    h.cache.copy_(dev(flat).view(h.cache.shape))
+    o, lse = h.run(splits=splits)
+    assert torch.isnan(o[0, :, 128:160]).all() and torch.equal(lse, clean[1])
+    keep = torch.tensor([c for c in range(W) if not 128 <= c < 160], device=CUDA)
+    assert torch.equal(o[0][:, keep], clean[0][0][:, keep]) and torch.equal(o[1], clean[0][1])
+    views[3][tile, 4, r] = old
+    views[2][tile, r, 15] = 0x7f                                # K columns 480 .. 511
+    h.cache.copy_(dev(flat).view(h.cache.shape))
+    o, lse = h.run(splits=splits)
+    assert torch.isnan(o[0]).all() and torch.isnan(lse[:, 0]).all()
+    assert torch.equal(o[1], clean[0][1]) and torch.equal(lse[:, 1], clean[1][:, 1])
+
+
+def test_attend_keeps_a_nan_query_in_its_head():
+    """Through the fused combine: NaN in that head of that token, every other output bit as before."""
+    from test_q4_chain_gpu import Layer
+    lay = pkg('s6_layer')
+    layer = Layer(16, 256, 512, 256, 32, 16, seed=21)
+    layer.run([(0, 60), (1, 100)])
+    ctx, *_ = layer.step([(0, 1), (1, 1)])
+    T, H, loop = 2, 16, 1
+    q, v = layer.rnd(T, H, 128), layer.rnd(T, H, 128)
+    exact = torch.nan_to_num(layer.caches.exact[loop]).transpose(1, 2)
+    q_lat = layer.rnd(T, H, 512, std=0.5)
+    call = lambda: lay.attend(layer.sl, loop, q_lat, q, None, v, layer.caches.main, layer.caches.latent_table,  # noqa: E731
+                              *layer.caches.main_scale, ctx, (exact, layer.caches.exact_table))
+    was = call()
+    assert torch.isfinite(was).all()
+    q_lat[1, 6, 100] = float('nan')
+    got = call()
+    assert torch.isnan(got[1, 6]).all()
+    got[1, 6] = was[1, 6]
+    assert torch.equal(got, was)
