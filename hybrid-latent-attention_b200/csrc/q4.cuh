@@ -55,10 +55,15 @@ __device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
   return d;
 }
 
-// The larger value, or NaN where one is NaN (fmaxf drops it).
+// The largest value, or NaN where one is NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -137,9 +142,9 @@ __device__ __forceinline__ float q4_scale_value(uint32_t byte) {
 // clamping x to 7 steps: |x| / step < 7.5 except where the scale saturated or was rounded in e4m3's subnormal range).
 // An infinity takes the group's largest code; a step of 0 gives 8.  (Groups with a NaN take kQ4ScaleNaN and kQ4Zeros.)
 // No division: z = x * inv + 1.5 * 2^23 + 8 has the rounded sum in its low bits.  inv = 1 / step is itself rounded, so
-// where x / step is (almost) half way z may have gone the wrong way; the remainder x - q step, exact for power-of-two
-// tensor scales (8 bits minus 3 x 4 bits), tells: more than half a step, or half a step from an odd code, moves the
-// code by one towards it.
+// where x / step is (almost) half way z may have gone the wrong way; the remainder x - q step tells: more than half a
+// step, or half a step from an odd code, moves the code by one towards it.  (fmaf rounds the remainder once; it is exact
+// where ts has up to 17 significant bits: 8 bits minus 3 x 4 x 17.)
 struct Q4Coder {
   float step, inv, lim;
   uint32_t half;  // bits of step / 2
@@ -165,8 +170,8 @@ __device__ __forceinline__ uint32_t q4_word(const uint32_t (&n)[8]) {
   for (int i = 0; i < 4; ++i) w |= (n[2 * i] << (4 * i)) | (n[2 * i + 1] << (16 + 4 * i));
   return w;
 }
-// Scale byte and codes of bf16 values for a power-of-two tensor scale (2^-124 .. 2^123), without divisions and in 6
-// instructions a value instead of 16:
+// Scale byte and codes of bf16 values for a power-of-two tensor scale (2^-117 .. 2^116: the smallest step, 2^-9 ts, is a
+// normal number and 7 of the largest, 448 ts, are finite), without divisions and in 6 instructions a value instead of 16:
 // * amax / 7 has at most 5 significant bits where it is half way between two e4m3 numbers, and is otherwise 2^-11 or
 //   more away from that, relative; so amax * (1 / 7), right to 2^-23, is rounded to 16 bits and falls as the quotient.
 // * a quotient of 8 by 4 significant bits that is not half way between two integers is at least 1/1000 away from that,
@@ -175,7 +180,13 @@ __device__ __forceinline__ uint32_t q4_word(const uint32_t (&n)[8]) {
 // amax: the group's largest value, which says whether anything has to be clamped (see above).
 __device__ __forceinline__ bool q4_pow2(float ts) {
   const uint32_t b = __float_as_uint(ts);
-  return (b & 0x7fffffu) == 0 && b - (3u << 23) <= (247u << 23);
+  return (b & 0x7fffffu) == 0 && b - (10u << 23) <= (233u << 23);
+}
+// Any other (normal) tensor scale: values and scale are multiplied by the power of two that puts the scale into [1, 4),
+// which changes no code; steps, reciprocals and remainders then stay among fp32's normal numbers.
+__device__ __forceinline__ float q4_norm(float ts) {
+  const uint32_t e = __float_as_uint(ts) >> 23;
+  return __uint_as_float((254u - (e < 253u ? e : 253u)) << 23);
 }
 __device__ __forceinline__ uint32_t q4_scale_byte_pow2(float amax, float ts) {
   const float seventh = __uint_as_float(__float_as_uint(1.f / 7.f) + (127u << 23) - __float_as_uint(ts));  // 1 / (7 ts)

@@ -20,23 +20,30 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
 // Quantise 8 columns of a group whose 32 columns sit in 4 neighbouring lanes: the word, and the scale byte
 // (the same in the 4 lanes).  The maximum carries a NaN on, and a group that holds one takes the scale NaN.
 __device__ __forceinline__ uint32_t quantize8(const float (&f)[8], float ts, uint32_t& scale) {
-  float a = 0.f;
+  float a = max_nan(fabsf(f[0]), fabsf(f[1]));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max_nan(a, fabsf(f[i]));
+  for (int i = 2; i < 8; i += 2) a = max_nan(a, fabsf(f[i]), fabsf(f[i + 1]));
   a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
   a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-  const bool number = a == a;
+  uint32_t w;
   if (q4_pow2(ts)) {
-    scale = number ? q4_scale_byte_pow2(a, ts) : kQ4ScaleNaN;
-    const uint32_t w = q4_word_pow2(f, a, q4_scale_value(scale) * ts);
-    return number ? w : kQ4Zeros;
-  }
-  scale = number ? q4_scale_byte(a, ts) : kQ4ScaleNaN;
-  const Q4Coder code(q4_scale_value(scale) * ts);
-  uint32_t n[8];
+    scale = q4_scale_byte_pow2(a, ts);
+    w = q4_word_pow2(f, a, q4_scale_value(scale) * ts);
+  } else {
+    const float norm = q4_norm(ts);
+    ts *= norm;
+    scale = q4_scale_byte(a * norm, ts);
+    const Q4Coder code(q4_scale_value(scale) * ts);
+    uint32_t n[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = code(f[i]);
-  return number ? q4_word(n) : kQ4Zeros;
+    for (int i = 0; i < 8; ++i) n[i] = code(f[i] * norm);
+    w = q4_word(n);
+  }
+  if (a != a) {
+    scale = kQ4ScaleNaN;
+    w = kQ4Zeros;
+  }
+  return w;
 }
 
 struct Q4CommitArgs {
@@ -265,6 +272,13 @@ static bool q4_ts_ok(float a, float b, const char* what) {
   set_error("%s: tensor scales must be positive and finite", what);
   return false;
 }
+// To quantise with, a tensor scale is a normal number too.
+static bool q4_ts_normal(float a, float b, const char* what) {
+  if (!q4_ts_ok(a, b, what)) return false;
+  if (a >= 0x1p-126f && b >= 0x1p-126f) return true;
+  set_error("%s: tensor scales below 2^-126 cannot be quantised with", what);
+  return false;
+}
 
 }  // namespace hla
 
@@ -279,7 +293,7 @@ int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, 
                           int32_t num_reqs, int32_t num_tokens, float k_scale, float v_scale, int64_t* slot_out,
                           void* stream) {
   if (!q4_cache_ok(cache, cache_stride_block, width, page, "commit rows (4 bit)") ||
-      !q4_ts_ok(k_scale, v_scale, "commit rows (4 bit)"))
+      !q4_ts_normal(k_scale, v_scale, "commit rows (4 bit)"))
     return kStatusInvalid;
   if (num_tokens < 0 || num_reqs < 1 || max_position < 1 || table_stride < width || max_blocks < 0 ||
       static_cast<int64_t>(max_blocks) * page >= (int64_t(1) << 31) || (table_stride % 8) ||
@@ -366,7 +380,7 @@ int hla_s6_quantize_weight_q4(const void* weight, int64_t weight_stride_n, int32
     set_error("quantize weight (4 bit) needs in_features %% 32 == 0, 1..1048560 out_features and 16-byte aligned rows");
     return kStatusInvalid;
   }
-  if (!q4_ts_ok(scale, scale, "quantize weight (4 bit)")) return kStatusInvalid;
+  if (!q4_ts_normal(scale, scale, "quantize weight (4 bit)")) return kStatusInvalid;
   q4_weight_kernel<<<dim3((in_features + 127) / 128, (out_features + 15) / 16), 256, 0,
                      static_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(weight), weight_stride_n,
                                                           out_features, in_features, scale,

@@ -48,8 +48,10 @@ def cache_width(cache):
 
 def tensor_scale(amax):
     """The smallest power of two that lets the largest group scale reach e4m3's range for values up to ``amax``
-    (a float); a power of two keeps every stored value exact in bf16."""
-    return 2.0 ** math.ceil(math.log2(amax / (7 * 448))) if amax > 0 else 1.0
+    (a float), from 2^-126 on; a power of two keeps every stored value exact in bf16."""
+    if not math.isfinite(amax):
+        raise ValueError(f'the largest value must be finite (got {amax})')
+    return 2.0 ** math.ceil(math.log2(max(amax / (7 * 448), 2.0 ** -126))) if amax > 0 else 1.0
 
 
 def new_cache(num_blocks, page, width, device='cuda'):

@@ -428,7 +428,7 @@ int hla_s6_export_rows(const void* const* main_caches, const void* const* l1_cac
  * in 1..15 and one tensor scale ts > 0 (k_scale, v_scale of a cache; scale of a weight).  Quantising:
  * s = e4m3(amax / (7 ts)), saturated at 448; n = 8 + rint(x / (s ts)) clamped to 1..15; a group whose
  * scale rounds to 0 stores zeros.  An infinity takes its group's largest code; a group that holds a NaN gets
- * the scale NaN (0x7f), so all of it reads back as NaN.  Codes travel in 32-bit words of 8 columns: nibble i holds column 2i,
+ * the scale NaN (0x7f), so all of it reads back as NaN.  To quantise with, ts is at least 2^-126.  Codes travel in 32-bit words of 8 columns: nibble i holds column 2i,
  * nibble i + 4 column 2i + 1.
  *
  * A 4-bit latent cache is uint8 [num_blocks, 1, page, 17 * width / 16], width 256, 512 or 1024, page a

@@ -58,6 +58,16 @@ def test_sizes_and_scales(q4):
             q4.new_cache(*bad, device='cpu')
 
 
+def test_tensor_scale_at_its_ends(q4):
+    """Never below fp32's smallest normal number, which is the least a row can be quantised with."""
+    for amax in (5e-324, 1e-40, 1e-38, 3136 * 2.0 ** -126):
+        assert q4.tensor_scale(amax) == 2.0 ** -126
+    assert q4.tensor_scale(3136 * 2.0 ** -126 * 1.001) == 2.0 ** -125
+    for amax in (float('nan'), float('inf')):
+        with pytest.raises(ValueError, match='finite'):
+            q4.tensor_scale(amax)
+
+
 def test_geometry_check_takes_4_bit_caches(q4):
     geo = pkg('geometry')
     rec = geo.check_latent_caches({512: q4.new_cache(5, 48, 512, 'cpu'), 256: torch.zeros(5, 1, 16, 512, dtype=BF16)})
@@ -240,6 +250,14 @@ def test_rows_entry_refusals(lib):
     refused(lib, 'hla_s6_gather_rows_q4', base, shared + [
         (dict(slots=A16), 'gather'), (dict(blocks=None), 'gather'), (dict(n=-1), 'gather'), (dict(n=1 << 31), 'gather'),
         (dict(out=A8), 'gather'), (dict(o_st=1028), 'gather'), (dict(o_st=1016), 'gather')])
+
+
+def test_entries_that_quantise_refuse_scales_below_the_normal_numbers(lib):
+    base = dict(row=A16, st=1024, W=512, pos=A16, table=A16, tab_st=512, max_pos=64, cache=A16, nb=4, sb=16 * 544,
+                page=16, bt=A16, bt_st=3, cols=3, qsl=A16, R=2, T=3, ks=1.0, vs=1.0, slots=None, stream=None)
+    refused(lib, 'hla_s6_commit_rows_q4', base, [(dict(ks=2.0 ** -127), '2^-126'), (dict(vs=1e-45), '2^-126')])
+    base = dict(w=A16, st=64, N=16, K=64, scale=2.0 ** -130, packed=A16, stream=None)
+    refused(lib, 'hla_s6_quantize_weight_q4', base, [(dict(), '2^-126')])
 
 
 def test_linear_entry_refusals(lib):

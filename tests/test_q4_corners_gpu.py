@@ -1,5 +1,6 @@
 """The 4-bit operators (``q4``) where a mistake would hide: not-a-number and infinities in rows, weights and
-queries.  The references are q4_reference's; the bounds are counted as in test_q4_gpu.
+queries, and tensor scales at either end of fp32.  The references are q4_reference's; the bounds are counted as in
+test_q4_gpu.
 """
 import numpy as np
 import pytest
@@ -161,3 +162,56 @@ def test_attend_keeps_a_nan_query_in_its_head():
     assert torch.isnan(got[1, 6]).all()
     got[1, 6] = was[1, 6]
     assert torch.equal(got, was)
+
+
+# ------------------------------------------------------------------------------------ tensor scales at either end
+@pytest.mark.parametrize('ts', [2.0 ** -126, 2.0 ** -124, 2.0 ** -119, 2.0 ** -118, 2.0 ** -117, 2.0 ** -100, 2.0 ** 100,
+                                2.0 ** 115, 2.0 ** 116, 2.0 ** 117, 2.0 ** 120, 2.0 ** 123, 2.0 ** 126, 2.0 ** 127,
+                                1.5 * 2.0 ** -125, 1.5 * 2.0 ** 126])
+def test_commit_at_the_ends_of_the_tensor_scales(ts):
+    """Codes and scales are the formula's for every tensor scale, infinities included.  (1.5: exact as 3 / 8 is.)"""
+    q4 = pkg('q4')
+    W = 256
+    c = commit_setup([24], W, 16, seed=1)
+    rng = np.random.default_rng(int(np.log2(ts)) & 255)
+    spread = np.exp2(rng.integers(-14, 13, (24, 2 * W // 32))).repeat(32, 1)
+    with np.errstate(over='ignore'):
+        x = torch.from_numpy(np.clip(rng.standard_normal((24, 2 * W)) * spread * ts, -3e38, 3e38)).to(BF16).double().numpy()
+    assert np.isfinite(x).all()
+    x[3, W:] = 0
+    x[5, W + 3], x[5, W + 4] = np.inf, -np.inf
+    x[6, :W // 2] = 0
+    x[6, 1] = -np.inf
+    c['table'][:, :W // 2], c['table'][:, W // 2:] = 1, 0       # the identity rotation
+    x[:, W // 2:W] = 0                                          # (inf * 0 of a partner would be NaN)
+    key = x[:, :W].copy()
+    key[6, W // 2 + 1] = np.nan
+    want = np.zeros((c['nb'], 1, 16, 17 * W // 16), dtype=np.uint8)
+    for t, s in enumerate(c['slots']):
+        ref.put_row(want, W, 16, int(s), np.nan_to_num(key[t], nan=0.0, posinf=np.inf, neginf=-np.inf), x[t, W:], ts, ts)
+    cache = dev(np.zeros_like(want))
+    q4.commit_rows(dev(x, BF16), dev(c['pos']), dev(c['table'], BF16), cache, dev(c['bt']), dev(c['qsl']), ts, ts)
+    got = cache.cpu().numpy()
+    slot = int(c['slots'][6])                                   # the partner's group holds a NaN: not compared here
+    for a in (got, want):
+        views = ref.tile_views(a[slot // 16].reshape(-1), W)
+        views[0][:, (W // 2 + 1) // 32, slot % 16] = 0
+        views[2][:, slot % 16, (W // 2 + 1) // 32] = 0
+    np.testing.assert_array_equal(got, want)
+    if 2.0 ** -110 < ts < 2.0 ** 110:                           # (beyond, values leave bf16's range)
+        back = q4.gather_slots(dev(want), dev(c['slots']), ts, ts).double().cpu().numpy()
+        np.testing.assert_array_equal(back[:, W:], ref.stored(x[:, W:], ts))
+
+
+@pytest.mark.parametrize('amax', [1e-38, 3e-36, 3.3e38])
+def test_weights_of_tiny_and_huge_values(amax):
+    """``quantize_weight`` picks its scale: the packed values are the formula's and within half a step of the weight."""
+    q4 = pkg('q4')
+    rng = np.random.default_rng(0)
+    w = torch.from_numpy(rng.uniform(-amax, amax, (48, 160))).to(BF16)
+    packed, scale = q4.quantize_weight(w.to(CUDA))
+    n, b = ref.quantize(w.double().numpy(), scale)
+    got = ref.unpack_weight(packed.cpu().numpy(), 48, 160)
+    np.testing.assert_array_equal(got, (n - 8) * np.repeat(ref.E4M3[b], 32, -1))
+    err = np.abs(got * scale - w.double().numpy()).reshape(48, -1, 32)
+    assert (err <= np.abs(w.double().numpy()).reshape(48, -1, 32).max(-1, keepdims=True) / 7 * (1 + 2.0 ** -4) / 2).all()
