@@ -13,7 +13,7 @@ import torch
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get('HLA_S6_LIB', _PKG / 'libhla_s6.so'))
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 OK, EINVAL, EOVERFLOW, ECUDA = 0, 1, 2, 3
 # codes a kernel writes to its optional device error word (HLA_S6_ERR_*)
@@ -81,6 +81,7 @@ SIGNATURES = {
     'hla_s6_gather_rows_q4': [P, _i64, _i64, _i32, _i32, P, P, _i64, _f32, _f32, P, _i64, P, P],
     'hla_s6_quantize_weight_q4': [P, _i64, _i32, _i32, _f32, P, P],
     'hla_s6_linear_q4': [P, _i64, P, _i32, _i32, _i32, _f32, P, _i64, P, _i64, P],
+    'hla_s6_linear_q4_checked': [P, _i64, P, _i32, _i32, _i32, _f32, P, _i64, P, _i64, P, P],
     'hla_s6_chunk_attention': [P, _i64, _i64, P, _i64, _i64, P, _i64, _i64, P, _i32, _i32, _i32, _i32, _f32, P, _i64,
                                _i64, P, P],
 }

@@ -37,6 +37,7 @@ struct Q4LinearParams {
   int64_t o_st;
   int vec;    // out (and residual) rows are 16-byte aligned
   int split;  // CTAs of a cluster that share a tile's K (many tokens)
+  int* err;   // error word or NULL
   uint64_t wait_ns;
 };
 
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
-  const tc::Waits wait{abort_flag, nullptr, p.wait_ns};
+  const tc::Waits wait{abort_flag, p.err, p.wait_ns};
 
   if (warp < DQ) {
     // lane: row 8 half + g of a 16-row tile, columns 32 c .. of the stage's 64
@@ -319,14 +320,16 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
   } else if (warp == DQ) {
     if (lane == 0) {
       prefetch_tmap(&tmap_x);
-      for (int kb = 0; kb < NK; ++kb) {
+      int kb = 0;
+      for (; kb < NK; ++kb) {
         const int s = kb % C::STAGES;
-        if (kb >= C::STAGES) wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty);
+        if (kb >= C::STAGES && !wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty)) break;
         mbar_arrive_expect_tx(&full[s], C::A_BYTES);
         tma_load_rows(smem + s * C::STAGE, &tmap_x, &full[s], (kfirst + kb) * 64, m0);  // rows and columns past x are zeros
       }
       // the last copies land before the CTA ends, also when a wait has given up
-      for (int kb = max(0, NK - C::STAGES); kb < NK; ++kb) mbar_wait(&full[kb % C::STAGES], (kb / C::STAGES) & 1, p.wait_ns);
+      for (int u = max(0, kb - C::STAGES); u < kb; ++u)
+        mbar_wait(&full[u % C::STAGES], (u / C::STAGES) & 1, p.wait_ns);
     }
   } else if (tc::elect()) {
     for (int kb = 0; kb < NK; ++kb) {
@@ -409,7 +412,7 @@ __global__ void __launch_bounds__(320, 1) q4_linear_wide_kernel(const __grid_con
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;  // columns: the output's 256 tokens, then a stage's 64 weight columns each
-  const tc::Waits wait{abort_flag, nullptr, p.wait_ns};
+  const tc::Waits wait{abort_flag, p.err, p.wait_ns};
 
   if (warp < 8) {
     const int grp = warp >> 2, w = warp & 3, row = 32 * w + lane;
@@ -512,24 +515,27 @@ __global__ void __launch_bounds__(320, 1) q4_linear_wide_kernel(const __grid_con
   } else if (warp == 8) {
     if (lane == 0) {
       prefetch_tmap(&tmap_x);
-      for (int kb = 0; kb < NK; ++kb) {
+      int kb = 0;
+      for (; kb < NK; ++kb) {
         const int s = kb % S;
-        if (kb >= S) wait(&empty[s], ((kb / S) - 1) & 1, kErrWaitEmpty);
+        if (kb >= S && !wait(&empty[s], ((kb / S) - 1) & 1, kErrWaitEmpty)) break;
         mbar_arrive_expect_tx(&x_full[s], kWideStage);  // rows and columns past x are zeros
         tma_load_rows(smem + s * kWideStage, &tmap_x, &x_full[s], kb * 64, m0);
         tma_load_rows(smem + s * kWideStage + kWideStage / 2, &tmap_x, &x_full[s], kb * 64, m0 + 128);
       }
       // the last copies land before the CTA ends, also when a wait has given up
-      for (int kb = max(0, NK - S); kb < NK; ++kb) mbar_wait(&x_full[kb % S], (kb / S) & 1, p.wait_ns);
+      for (int u = max(0, kb - S); u < kb; ++u)
+        mbar_wait(&x_full[u % S], (u / S) & 1, p.wait_ns);
     }
   } else if (tc::elect()) {
     uint32_t phase = 0;
-    for (int kb0 = 0; kb0 < NK; kb0 += S, phase ^= 1) {
+    bool go = true;
+    for (int kb0 = 0; kb0 < NK && go; kb0 += S, phase ^= 1) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (kb0 + s >= NK) break;
-        wait(&a_full[s], phase, kErrWaitFull);
-        wait(&x_full[s], phase, kErrWaitFull);
+        go = wait(&a_full[s], phase, kErrWaitFull) && wait(&x_full[s], phase, kErrWaitFull);
+        if (!go) break;
         tc::fence_after();
         const uint64_t xd = tc::desc_sw128(smem_u32(smem + s * kWideStage));
 #pragma unroll
@@ -586,9 +592,9 @@ using namespace hla;
 
 extern "C" {
 
-int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens, int32_t out_features,
-                     int32_t in_features, float scale, const void* residual, int64_t residual_stride_t, void* out,
-                     int64_t out_stride_t, void* stream) {
+int hla_s6_linear_q4_checked(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens,
+                             int32_t out_features, int32_t in_features, float scale, const void* residual,
+                             int64_t residual_stride_t, void* out, int64_t out_stride_t, int* error_flag, void* stream) {
   if (num_tokens < 0 || out_features < 1 || out_features > 16 * 65535 || in_features < 32 || in_features % 32 ||
       (x_stride_t % 8) || (reinterpret_cast<uintptr_t>(x) % 16) || (reinterpret_cast<uintptr_t>(packed) % 16)) {
     set_error("linear (4 bit) needs in_features %% 32 == 0, 1..1048560 out_features and 16-byte aligned x rows and "
@@ -618,7 +624,8 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
   p.o_st = out_stride_t;
   auto a16 = [](const void* q, int64_t st) { return (reinterpret_cast<uintptr_t>(q) % 16) == 0 && st % 8 == 0; };
   p.vec = a16(out, out_stride_t) && (!residual || a16(residual, residual_stride_t));
-  p.wait_ns = wait_limit_ns();
+  p.err = error_flag;
+  p.wait_ns = std::max(wait_limit_ns(), tc::kLeastWaitNs);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Few tokens: tiles of 16 outputs x 8 tokens.  One token tile: two row tiles a CTA once there are enough CTAs (1 x 2048
   // -> 12288 5.0 us instead of 5.3; -> 6144 4.7 instead of 4.3).
@@ -640,6 +647,13 @@ int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int3
   p.split = 1;
   while (p.split < 8 && tiles * p.split * 2 <= 148 && (in_features + 63) / 64 >= 8 * p.split) p.split *= 2;
   return launch_many(p, s);
+}
+
+int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens, int32_t out_features,
+                     int32_t in_features, float scale, const void* residual, int64_t residual_stride_t, void* out,
+                     int64_t out_stride_t, void* stream) {
+  return hla_s6_linear_q4_checked(x, x_stride_t, packed, num_tokens, out_features, in_features, scale, residual,
+                                  residual_stride_t, out, out_stride_t, nullptr, stream);
 }
 
 }  // extern "C"

@@ -94,9 +94,15 @@ __device__ __forceinline__ void st_16x256(uint32_t a, uint32_t r0, uint32_t r1, 
   asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(r0), "r"(r1), "r"(r2), "r"(r3));
 }
 
-// Bounded waits of a CTA's roles.  The first that runs out records `code` and raises the shared abort flag;
-// from then on every wait of the CTA returns at once, so each role still takes all its steps (the barriers that
-// count arrivals stay in step, nothing leaves a loop early) and the CTA ends with wrong values and an error code.
+// The least limit of these kernels' waits.  They wait for nothing but their own copies and products, which take
+// microseconds: when a wait runs out after this long, what was in flight has landed (the GPU ran something else
+// meanwhile) or never will.  With a shorter limit a CTA could end before its copies.
+constexpr uint64_t kLeastWaitNs = 100 * 1000 * 1000;
+
+// Bounded waits of a CTA's roles.  The first that runs out records `code` in the error word and raises the shared abort
+// flag; from then on every wait of the CTA returns, with false where its phase has not completed.  The roles take all
+// their steps all the same (the barriers that count arrivals stay in step, nothing leaves a loop early), but a role that
+// issues copies stops at the first false; the CTA ends with wrong values and an error code.
 struct Waits {
   int* abort_flag;  // shared memory, zeroed
   int* err;
@@ -116,19 +122,20 @@ struct Waits {
         : "memory");
     return ok != 0;
   }
-  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity, int code) const {
-    if (!attempt(bar, parity)) retry(bar, parity, code);
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity, int code) const {
+    return attempt(bar, parity) || retry(bar, parity, code);
   }
-  __device__ __noinline__ void retry(uint64_t* bar, uint32_t parity, int code) const {
+  __device__ __noinline__ bool retry(uint64_t* bar, uint32_t parity, int code) const {
     const uint64_t t0 = global_ns();
     while (!attempt(bar, parity)) {
-      if (aborted()) return;
+      if (aborted()) return false;
       if (global_ns() - t0 > limit_ns) {
         record_error(err, code);
         atomicExch(abort_flag, 1);
-        return;
+        return false;
       }
     }
+    return true;
   }
 };
 

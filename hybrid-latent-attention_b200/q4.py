@@ -251,10 +251,11 @@ def _check_rows(y, T, N):
         raise ValueError(f'residual and out must be bf16 [{T}, {N}] with a unit last-dim stride')
 
 
-def linear(x, packed, out_features, scale, residual=None, out=None):
+def linear(x, packed, out_features, scale, residual=None, out=None, error_flag=None):
     """``bf16(scale * x . w^T + residual)`` for ``x [T, K]`` bf16 and the packed weight ``[N, K]``: fp32 sums, one
     rounding.  ``residual`` and ``out`` are bf16 ``[T, N]``; ``out`` may be ``residual``, and overlaps no other input.
-    Rows of x start at 16-byte boundaries."""
+    Rows of x start at 16-byte boundaries.  ``error_flag`` (int32 [1], optional) receives 1 or 2 where a kernel's wait
+    ran out, whose output is then wrong."""
     stride = x.stride()
     if len(stride) != 2 or x.dtype is not BF16 or stride[1] != 1:
         raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
@@ -271,13 +272,14 @@ def linear(x, packed, out_features, scale, residual=None, out=None):
         _check_rows(residual, T, N)
     if out is not None:
         _check_rows(out, T, N)
-    index = _device_of(x, packed, residual, out)
+    _check_flag(error_flag)
+    index = _device_of(x, packed, residual, out, error_flag)
     fresh = out is None
     if fresh:
         out = x.new_empty(T, N)
-    _launch(index, 'hla_s6_linear_q4', x.data_ptr(), x_stride, packed.data_ptr(), T, N, K, float(scale),
+    _launch(index, 'hla_s6_linear_q4_checked', x.data_ptr(), x_stride, packed.data_ptr(), T, N, K, float(scale),
             _address(residual), 0 if residual is None else residual.stride(0), out.data_ptr(),
-            N if fresh else out.stride(0))
+            N if fresh else out.stride(0), _address(error_flag))
     return out
 
 
@@ -295,5 +297,5 @@ class Weight:
         packed, scale = quantize_weight(weight, scale)
         return cls(packed, weight.shape[0], scale)
 
-    def linear(self, x, residual=None, out=None):
-        return linear(x, self.packed, self.out_features, self.scale, residual, out)
+    def linear(self, x, residual=None, out=None, error_flag=None):
+        return linear(x, self.packed, self.out_features, self.scale, residual, out, error_flag)

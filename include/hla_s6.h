@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 5
+#define HLA_S6_ABI_VERSION 6
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1
 #define HLA_S6_EOVERFLOW 2
@@ -58,7 +58,8 @@ const char* hla_s6_last_error(void);
 /* Limit, in nanoseconds of device time, of every bounded wait in the kernels launched after this
  * call (mbarrier phases of the TMA rings, the sequence-split combine's wait for the other GPUs'
  * parts): when it runs out the kernel writes its error code to error_flag and returns.
- * Process-wide; 0 restores the default of 2 s.  A CUDA graph keeps the limit its launches were
+ * Process-wide; 0 restores the default of 2 s.  hla_s6_linear_q4 takes 100 ms for a shorter limit (its kernels wait
+ * for nothing but their own copies and products).  A CUDA graph keeps the limit its launches were
  * captured with.  Returns the previous limit.  No counterpart in the reference (its Triton and
  * FA2 kernels never wait on another agent). */
 uint64_t hla_s6_set_wait_limit_ns(uint64_t ns);
@@ -491,6 +492,11 @@ int hla_s6_quantize_weight_q4(const void* weight, int64_t weight_stride_n, int32
 int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens, int32_t out_features,
                      int32_t in_features, float scale, const void* residual, int64_t residual_stride_t, void* out,
                      int64_t out_stride_t, void* stream);
+
+/* The same with an error word: 1 or 2 where a wait of a kernel ran out, and out is then wrong. */
+int hla_s6_linear_q4_checked(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens,
+                             int32_t out_features, int32_t in_features, float scale, const void* residual,
+                             int64_t residual_stride_t, void* out, int64_t out_stride_t, int* error_flag, void* stream);
 
 #ifdef __cplusplus
 }

@@ -191,6 +191,21 @@ def test_linear_refusals(q4):
         q4.quantize_weight(torch.zeros(16, 64, dtype=BF16))
 
 
+def test_linear_takes_an_error_word(q4, lib):
+    """The kernels' bounded waits have somewhere to report to: ``linear``, ``Weight.linear`` and the C entry behind them."""
+    x, w = torch.zeros(3, 160, dtype=BF16), torch.zeros(2, 2, 1088, dtype=U8)
+    for bad in (torch.zeros(1, dtype=I64), torch.zeros(0, dtype=I32)):
+        with pytest.raises(ValueError, match='error_flag must be int32'):
+            q4.linear(x, w, 20, 1.0, error_flag=bad)
+        with pytest.raises(ValueError, match='error_flag must be int32'):
+            q4.Weight(w, 20, 1.0).linear(x, error_flag=bad)
+    with pytest.raises(ValueError, match='CUDA'):
+        q4.linear(x, w, 20, 1.0, error_flag=torch.zeros(1, dtype=I32))
+    base = dict(x=A16, st=2048, w=A16, T=3, N=64, K=2048, scale=1.0, res=None, r_st=0, out=A16, o_st=64, err=A16,
+                stream=None)
+    refused(lib, 'hla_s6_linear_q4_checked', base, [(dict(T=-1), 'linear'), (dict(o_st=63), 'linear')])
+
+
 def test_callers_refuse_mixed_and_misnamed_caches(q4):
     ce, oa = pkg('cache_export'), pkg('ouro_attention')
     four, two = q4.new_cache(4, 16, 512, 'cpu'), torch.zeros(4, 1, 16, 512, dtype=BF16)

@@ -365,6 +365,17 @@ def test_linear_large_tiles_with_few_tokens(T, N, K, residual):
     test_linear(T, N, K, residual)
 
 
+@pytest.mark.parametrize('T,N', [(3, 256), (20, 256), (40, 1200), (130, 256), (300, 2000), (1030, 2001)])
+def test_linear_leaves_the_error_word_alone(T, N):
+    """Every kernel with an error word: nothing in it after a call that went well, and the same output."""
+    q4 = pkg('q4')
+    rng = np.random.default_rng(T)
+    w = q4.Weight.of(dev(bf(rng, N, 512), BF16))
+    x = dev(bf(rng, T, 512), BF16)
+    flag = torch.zeros(1, dtype=torch.int32, device=CUDA)
+    assert torch.equal(w.linear(x, error_flag=flag), w.linear(x)) and flag.item() == 0
+
+
 @pytest.mark.parametrize('share,W', [([18000, 1, 950], 512), ([37000, 0, 900, 7], 256)])
 def test_commit_of_a_prompt_at_the_usual_widths(share, W):
     """Enough tokens for several rows a thread, at the widths of the two latents; rows nobody commits stay."""
