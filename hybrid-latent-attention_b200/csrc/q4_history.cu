@@ -763,7 +763,7 @@ static int launch_q4(const HistoryArgs& a, const HistoryPlan& plan, float v_ts, 
   p.stream_mode = plan.stream_mode;
   p.sixteen = 16;
   p.err = a.err;
-  p.wait_ns = wait_limit_ns();
+  p.wait_ns = std::max(wait_limit_ns(), tc::kLeastWaitNs);
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

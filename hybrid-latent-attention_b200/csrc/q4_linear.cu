@@ -320,16 +320,14 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
   } else if (warp == DQ) {
     if (lane == 0) {
       prefetch_tmap(&tmap_x);
-      int kb = 0;
-      for (; kb < NK; ++kb) {
+      for (int kb = 0; kb < NK; ++kb) {
         const int s = kb % C::STAGES;
-        if (kb >= C::STAGES && !wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty)) break;
+        if (kb >= C::STAGES) wait(&empty[s], ((kb / C::STAGES) - 1) & 1, kErrWaitEmpty);
         mbar_arrive_expect_tx(&full[s], C::A_BYTES);
         tma_load_rows(smem + s * C::STAGE, &tmap_x, &full[s], (kfirst + kb) * 64, m0);  // rows and columns past x are zeros
       }
       // the last copies land before the CTA ends, also when a wait has given up
-      for (int u = max(0, kb - C::STAGES); u < kb; ++u)
-        mbar_wait(&full[u % C::STAGES], (u / C::STAGES) & 1, p.wait_ns);
+      for (int kb = max(0, NK - C::STAGES); kb < NK; ++kb) mbar_wait(&full[kb % C::STAGES], (kb / C::STAGES) & 1, p.wait_ns);
     }
   } else if (tc::elect()) {
     for (int kb = 0; kb < NK; ++kb) {
@@ -515,27 +513,24 @@ __global__ void __launch_bounds__(320, 1) q4_linear_wide_kernel(const __grid_con
   } else if (warp == 8) {
     if (lane == 0) {
       prefetch_tmap(&tmap_x);
-      int kb = 0;
-      for (; kb < NK; ++kb) {
+      for (int kb = 0; kb < NK; ++kb) {
         const int s = kb % S;
-        if (kb >= S && !wait(&empty[s], ((kb / S) - 1) & 1, kErrWaitEmpty)) break;
+        if (kb >= S) wait(&empty[s], ((kb / S) - 1) & 1, kErrWaitEmpty);
         mbar_arrive_expect_tx(&x_full[s], kWideStage);  // rows and columns past x are zeros
         tma_load_rows(smem + s * kWideStage, &tmap_x, &x_full[s], kb * 64, m0);
         tma_load_rows(smem + s * kWideStage + kWideStage / 2, &tmap_x, &x_full[s], kb * 64, m0 + 128);
       }
       // the last copies land before the CTA ends, also when a wait has given up
-      for (int u = max(0, kb - S); u < kb; ++u)
-        mbar_wait(&x_full[u % S], (u / S) & 1, p.wait_ns);
+      for (int kb = max(0, NK - S); kb < NK; ++kb) mbar_wait(&x_full[kb % S], (kb / S) & 1, p.wait_ns);
     }
   } else if (tc::elect()) {
     uint32_t phase = 0;
-    bool go = true;
-    for (int kb0 = 0; kb0 < NK && go; kb0 += S, phase ^= 1) {
+    for (int kb0 = 0; kb0 < NK; kb0 += S, phase ^= 1) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (kb0 + s >= NK) break;
-        go = wait(&a_full[s], phase, kErrWaitFull) && wait(&x_full[s], phase, kErrWaitFull);
-        if (!go) break;
+        wait(&a_full[s], phase, kErrWaitFull);
+        wait(&x_full[s], phase, kErrWaitFull);
         tc::fence_after();
         const uint64_t xd = tc::desc_sw128(smem_u32(smem + s * kWideStage));
 #pragma unroll

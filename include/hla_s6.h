@@ -58,8 +58,8 @@ const char* hla_s6_last_error(void);
 /* Limit, in nanoseconds of device time, of every bounded wait in the kernels launched after this
  * call (mbarrier phases of the TMA rings, the sequence-split combine's wait for the other GPUs'
  * parts): when it runs out the kernel writes its error code to error_flag and returns.
- * Process-wide; 0 restores the default of 2 s.  hla_s6_linear_q4 takes 100 ms for a shorter limit (its kernels wait
- * for nothing but their own copies and products).  A CUDA graph keeps the limit its launches were
+ * Process-wide; 0 restores the default of 2 s.  The 4-bit reader and linear take 100 ms for a shorter limit (their
+ * kernels wait for nothing but their own copies and products).  A CUDA graph keeps the limit its launches were
  * captured with.  Returns the previous limit.  No counterpart in the reference (its Triton and
  * FA2 kernels never wait on another agent). */
 uint64_t hla_s6_set_wait_limit_ns(uint64_t ns);
