@@ -184,6 +184,7 @@ __device__ __forceinline__ void store16(const Q4LinearParams& p, int t, int n, f
   }
 }
 
+// Called by whole warps (the forms that are not aligned take 0.5 us longer).
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
@@ -343,6 +344,7 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
     tc::commit(done);
     mbar_wait(done, 0, p.wait_ns);
   }
+  if (warp >= DQ) __syncwarp();  // one lane's branch ends
   if (p.split > 1) {
     // the cluster's CTAs hold a part of the sum each; CTA k adds up and writes every split-th row from k
     cluster_sync();
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__((Q4Many::DQ + 2) * 32) q4_linear_many_kernel(
         p.out[static_cast<int64_t>(t) * p.o_st + n + e] = __float2bfloat16_rn(v[e] * p.ts + rs);
       }
     }
+    __syncwarp();
     cluster_sync();  // no CTA's memory goes before the others have read it
   }
   tc::fence_before();
