@@ -9,6 +9,7 @@ reference student state dict loads strictly.  All arithmetic on them runs in the
 from __future__ import annotations
 
 import math
+from dataclasses import replace
 
 import torch
 from torch import nn
@@ -37,9 +38,15 @@ class LatentLayer(nn.Module):
 
     def pack_writers(self):
         """From now on ``s6_layer.write_rows`` runs on 4-bit copies of the writers' weights (``packed_writers``, by
-        loop), made here (on CUDA, bf16).  ``writer`` and the state dict stay as they are; a copy is not made again
-        when its parameter changes."""
+        loop), made here (on CUDA, bf16).  ``writer`` and the state dict stay as they are; a copy moves with the
+        module but is not made again when its parameter changes."""
         self.packed_writers = [q4.Weight.of(w.weight.detach()) for w in (self.cand1, *self.cand_s)]
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.packed_writers is not None:
+            self.packed_writers = [replace(w, packed=fn(w.packed)) for w in self.packed_writers]
+        return self
 
     def readers(self, loop):
         """``(A, B, width)`` of a loop: loop 0 reads the loop-1 latent, later loops the main latent."""

@@ -206,6 +206,21 @@ def test_linear_takes_an_error_word(q4, lib):
     refused(lib, 'hla_s6_linear_q4_checked', base, [(dict(T=-1), 'linear'), (dict(o_st=63), 'linear')])
 
 
+def test_packed_writers_move_with_their_module(q4):
+    """``.to`` of a layer, and of what holds it, takes the packed copies along; their bytes keep their type."""
+    lat = pkg('latent')
+    layer = lat.LatentLayer(64, 2, 128, 3, 256, 256, 256)
+    shapes = [(512, 64)] * 3
+    layer.packed_writers = [q4.Weight(torch.zeros(q4.weight_tiles(*s), dtype=U8), s[0], 0.5) for s in shapes]
+    torch.nn.ModuleList([layer]).to('meta', BF16)
+    assert layer.cand1.weight.device.type == 'meta' and layer.cand1.weight.dtype is BF16
+    assert len(layer.packed_writers) == 3
+    for w, s in zip(layer.packed_writers, shapes):
+        assert w.packed.device.type == 'meta' and w.packed.dtype is U8 and w.packed.shape == q4.weight_tiles(*s)
+        assert w.out_features == s[0] and w.scale == 0.5
+    assert not any('packed' in name for name in layer.state_dict())
+
+
 def test_callers_refuse_mixed_and_misnamed_caches(q4):
     ce, oa = pkg('cache_export'), pkg('ouro_attention')
     four, two = q4.new_cache(4, 16, 512, 'cpu'), torch.zeros(4, 1, 16, 512, dtype=BF16)
