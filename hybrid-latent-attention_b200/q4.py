@@ -164,7 +164,7 @@ def commit_rows(row, positions, table, cache, block_table, query_start_loc, k_sc
     pos % page``.  Returns the slots (int64 [T]); padding tokens (``t >= query_start_loc[-1]``) and positions
     without a block in the cache are skipped, their slot is -1.  Two tokens of one call must not share a slot."""
     stride = row.stride()
-    if len(stride) != 2 or row.dtype is not BF16 or stride[1] != 1:
+    if len(stride) != 2 or row.dtype is not BF16 or stride[1] != 1 or row.shape[1] & 1:
         raise ValueError('row must be bf16 [T, 2 * width] with a unit last-dim stride')
     T, W = row.shape
     W //= 2

@@ -141,6 +141,12 @@ def test_commit_refusals(q4, kw, match):
         q4.commit_rows(**commit_args(**kw))
 
 
+def test_commit_refuses_rows_of_an_odd_width(q4):
+    """A column more than K and V have is no row of this cache, though half of it rounds to its width."""
+    with pytest.raises(ValueError, match='row must be bf16'):
+        q4.commit_rows(**commit_args(row=torch.zeros(3, 1032, dtype=BF16)[:, :1025]))
+
+
 def test_gather_refusals(q4):
     cache = q4.new_cache(4, 16, 256, 'cpu')
     blocks, slots = torch.zeros(2, dtype=I32), torch.zeros(5, dtype=I64)
