@@ -599,6 +599,10 @@ int hla_s6_linear_q4_checked(const void* x, int64_t x_stride_t, const void* pack
               "weight");
     return kStatusInvalid;
   }
+  if (num_tokens > 65535 * kWideTokens) {
+    set_error("linear (4 bit): at most %d tokens (got %d)", 65535 * kWideTokens, num_tokens);
+    return kStatusInvalid;
+  }
   if (out_stride_t < out_features && num_tokens > 1) {
     set_error("linear (4 bit): output rows overlap (stride %lld)", static_cast<long long>(out_stride_t));
     return kStatusInvalid;

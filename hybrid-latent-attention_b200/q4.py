@@ -33,6 +33,7 @@ from . import _lib
 
 GROUP = 32
 WEIGHT_TILE_BYTES = 1088   # HLA_S6_Q4_WEIGHT_TILE_BYTES
+LINEAR_TOKENS = 65535 * 256   # the most tokens of one linear (a grid of tiles of 256)
 BF16, U8, I32, I64 = torch.bfloat16, torch.uint8, torch.int32, torch.int64
 
 
@@ -260,6 +261,8 @@ def linear(x, packed, out_features, scale, residual=None, out=None, error_flag=N
     if len(stride) != 2 or x.dtype is not BF16 or stride[1] != 1:
         raise ValueError('x must be bf16 [T, K] with a unit last-dim stride')
     T, K = x.shape
+    if T > LINEAR_TOKENS:
+        raise ValueError(f'a 4-bit linear takes at most {LINEAR_TOKENS} tokens, got {T}')
     N = out_features
     if (packed.dtype is not U8 or packed.shape != (-(-N // 16), -(-K // 128), WEIGHT_TILE_BYTES)
             or not packed.is_contiguous()):

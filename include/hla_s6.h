@@ -487,7 +487,7 @@ int hla_s6_quantize_weight_q4(const void* weight, int64_t weight_stride_n, int32
                               float scale, void* packed, void* stream);
 
 /* out[t, n] = bf16(scale * sum_k x[t, k] w[n, k] + residual[t, n]) with a packed 4-bit weight; residual
- * (bf16, may be NULL) and out have unit last strides, out may be residual.  The 4-bit form of
+ * (bf16, may be NULL) and out have unit last strides, out may be residual.  At most 65535 * 256 tokens.  The 4-bit form of
  * hla_s6_writer_project and of the adapter's QKV / output projections (ouro_latent.py:109-110, 130). */
 int hla_s6_linear_q4(const void* x, int64_t x_stride_t, const void* packed, int32_t num_tokens, int32_t out_features,
                      int32_t in_features, float scale, const void* residual, int64_t residual_stride_t, void* out,

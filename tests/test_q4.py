@@ -197,6 +197,17 @@ def test_linear_refusals(q4):
         q4.quantize_weight(torch.zeros(16, 64, dtype=BF16))
 
 
+def test_linear_refuses_more_tokens_than_its_grid_holds(q4, lib):
+    """Above 65535 tiles of 256, and where the count would not fit the entry's 32 bits."""
+    w = torch.zeros(1, 1, 1088, dtype=U8)
+    for T in (65535 * 256 + 1, 2 ** 31 + 5, 2 ** 32 + 3):
+        with pytest.raises(ValueError, match='at most 16776960 tokens'):
+            q4.linear(torch.zeros(1, 32, dtype=BF16).expand(T, 32), w, 16, 1.0)
+    base = dict(x=A16, st=2048, w=A16, T=65535 * 256 + 1, N=64, K=2048, scale=1.0, res=None, r_st=0, out=A16, o_st=64,
+                stream=None)
+    refused(lib, 'hla_s6_linear_q4', base, [(dict(), 'at most 16776960 tokens')])
+
+
 def test_linear_takes_an_error_word(q4, lib):
     """The kernels' bounded waits have somewhere to report to: ``linear``, ``Weight.linear`` and the C entry behind them."""
     x, w = torch.zeros(3, 160, dtype=BF16), torch.zeros(2, 2, 1088, dtype=U8)
