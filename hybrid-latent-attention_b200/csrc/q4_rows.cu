@@ -68,7 +68,7 @@ struct Q4CommitArgs {
 // W / 16 threads per row; thread k holds columns 8k .. and W/2 + 8k .. of both halves, i.e. whole RoPE
 // pairs and quarters of groups, so the amax of a group is two shuffles.
 constexpr int kQ4CommitThreads = 128;
-constexpr int kQ4CommitRounds = 4;  // rows of a thread group, one after the other, with many tokens
+constexpr int kQ4CommitRounds = 4;  // rows of a thread group, one after the other, with many tokens (rule at the launch)
 template <int W>
 __global__ void __launch_bounds__(kQ4CommitThreads) q4_commit_kernel(const Q4CommitArgs a) {
   constexpr int PER = W / 16;
@@ -185,7 +185,9 @@ __device__ __forceinline__ uint4 q4_values(uint32_t w, uint32_t scale, float ts,
 // PER = W / (8 OCT) threads per row: thread k takes octets k, k + PER .. of the K and of the V half.  With one octet a
 // thread a row's look-up and the tensor scale in fp32 made 12 instructions a value, which bound it (32768 rows of width
 // 512: 17 us; 14.4 with four octets and the scale folded, 85 MB at 5.9 TB/s).  Few rows keep one octet a thread: they
-// need the threads (77 rows of width 256: 1.6 us, 2.2 with four).
+// need the threads (77 rows of width 256: 1.6 us, 2.2 with four).  At 4096 rows the two take the same time at every width
+// (one and four octets: 2.65 and 2.60 us, 3.36 and 3.27, 4.87 and 4.98 for 256, 512 and 1024; at 16384 4.7 and 4.5, 7.4
+// and 6.9, 16.9 and 14.0).
 template <int W, int OCT>
 __global__ void __launch_bounds__(256) q4_gather_kernel(const Q4GatherArgs a) {
   constexpr int PER = W / (8 * OCT);
@@ -323,9 +325,11 @@ int hla_s6_commit_rows_q4(const void* row, int64_t row_stride_t, int32_t width, 
   a.k_ts = k_scale;
   a.v_ts = v_scale;
   a.slot_out = slot_out;
-  // rounds only once every SM has its CTAs without them (their rows are then in flight together)
+  // Rounds from 12 CTAs without them per SM on, at each width (without and with them: 256 wide 9472 rows 6.7 and 7.0 us,
+  // 18944 rows 10.3 and 9.0, 75776 37.1 and 29.4; 512 wide 4736 6.9 and 7.3, 9472 10.4 and 9.3, 37888 37.5 and 30.4; 1024
+  // wide 4736 10.6 and 9.4, 37888 74 and 57).
   int rows = kQ4CommitThreads / (width / 16);
-  a.rounds = num_tokens >= rows * kQ4CommitRounds * 148 * 8 ? kQ4CommitRounds : 1;
+  a.rounds = num_tokens >= rows * 148 * 12 ? kQ4CommitRounds : 1;
   rows *= a.rounds;
   const int grid = (num_tokens + rows - 1) / rows;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
