@@ -632,13 +632,19 @@ int hla_s6_linear_q4_checked(const void* x, int64_t x_stride_t, const void* pack
   // Few tokens: tiles of 16 outputs x 8 tokens.  One token tile: two row tiles a CTA once there are enough CTAs (1 x 2048
   // -> 12288 5.0 us instead of 5.3; -> 6144 4.7 instead of 4.3).
   if (num_tokens <= 8) return out_features >= 8192 ? launch_few<1, 2>(p, s) : launch_few<1, 1>(p, s);
-  // Then two token tiles share a row tile's codes, or four two row tiles' from 900 tiles on (48 tokens x 2048 -> 2048,
-  // 768 tiles: 6.5 and 6.4 us; 64, 1024 tiles: 8.0 and 6.5; 64 x 2048 -> 512, 256 tiles: 3.8 and 6.3).  From 32 tokens
-  // and 1280 tiles on the kernel for many tokens is as fast (32 x 2048 -> 6144: 11.2 and 11.2 us; 48: 14.4 and 11.3;
-  // 64 x 2048 -> 2048: 6.5 and 7.0); with fewer tokens it is not (24 x 2048 -> 49152: 54 and 78).
+  // Then two token tiles share a row tile's codes; up to 64 tokens, from 768 tiles on (3 CTAs of two tiles per SM), four
+  // share two row tiles' while their CTAs still run at once.  Two by one, four by two and the kernel for many tokens:
+  //   48 x 2048 -> 2048 (768 tiles) 6.5, 6.4 us; 64 x 2048 -> 512 (256) 3.8, 6.3; 64 x 2048 -> 2048 (1024) 8.2, 7.0, 7.5
+  //   32 x 2048 -> 3616 (904, 113 CTAs) 8.2, 7.1, 9.2; -> 5120 (1280, 160 CTAs) 9.9, 11.6, 12.0
+  //   64 x 2048 -> 2560 (1280, 160 CTAs) 10.0, 11.7, 9.4; 48 x 2048 -> 2560 (960, 160) 8.2, 9.5, 9.1; -> 3392 (1272, 212)
+  //   10.1, 10.6, 9.2
+  // with fewer than 32 tokens 24 x 2048 -> 49152 54, -, 78.  K moves them alike: 64 x 512 -> 2048 4.5, 3.9, 6.2 and 4096
+  // -> 2048 13.1, 10.0, 9.7; 48 x 512 -> 3392 4.9, 5.7, 6.0 and 4096 -> 3392 16.1, 15.7, 13.4.
   const int64_t few = static_cast<int64_t>((out_features + 15) / 16) * ((num_tokens + 7) / 8);
-  if (num_tokens < 32 || (num_tokens <= kQ4FewTokens && few <= 900)) return launch_few<2, 1>(p, s);
-  if (num_tokens <= kQ4FewTokens && few <= 1280) return launch_few<4, 2>(p, s);
+  const int64_t four = static_cast<int64_t>((out_features + 31) / 32) * ((num_tokens + 31) / 32);  // CTAs of four by two
+  if (num_tokens < 32) return launch_few<2, 1>(p, s);
+  if (num_tokens <= kQ4FewTokens && few >= 768 && four <= 148) return launch_few<4, 2>(p, s);
+  if (num_tokens <= kQ4FewTokens && few <= 1280) return launch_few<2, 1>(p, s);
   // More tiles of 128 tokens x 64 outputs than SMs: the large tiles, which take the same time however few there are
   // (512 x 2048 -> 2048, 128 of the small ones: 15.0 us with the large, 13.0 with the small; 256 x 2048 -> 6144, 192:
   // 15.4 and 18.7)
