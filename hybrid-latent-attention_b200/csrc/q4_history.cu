@@ -4,7 +4,7 @@
 // (slot = CTA + row, slot ranges in meta) in the same workspace, so the reduces and the fused combine of
 // history.cu / combine.cu follow it unchanged.
 //
-// What bounds it.  A row of 512-wide latents is 544 bytes and 32768 multiply-adds for 16 heads: 60 flop per
+// What bounds it.  A row of 512-wide latents is 544 bytes and 16384 multiply-adds for 16 heads: 60 flop per
 // byte, four times the bf16 reader's.  mma.sync runs at 1024 multiply-adds per clock and SM here (8 clocks of
 // issue per m16n8k16 and scheduler, measured), which alone is 0.7 of the time HBM gives a row; the codes also
 // have to become f16 values, two per register, at about 11 instructions per word of 8.  A first version on
@@ -28,14 +28,16 @@
 //   warp 26, 27 bulk copies of the tiles' K and V halves into a ring each, of 5 units of 17408 bytes (2, 4 or 8 tiles):
 //               K is used a step or more before V, and in one ring of whole tiles its units waited for that.
 // Code size is what costs most after the arithmetic: the warps of a scheduler run different roles, whose loops share
-// its instruction caches.  The dequantising loops are kept rolled (unrolled over a step 190 us with one group of each,
-// 137 rolled with a softmax group; K by two chunks 99 instead of 91), and so are the issuing ones but for the MMAs of
-// one chunk (91 -> 85).
+// its instruction caches.  So the loops over chunks, tiles and steps are rolled and the short ones inside unrolled (64
+// requests of 8160 rows, 79 us as it is: K chunks unrolled 99, V tiles unrolled 94, V octets rolled 86, K halves rolled
+// 82, the issuing loops unrolled 5 more).
 //
-// Measured: 64 requests of 8160 rows, width 512: 79 us (3.6 TB/s, 215 TFLOP/s; the bytes alone 44); 4 of 65501: 45 us
-// (22); 37 of 0 to 16384, width 256: 27 us.  A step of 128 rows takes 5200 clocks and 14000 warp instructions; the
-// hand-over between the roles (waits, barriers, instruction fetch) bounds it as much as the arithmetic.  Without a
-// gain: two CTAs of 13 warps (112 us), all on mma.sync (118).
+// Measured: 64 requests of 8160 rows, width 512: 79.5 us (3.6 TB/s, 215 TFLOP/s; the bytes alone 43.6); 4 of 65501: 45.5
+// us (21.7); 37 of 0 to 16384, width 256: 27.4 us.  A step of 128 rows takes 5200 clocks, its bytes 2980.  It is 14000
+// warp instructions, 3500 a scheduler: their issue alone is 1.17 times the bytes.  5600 of them dequantise (11 for each of
+// the 16384 words of a step, 32 words a warp); the rest is softmax, tensor-memory and shared-memory traffic, addresses
+// and waits, and the other 1700 clocks are hand-overs between the roles that nothing covers.  Slower: two CTAs of 13
+// warps per SM (112 us), all on mma.sync (118).
 // f16 instead of bf16 because its 10-bit mantissa takes a nibble at either of two places (q4.cuh): both operands
 // of an MMA have one type, so q is scaled by a power of two per head into f16's range (exact but for elements
 // 2^-26 below the head's largest, whose error is 2^-37 of it), and p is carried as 2^11 p <= 2^15, rounded to 11
@@ -77,7 +79,7 @@ struct Q4Cfg {
   static constexpr int UT = 2048 / W;            // tiles per ring unit
   static constexpr int UNIT = UT * HALF;         // 17408
   static constexpr int UNITS = 5;
-  // tiles per V chunk (width 512: with the rings apart 85.6, 80.3 and 79.4 us at 1, 2 and 4)
+  // tiles per V chunk (width 512, 64 x 8160 rows: 85.6, 80.3 and 79.4 us at 1, 2 and 4)
   static constexpr int VT = W == 256 ? 2 : W == 512 ? 4 : 1;
   static constexpr int VCOLS = NB * VT * 8;      // its tensor-memory columns
   static constexpr int KB = 2;                   // K chunks in tensor memory (4 at width 256: no faster)
@@ -146,7 +148,7 @@ __device__ __forceinline__ bool named_bar_or(int id, int threads, bool pred) {
 // The partition over the CTAs (stream mode) counts half steps: a row costs 2 a step of 128 rows and 1 for what its
 // segment takes to begin and end, and is only cut between steps (a cut one costs its CTAs a step each).  Cut at pages
 // and without that 1, short rows piled up in a CTA, up to 5 segments and 8 steps where 5 were due (37 rows of 0 to
-// 16384, width 256: 35 -> 29 us; 64 rows of 8160, width 512: 102 -> 97).
+// 16384, width 256: 35 us against 29; 64 rows of 8160, width 512: 102 against 97, both on a form before this one).
 __device__ __forceinline__ int q4_cost(int ctx) { return ctx > 0 ? 2 * ((ctx - 1) / 128 + 1) + 1 : 0; }
 // The step at cost x of a row: a CTA that starts there begins with it, one that ends there ends before it.
 __device__ __forceinline__ int q4_step_at(int x) { return x > 0 ? (x - 1) >> 1 : 0; }
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(kQ4HistThreads, 1) q4_history_kernel(const Q4H
     const Q4Tile tl(W);
     const int codes_at = is_v ? tl.v_codes(0, 0) : 0, scales_at = is_v ? tl.v_scale(0, 0) : tl.k_scale(0, 0);
     // The lanes look up 32 tiles at once: a lookup per unit, when its slot was free, kept this warp busy for longer
-    // than the others took to use the unit up (64 x 8160 rows, then in one ring: 95 -> 91 us).
+    // than the others took to use the unit up (64 x 8160 rows, on a form with one ring: 95 us against 91).
     int unit = 0;
     while (st.next()) {
       for (int b = st.tile; b < st.tend; b += 32) {

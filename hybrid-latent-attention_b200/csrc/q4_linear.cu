@@ -12,7 +12,7 @@
 // q4_linear_wide: with enough tiles the products bound it, and shared memory their operands: with x and 256 outputs'
 // weights there an SM moves 96 KB for 512 clocks of products (28 us for 4096 x 2048 -> 1024).  So the weights are the
 // A operand in tensor memory, 128 outputs, written there by the dequantising warps, and 256 tokens of x the B operand:
-// 64 KB per 512 clocks, half of the dequantisation, 550 clocks a stage (16.2 us; 1059 TFLOP/s).  What is left is
+// 64 KB per 512 clocks, half of the dequantisation, 550 clocks a stage (15.8 us; 1090 TFLOP/s).  What is left is
 // mostly the start and the output of the one tile a CTA has (about 5.7 us).
 //
 // None has a workspace or a second launch.
@@ -639,7 +639,8 @@ int hla_s6_linear_q4_checked(const void* x, int64_t x_stride_t, const void* pack
   //   64 x 2048 -> 2560 (1280, 160 CTAs) 10.0, 11.7, 9.4; 48 x 2048 -> 2560 (960, 160) 8.2, 9.5, 9.1; -> 3392 (1272, 212)
   //   10.1, 10.6, 9.2
   // with fewer than 32 tokens 24 x 2048 -> 49152 54, -, 78.  K moves them alike: 64 x 512 -> 2048 4.5, 3.9, 6.2 and 4096
-  // -> 2048 13.1, 10.0, 9.7; 48 x 512 -> 3392 4.9, 5.7, 6.0 and 4096 -> 3392 16.1, 15.7, 13.4.
+  // -> 2048 13.1, 10.0, 9.7; 48 x 512 -> 3392 4.9, 5.7, 6.0 and 4096 -> 3392 16.1, 15.7, 13.4.  (About 1280 tiles the
+  // third is the quicker for long K and 48 tokens or more, the first by more for short K or 32.)
   const int64_t few = static_cast<int64_t>((out_features + 15) / 16) * ((num_tokens + 7) / 8);
   const int64_t four = static_cast<int64_t>((out_features + 31) / 32) * ((num_tokens + 31) / 32);  // CTAs of four by two
   if (num_tokens < 32) return launch_few<2, 1>(p, s);

@@ -39,7 +39,8 @@ class LatentLayer(nn.Module):
     def pack_writers(self):
         """From now on ``s6_layer.write_rows`` runs on 4-bit copies of the writers' weights (``packed_writers``, by
         loop), made here (on CUDA, bf16).  ``writer`` and the state dict stay as they are; a copy moves with the
-        module but is not made again when its parameter changes."""
+        module but is not made again when its parameter changes.  (The native engines, ``decode.S6DecodeModel`` and
+        ``prefill.PrefillWriter``, run the bf16 weights whether or not there are copies.)"""
         self.packed_writers = [q4.Weight.of(w.weight.detach()) for w in (self.cand1, *self.cand_s)]
 
     def _apply(self, fn, recurse=True):

@@ -442,3 +442,17 @@ def test_partials_go_into_the_exchange_and_the_combine(width, parts):
             assert (got[s['R']:] == 0).all()
             np.testing.assert_allclose(got, want, **O_TOL)
     assert int(run.err.item()) == 0 and (run.epochs == 2).all()
+
+
+def test_commit_with_more_requests_than_fit_shared_memory():
+    """1100 requests of one token, some padding: the kernel searches the request list in global memory."""
+    q4 = pkg('q4')
+    W = 256
+    c = commit_setup([1, 0, 2] * 367, W, 16, seed=6, padding=3, start=[i % 50 for i in range(1101)])
+    cache = q4.new_cache(c['nb'], 16, W)
+    slots = q4.commit_rows(dev(c['row'], BF16), dev(c['pos']), dev(c['table'], BF16), cache, dev(c['bt']), dev(c['qsl']))
+    assert np.array_equal(slots.cpu().numpy(), c['slots'])
+    real = c['slots'] >= 0
+    rotated = ref.rope(c['row'][:, :W], c['table'], c['pos'])
+    want = np.concatenate((ref.stored(rotated, 1.0), ref.stored(c['row'][:, W:], 1.0)), 1)
+    assert np.array_equal(q4.gather_slots(cache, slots).double().cpu().numpy()[real], want[real])
